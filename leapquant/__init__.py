@@ -8,11 +8,11 @@
 import sys
 
 import leapquant_amd
-from leapquant_amd import kernels, state, vllm
+from leapquant_amd import kernels, seq, state, vllm
 from leapquant_amd.vllm import gdn as _gdn, glm as _glm
 
 __version__ = leapquant_amd.__version__
 
-for _name, _mod in (("kernels", kernels), ("state", state), ("vllm", vllm), ("vllm.gdn", _gdn), ("vllm.glm", _glm)):
+for _name, _mod in (("kernels", kernels), ("state", state), ("seq", seq), ("vllm", vllm), ("vllm.gdn", _gdn), ("vllm.glm", _glm)):
     sys.modules[__name__ + "." + _name] = _mod
 del _name, _mod

@@ -1,10 +1,11 @@
-"""ctypes binding of liblq.so (include/lq.h).  The product path has no fallback: if the library is missing or a call
-fails, this raises."""
+"""ctypes binding of liblq.so (include/lq.h) and liblq_seq.so (include/lq_seq.h).  The product path has no fallback: if a
+library is missing or a call fails, this raises."""
 import ctypes
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_build", "liblq.so")
+SEQ_LIB_PATH = os.path.join(_HERE, "_build", "liblq_seq.so")
 ABI_VERSION = 6
 SCHED_INTS = 512           # include/lq.h: LQ_SCHED_INTS
 
@@ -26,6 +27,24 @@ class LqStepIO(ctypes.Structure):
 class LqConv(ctypes.Structure):
     _fields_ = [("state", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("slot_stride", c_ll),
                 ("ch_stride", c_ll), ("tap_stride", c_ll), ("W", c_int), ("silu", c_int), ("NS", c_int)]
+
+
+class LqSeqs(ctypes.Structure):
+    _fields_ = [("loc", c_void_p), ("idx", c_void_p), ("src", c_void_p), ("N", c_int), ("T", c_int)]
+
+
+class LqDelta(ctypes.Structure):
+    _fields_ = [("S", c_void_p), ("slot_stride", c_ll)] + [(n, c_int) for n in ("NS", "HV", "H", "K", "V")] + \
+               [(n, c_void_p) for n in ("mixed", "a", "b", "A_log", "dt_bias", "out")] + \
+               [(n, c_ll) for n in ("mixed_ld", "a_ld", "b_ld")] + \
+               [("scale", c_float), ("gate_bf16", c_int), ("kda", c_int), ("glb", c_float)]
+
+
+class LqNorm(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("x", "z", "weight", "res", "out")] + \
+               [(n, c_ll) for n in ("x_ld", "x_hd", "z_ld", "z_hd", "o_ld", "o_hd")] + \
+               [(n, c_int) for n in ("rows", "heads", "D")] + [(n, c_float) for n in ("eps", "scale", "offset")] + \
+               [("act", c_int), ("weight_bf16", c_int)]
 
 
 # exported symbol -> (restype, argtypes); must match include/lq.h
@@ -52,24 +71,48 @@ SIGNATURES = {
                                   c_void_p]),
 }
 
+# the same of include/lq_seq.h
+SEQ_SIGNATURES = {
+    "lq_delta_steps": (c_int, [ctypes.POINTER(LqDelta), ctypes.POINTER(LqSeqs), c_void_p]),
+    "lq_delta_prefill": (c_int, [ctypes.POINTER(LqDelta), ctypes.POINTER(LqSeqs), c_void_p, c_ll, c_void_p]),
+    "lq_delta_workspace": (c_ll, [ctypes.POINTER(LqDelta), ctypes.POINTER(LqSeqs)]),
+    "lq_conv_seq": (c_int, [ctypes.POINTER(LqConv), ctypes.POINTER(LqSeqs), c_void_p, c_ll, c_void_p, c_int, c_void_p]),
+    "lq_gated_norm": (c_int, [ctypes.POINTER(LqNorm), c_void_p]),
+    "lq_add_norm": (c_int, [ctypes.POINTER(LqNorm), c_void_p]),
+}
+
 _LIB = [None]
+_SEQ_LIB = [None]
+
+
+def _load(path, signatures):
+    if not os.path.exists(path):
+        raise RuntimeError("%s is missing (%s): build it with `python -m leapquant_amd.build`"
+                           % (os.path.basename(path), path))
+    L = ctypes.CDLL(path)
+    for name, (res, args) in signatures.items():
+        f = getattr(L, name)
+        f.restype = res
+        f.argtypes = args
+    return L
 
 
 def lib():
     """The loaded liblq.so (raises if it has not been built)."""
     if _LIB[0] is None:
-        if not os.path.exists(LIB_PATH):
-            raise RuntimeError("liblq.so is missing (%s): build it with `python -m leapquant_amd.build`" % LIB_PATH)
-        L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
-            f = getattr(L, name)
-            f.restype = res
-            f.argtypes = args
+        L = _load(LIB_PATH, SIGNATURES)
         v = L.lq_abi_version()
         if v != ABI_VERSION:
             raise RuntimeError("liblq.so ABI %d, expected %d: rebuild it" % (v, ABI_VERSION))
         _LIB[0] = L
     return _LIB[0]
+
+
+def seq_lib():
+    """The loaded liblq_seq.so (raises if it has not been built)."""
+    if _SEQ_LIB[0] is None:
+        _SEQ_LIB[0] = _load(SEQ_LIB_PATH, SEQ_SIGNATURES)
+    return _SEQ_LIB[0]
 
 
 _ERR = {-1: "bad argument (unsupported shape / size / pointer)", -2: "HIP launch error",

@@ -1,7 +1,8 @@
-"""Builds liblq.so (the HIP kernels + C ABI of include/lq.h) in-tree for gfx950, and liblq_probe.so (a streaming-read
-probe that bench.py times as the memory system's ceiling; not part of the API).
+"""Builds liblq.so (the HIP kernels + C ABI of include/lq.h) in-tree for gfx950, liblq_seq.so (the operators on whole
+sequences, include/lq_seq.h), and liblq_probe.so (a streaming-read probe that bench.py times as the memory system's ceiling;
+not part of the API).
 
-    python -m leapquant_amd.build          # -> leapquant_amd/_build/liblq.so, liblq_probe.so
+    python -m leapquant_amd.build          # -> leapquant_amd/_build/liblq.so, liblq_seq.so, liblq_probe.so
 
 hipcc cross-compiles without a GPU.  Every HIP file gets `-Xclang -target-feature -Xclang -packed-fp32-ops` (no
 packed FP32 instructions in the device code).
@@ -16,6 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "_build")
 LIB = os.path.join(OUT, "liblq.so")
 SOURCES = ("lq_step.hip", "lq_step_bf16.hip", "lq_flush.hip", "lq_dequant.hip", "lq_dense.hip", "lq_noalloc.hip")
+SEQ_LIB = os.path.join(OUT, "liblq_seq.so")
+SEQ_SOURCES = ("lq_seq_conv.hip", "lq_seq_norm.hip", "lq_seq_steps.hip", "lq_seq_delta.hip")
 PROBE_LIB = os.path.join(OUT, "liblq_probe.so")
 PROBE_SOURCES = ("lq_probe.hip",)
 ARCH = os.environ.get("LQ_OFFLOAD_ARCH", "gfx950")
@@ -64,6 +67,7 @@ def build(verbose=False):
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
     _compile_link(cc, flags, SOURCES, LIB, verbose)
+    _compile_link(cc, flags, SEQ_SOURCES, SEQ_LIB, verbose)
     _compile_link(cc, flags, PROBE_SOURCES, PROBE_LIB, verbose)
     return LIB
 
