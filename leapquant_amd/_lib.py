@@ -2,6 +2,7 @@
 library is missing or a call fails, this raises."""
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_build", "liblq.so")
@@ -71,15 +72,20 @@ SIGNATURES = {
                                   c_void_p]),
 }
 
-# the same of include/lq_seq.h
+# the same of include/lq_seq.h; the structures go as addresses, so that a caller may hand over their bytes (PACK_*), which a
+# call from Python builds in a quarter of a structure's time
 SEQ_SIGNATURES = {
-    "lq_delta_steps": (c_int, [ctypes.POINTER(LqDelta), ctypes.POINTER(LqSeqs), c_void_p]),
-    "lq_delta_prefill": (c_int, [ctypes.POINTER(LqDelta), ctypes.POINTER(LqSeqs), c_void_p, c_ll, c_void_p]),
-    "lq_delta_workspace": (c_ll, [ctypes.POINTER(LqDelta), ctypes.POINTER(LqSeqs)]),
-    "lq_conv_seq": (c_int, [ctypes.POINTER(LqConv), ctypes.POINTER(LqSeqs), c_void_p, c_ll, c_void_p, c_int, c_void_p]),
-    "lq_gated_norm": (c_int, [ctypes.POINTER(LqNorm), c_void_p]),
-    "lq_add_norm": (c_int, [ctypes.POINTER(LqNorm), c_void_p]),
+    "lq_delta_steps": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "lq_delta_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p]),
+    "lq_delta_workspace": (c_ll, [c_void_p, c_void_p]),
+    "lq_conv_seq": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
+    "lq_gated_norm": (c_int, [c_void_p, c_void_p]),
+    "lq_add_norm": (c_int, [c_void_p, c_void_p]),
 }
+_SEQS, _DELTA, _NORM = struct.Struct("@3P2i0P"), struct.Struct("@Pq5i6P3qf2if0P"), struct.Struct("@5P6q3i3f2i0P")
+for _layout, _type in ((_SEQS, LqSeqs), (_DELTA, LqDelta), (_NORM, LqNorm)):
+    assert _layout.size == ctypes.sizeof(_type)
+pack_seqs, pack_delta, pack_norm = _SEQS.pack, _DELTA.pack, _NORM.pack
 
 _LIB = [None]
 _SEQ_LIB = [None]

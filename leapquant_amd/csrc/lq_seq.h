@@ -3,6 +3,11 @@
 #include "../../include/lq_seq.h"
 #include "lq_common.h"
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__attribute__((visibility("hidden"))) int lq_seq_cus();      // compute units of the current GPU
+
 struct SeqRun {      // a run of a sequence's tokens, as its workgroup finds it
   int n, j;          // sequence, run of it
   int lo, hi;        // the sequence's packed tokens
@@ -13,19 +18,25 @@ __device__ __forceinline__ int seq_at(const lq_seqs& s, int n) { return min(max(
 
 // Runs of RUN tokens of a ragged batch, numbered without a scan over the batch: run j of sequence n has the number
 // loc[n] / RUN + n + j.  Sequence n owns loc[n+1] / RUN - loc[n] / RUN + 1 numbers, which is at least its ceil(len / RUN)
-// runs and at least one; the numbers left over find j past the end.  The batch has T / RUN + N of them.
+// runs and at least one; the numbers left over, and those before the first sequence, find an empty run past the end.  The
+// batch has T / RUN + N of them.  A whole wave looks for its run at once, 64 sequences a step: one load up to 64 of them.
 template <int RUN>
 __device__ __forceinline__ SeqRun seq_run(const lq_seqs& s, int number) {
-  int a = 0, b = s.N - 1;                        // the last n whose first number is not above `number`
-  while (a < b) {
-    const int m = (a + b + 1) >> 1;
-    if (seq_at(s, m) / RUN + m <= number) a = m; else b = m - 1;
+  const int lane = threadIdx.x & 63;
+  int a = 0, len = s.N;                          // the last n of a .. a + len - 1 whose first number is not above `number`
+  while (len > 1) {
+    const int step = (len + 63) >> 6, m = a + lane * step;
+    const bool below = lane * step < len && seq_at(s, m) / RUN + m <= number;
+    const int at = max((int)__popcll(__ballot(below)) - 1, 0) * step;     // the count is unsigned
+    a += at;
+    len = min(step, len - at);
   }
   SeqRun r;
   r.n = a;
   r.lo = seq_at(s, a);
   r.hi = max(r.lo, seq_at(s, a + 1));
   r.j = number - (r.lo / RUN + a);
+  if (r.j < 0 || r.j > s.T / RUN) { r.j = 1; r.lo = r.hi; }
   return r;
 }
 template <int RUN>
@@ -47,3 +58,16 @@ __device__ __forceinline__ float gate_param(const void* p, int bf16, long long i
 }
 // e^x and 1 / (1 + e^-x) from the hardware's exp2 and reciprocal (1 ulp each): for results that are rounded to bf16
 __device__ __forceinline__ float fast_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+// e^x, the argument's product with log2 e carried in two parts (a few 1e-7 for any x; __expf loses |x| 1e-7)
+__device__ __forceinline__ float exp_f(float x) {
+  const float t = x * 1.44269504f, r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fabsf(t) < 150.f ? e * fmaf(r, 0.693147181f, 1.0f) : e;             // zero, infinity and NaN as they are
+}
+// log(1 + e^x), x above the threshold itself; log(1 + u) as log(w) u / (w - 1), w = 1 + u, which has w's rounding cancel
+__device__ __forceinline__ float softplus_f(float x) {
+  const float u = exp_f(fminf(x, (float)LQ_SOFTPLUS_THRESHOLD)), w = 1.0f + u, d = w - 1.0f;
+  const float y = __builtin_amdgcn_logf(w) * 0.693147181f * u * __builtin_amdgcn_rcpf(d);
+  const float z = d == 0.f ? u : y;
+  return x <= (float)LQ_SOFTPLUS_THRESHOLD ? z : x;
+}

@@ -1,28 +1,37 @@
 // Depthwise causal conv1d over a ragged batch (lq_conv_seq): y_t = act(w0 x_{t-3} + w1 x_{t-2} + w2 x_{t-1} + w3 x_t + bias).
 //
 // Reads 2 and writes 2 bytes an element; ~11 vector instructions an element keep it bound by memory.  A thread owns VEC
-// neighbouring channels of a run of RUN tokens of one sequence and carries the last three inputs in registers, so each
-// input is requested once and the three before the run once more.
+// neighbouring channels of a run of RUN tokens of one sequence: all of the run's loads are in flight before its arithmetic,
+// the three inputs before the run are requested once more (out of a cache), and the last three move through registers.
 // The workgroup of a sequence's first run also moves its taps: it reads them before it writes them, and no other
 // workgroup touches them, so a call can run in place.
+//
+// VEC = 8 where the call is large (WIDE): a workgroup's rows are then 4 KiB pieces, and 32768 tokens of 8192 channels take
+// 215 us (1.07 GB: 5.0 TB/s, a large copy's rate), against 276 us with VEC = 2.  VEC = 2 below: a thread moves 2 channels'
+// taps and not 8, and there are four times the waves: 64 tokens 4.5 us against 9.4, 333 tokens 6.4 against 10.8, 8000
+// tokens 66 against 70, which is about where they meet.  Small calls are bound by their chain of loads: the run's
+// sequence, its slots, the taps.
 #include "lq_seq.h"
 
 namespace {
 
-constexpr int RUN = 16;
+constexpr int RUN = 8;
+static_assert(RUN >= 3, "the three inputs before a later run belong to its own sequence");
+constexpr long long WIDE = 1ll << 27;            // elements of a call
 
-template <int VEC> struct Elems;
-template <> struct Elems<8> {
-  typedef uint4 raw;
-  static __device__ __forceinline__ void unpack(const uint4& u, float* f) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+template <int VEC> struct Elems {
+  typedef uint32_t raw __attribute__((ext_vector_type(VEC / 2)));
+  static __device__ __forceinline__ void unpack(const raw& u, float* f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); }
+    for (int i = 0; i < VEC / 2; ++i) { f[2 * i] = bf_lo(u[i]); f[2 * i + 1] = bf_hi(u[i]); }
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7]));
+  static __device__ __forceinline__ raw pack(const float* f) {
+    raw u;
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) u[i] = pk_bf16(f[2 * i], f[2 * i + 1]);
+    return u;
   }
-  static __device__ __forceinline__ uint4 zero() { return make_uint4(0, 0, 0, 0); }
+  static __device__ __forceinline__ raw zero() { return raw(0); }
 };
 template <> struct Elems<1> {
   typedef bf16_t raw;
@@ -41,33 +50,49 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(lq_conv cv, lq_seqs s, co
   if (n <= 0 && r.j > 0) return;
   const int c = (blockIdx.y * 256 + threadIdx.x) * VEC;
   if (c >= C) return;
-  const int dst = seq_dst(s, r.n, cv.NS), src = seq_src(s, r.n, cv.NS);
-  if (dst == 0) {
-    for (int i = 0; i < n; ++i) *(raw_t*)(out + (long long)(t0 + i) * C + c) = E::zero();
-    return;
-  }
   const bf16_t* p = x + (long long)t0 * ld + c;
+  raw_t u[RUN];                                  // all loads of the run in flight before its arithmetic
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) u[i] = *(const raw_t*)(p + (long long)min(i, n - 1) * ld);
+  }
+  float w[4][VEC], b[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const uint2 v = ((const uint2*)cv.weight)[c + e];
+    w[0][e] = bf_lo(v.x); w[1][e] = bf_hi(v.x); w[2][e] = bf_lo(v.y); w[3][e] = bf_hi(v.y);
+    b[e] = cv.bias ? bf2f(((const bf16_t*)cv.bias)[c + e]) : 0.f;
+  }
+  const int dst = seq_dst(s, r.n, cv.NS), src = seq_src(s, r.n, cv.NS);
   float h[3][VEC];                               // the three inputs before the run, oldest first
   if (r.j == 0) {
-    bf16_t tap[3][VEC];
     const bf16_t* S = (const bf16_t*)cv.state + (long long)src * cv.slot_stride + (long long)c * cv.ch_stride;
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        tap[i][e] = src ? S[e * cv.ch_stride + i * cv.tap_stride] : (bf16_t)0;
-        h[i][e] = bf2f(tap[i][e]);
+    for (int e = 0; e < VEC; ++e) {
+      h[0][e] = h[1][e] = h[2][e] = 0.f;
+      if (src) {
+        const bf16_t* f = S + e * cv.ch_stride;
+        h[0][e] = bf2f(f[0]); h[1][e] = bf2f(f[cv.tap_stride]); h[2][e] = bf2f(f[2 * cv.tap_stride]);
       }
-    const int len = r.hi - r.lo;                 // the last three inputs: of the sequence, and of the taps where it is short
-    bf16_t* D = (bf16_t*)cv.state + (long long)dst * cv.slot_stride + (long long)c * cv.ch_stride;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const int at = len - 3 + i;                // -3 + i .. : a tap where negative
+    }
+    if (dst) {                                   // the last three inputs: of the sequence, and of the taps where it is short
+      const int len = r.hi - r.lo;
+      bf16_t* D = (bf16_t*)cv.state + (long long)dst * cv.slot_stride + (long long)c * cv.ch_stride;
+      const bf16_t* last = p + (long long)(len - 3) * ld;
+      float f[3][VEC] = {};
+      if (len >= 3) E::unpack(*(const raw_t*)last, f[0]);
+      if (len >= 2) E::unpack(*(const raw_t*)(last + ld), f[1]);
+      if (len >= 1) E::unpack(*(const raw_t*)(last + 2 * ld), f[2]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        bf16_t v = at == -3 ? tap[0][e] : at == -2 ? tap[1][e] : tap[2][e];
-        if (at >= 0) v = p[(long long)at * ld + e];
-        D[e * cv.ch_stride + i * cv.tap_stride] = v;
+        const float a0 = h[0][e], a1 = h[1][e], a2 = h[2][e];
+        const float f0 = len >= 3 ? f[0][e] : len == 2 ? a2 : len == 1 ? a1 : a0;
+        const float f1 = len >= 2 ? f[1][e] : len == 1 ? a2 : a1;
+        const float f2 = len >= 1 ? f[2][e] : a2;
+        bf16_t* to = D + e * cv.ch_stride;
+        to[0] = (bf16_t)(__float_as_uint(f0) >> 16);
+        to[cv.tap_stride] = (bf16_t)(__float_as_uint(f1) >> 16);
+        to[2 * cv.tap_stride] = (bf16_t)(__float_as_uint(f2) >> 16);
       }
     }
     if (n <= 0) return;
@@ -75,35 +100,28 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(lq_conv cv, lq_seqs s, co
 #pragma unroll
     for (int i = 0; i < 3; ++i) E::unpack(*(const raw_t*)(p + (long long)(i - 3) * ld), h[i]);
   }
-  float w[4][VEC], b[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) {
-    const uint2 u = ((const uint2*)cv.weight)[c + e];
-    w[0][e] = bf_lo(u.x); w[1][e] = bf_hi(u.x); w[2][e] = bf_lo(u.y); w[3][e] = bf_hi(u.y);
-    b[e] = cv.bias ? bf2f(((const bf16_t*)cv.bias)[c + e]) : 0.f;
-  }
   bf16_t* o = out + (long long)t0 * C + c;
   const bool silu = cv.silu;
-  auto token = [&](const raw_t& u, int i) {
+#pragma unroll
+  for (int i = 0; i < RUN; ++i) {
     float f[VEC], y[VEC];
-    E::unpack(u, f);
+    E::unpack(u[i], f);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       y[e] = fmaf(w[3][e], f[e], fmaf(w[2][e], h[2][e], fmaf(w[1][e], h[1][e], fmaf(w[0][e], h[0][e], b[e]))));
       if (silu) y[e] *= fast_sigmoid(y[e]);
       h[0][e] = h[1][e]; h[1][e] = h[2][e]; h[2][e] = f[e];
     }
-    *(raw_t*)(o + (long long)i * C) = E::pack(y);
-  };
-  if (n == RUN) {                                // all loads of the run in flight before its arithmetic
-    raw_t u[RUN];
-#pragma unroll
-    for (int i = 0; i < RUN; ++i) u[i] = *(const raw_t*)(p + i * ld);
-#pragma unroll
-    for (int i = 0; i < RUN; ++i) token(u[i], i);
-  } else {
-    for (int i = 0; i < n; ++i) token(*(const raw_t*)(p + i * ld), i);
+    if (i < n) *(raw_t*)(o + (long long)i * C) = dst ? E::pack(y) : E::zero();
   }
+}
+
+template <int VEC>
+int launch(const lq_conv* cv, const lq_seqs* s, const void* x, long long x_ld, void* out, int C, hipStream_t st) {
+  const dim3 grid((unsigned)seq_runs<RUN>(s), (unsigned)((C + 256 * VEC - 1) / (256 * VEC)));
+  if (grid.y > 65535u) return LQ_ERR_ARG;
+  conv_seq_kernel<VEC><<<grid, 256, 0, st>>>(*cv, *s, (const bf16_t*)x, x_ld, (bf16_t*)out, C);
+  return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
 }
 
 }  // namespace
@@ -117,13 +135,10 @@ extern "C" int lq_conv_seq(const lq_conv* cv, const lq_seqs* s, const void* x, l
   if ((uintptr_t)cv->weight & 7) return LQ_ERR_ARG;
   if (s->N == 0) return LQ_OK;
   if (s->T > 0 && (!x || !out)) return LQ_ERR_ARG;
-  const bool wide = C % 8 == 0 && x_ld % 8 == 0 && (((uintptr_t)x | (uintptr_t)out) & 15) == 0;
-  const int per = 256 * (wide ? 8 : 1);
-  const dim3 grid((unsigned)seq_runs<RUN>(s), (unsigned)((C + per - 1) / per));
-  if (grid.y > 65535u) return LQ_ERR_ARG;
-  if (wide)
-    conv_seq_kernel<8><<<grid, 256, 0, (hipStream_t)stream>>>(*cv, *s, (const bf16_t*)x, x_ld, (bf16_t*)out, C);
-  else
-    conv_seq_kernel<1><<<grid, 256, 0, (hipStream_t)stream>>>(*cv, *s, (const bf16_t*)x, x_ld, (bf16_t*)out, C);
-  return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
+  const uintptr_t where = (uintptr_t)x | (uintptr_t)out;
+  hipStream_t st = (hipStream_t)stream;
+  if (C % 8 == 0 && x_ld % 8 == 0 && where % 16 == 0 && (long long)s->T * C >= WIDE)
+    return launch<8>(cv, s, x, x_ld, out, C, st);
+  if (C % 2 == 0 && x_ld % 2 == 0 && where % 4 == 0) return launch<2>(cv, s, x, x_ld, out, C, st);
+  return launch<1>(cv, s, x, x_ld, out, C, st);
 }

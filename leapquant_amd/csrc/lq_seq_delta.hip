@@ -26,7 +26,6 @@ __attribute__((visibility("hidden"))) int lq_check_delta(const lq_delta* d, cons
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
@@ -82,19 +81,6 @@ __device__ __forceinline__ void to_lds(const void* base, unsigned off, unsigned 
                : "memory", "m0");
 }
 #pragma clang diagnostic pop
-// e^x, the argument's product with log2 e carried in two parts (a few 1e-7 for any x; __expf loses |x| 1e-7)
-__device__ __forceinline__ float exp_f(float x) {
-  const float t = x * 1.44269504f, r = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-  const float e = __builtin_amdgcn_exp2f(t);
-  return fabsf(t) < 150.f ? e * fmaf(r, 0.693147181f, 1.0f) : e;             // zero, infinity and NaN as they are
-}
-// log(1 + e^x), x above the threshold itself; log(1 + u) as log(w) u / (w - 1), w = 1 + u, which has w's rounding cancel
-__device__ __forceinline__ float softplus_f(float x) {
-  const float u = exp_f(fminf(x, (float)LQ_SOFTPLUS_THRESHOLD)), w = 1.0f + u, d = w - 1.0f;
-  const float y = __builtin_amdgcn_logf(w) * 0.693147181f * u * __builtin_amdgcn_rcpf(d);
-  const float z = d == 0.f ? u : y;
-  return x <= (float)LQ_SOFTPLUS_THRESHOLD ? z : x;
-}
 template <int SHR> __device__ __forceinline__ double from_below(double x) {      // of lane l - SHR of the same 16, else 0
   const unsigned long long b = __builtin_bit_cast(unsigned long long, x);
   const unsigned lo = __builtin_amdgcn_mov_dpp((int)(unsigned)b, 0x110 + SHR, 0xf, 0xf, true);
@@ -355,6 +341,7 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
 // ---- the walk over a sequence's chunks -----------------------------------------------------------------------------------
 // Chunk c is requested in step c - 1 - AHEAD, has landed when step c - 1 begins, and meets the waves in the steps c - 1 (K in
 // K_c S_{c-1} and X), c (Q, V, T', c, ..) and c + 1 (K^T in the state's update, W, d, e^{G_C}).
+constexpr int AHEAD = 2;               // chunks requested before the step that first needs one
 constexpr int SERVICE = 4;             // service waves of a workgroup
 constexpr int ROLES = 4;               // waves of 16 rows of the state: chain, two halves of the channels, outputs
 struct Pass {                          // between the waves of 16 rows, of one step
@@ -363,35 +350,35 @@ struct Pass {                          // between the waves of 16 rows, of one s
 };
 constexpr int PASS = (int)sizeof(Pass) / 16;
 
-template <int K, int NW, int AHEAD>
+template <int K>
 struct Tiles {                         // places in LDS, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB;                    // blocks of a row of K, of a tile
-  static constexpr int VB = 2 * NW, VU = C * VB;                   // the same of the workgroup's columns of V
-  static constexpr int CU = (int)sizeof(Coef) / 16, CN = AHEAD > 1 ? 8 : (CU + 63) / 64;
+  static constexpr int VB = 2, VU = C * VB;                        // the same of the workgroup's columns of V
+  static constexpr int CU = (int)sizeof(Coef) / 16, CN = 8;
   static constexpr int KN = AHEAD + 3, QN = AHEAD + 2, VN = AHEAD + 2;
   static constexpr int QAT = KN * TU, VAT = QAT + QN * TU, CAT = VAT + VN * VU, XAT = CAT + KN * CN * 64;
-  static constexpr int PAT = XAT + 2 * 4 * 64, SAT = PAT + 2 * NW * PASS;          // what the waves pass on; scratch
+  static constexpr int PAT = XAT + 2 * 4 * 64, SAT = PAT + 2 * PASS;          // what the waves pass on; scratch
   static constexpr int END = SAT + SERVICE * 16 * 5, BYTES = 16 * END;
-  // loads of a service wave for a chunk (the same for each where AHEAD > 1: waves with no part of V or Coef of their own
-  // repeat another's, so that one count says what is still on its way)
-  static constexpr int LOADS = 2 * TU / 64 / SERVICE + (NW + SERVICE - 1) / SERVICE + (CN + SERVICE - 1) / SERVICE;
+  // loads of a service wave for a chunk, the same for each: all four load V, and Coef's last blocks more than once, so that
+  // one count says what is still on its way
+  static constexpr int LOADS = 2 * TU / 64 / SERVICE + 1 + CN / SERVICE;
+  static_assert(VU == 64 && CN * 64 >= CU && CN % SERVICE == 0, "loads of a chunk");
   static_assert(BYTES <= 160 * 1024, "LDS of a CU");
   static_assert(LOADS < 64, "what a wave may have outstanding");
 };
 
-template <int K, int V, int NW, int AHEAD>
+template <int K, int V>
 struct Walk {
-  typedef Tiles<K, NW, AHEAD> B;
+  typedef Tiles<K> B;
   static constexpr int KS = K / 32, RB = B::RB, TU = B::TU, VB = B::VB;
   const lq_delta& p;
   u32x4* lds;
   int lo, len, nc, hv, part;
 
   __device__ __forceinline__ const u32x4* ktile(int c) const { return lds + (unsigned)c % B::KN * TU; }
-  __device__ __forceinline__ const u32x4* qtile(int c) const { return lds + B::QAT + (unsigned)c % B::QN * TU; }
   __device__ __forceinline__ const Coef& coef(int c) const { return *(const Coef*)(lds + B::CAT + (unsigned)c % B::KN * B::CN * 64); }
   __device__ __forceinline__ bf16x8* xtile(int c) const { return (bf16x8*)(lds + B::XAT + (c & 1) * 256); }
-  __device__ __forceinline__ Pass& pass(int w, int c) const { return ((Pass*)(lds + B::PAT))[2 * w + (c & 1)]; }
+  __device__ __forceinline__ Pass& pass(int c) const { return ((Pass*)(lds + B::PAT))[c & 1]; }
 
   // the order of what comes before: N matrix instructions with M vector ones under each, and LDS reads among the first
   template <int N, int M> static __device__ __forceinline__ void under() {
@@ -409,7 +396,7 @@ struct Walk {
     const unsigned ld = 2u * (unsigned)p.mixed_ld, lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)(char*)lds;
     const char* rows = (const char*)p.mixed + (long long)lo * ld;
     const char *kb = rows + 2u * (p.H + hk) * K, *qb = rows + 2u * hk * K;
-    const char* vb = rows + 2u * (2 * p.H * K + hv * V + part * 16 * NW);
+    const char* vb = rows + 2u * (2 * p.H * K + hv * V + part * 16);
     const char* cb = (const char*)work;
     float(*m)[20] = (float(*)[20])(lds + B::SAT + 80 * k);
     const int xi = k >> 1, xe = k & 1;           // rows of this chunk, of the one before
@@ -427,15 +414,11 @@ struct Walk {
           to_lds(kb, off, ka + 1024u * at);
           to_lds(qb, off, qa + 1024u * at);
         }
+        to_lds(vb, (unsigned)min(l / VB, nv - 1) * ld + 16u * ((l % VB) ^ swz(l / VB, VB)), va);
 #pragma unroll
-        for (int i = 0; i < (NW + SERVICE - 1) / SERVICE; ++i) {
-          const int at = (SERVICE * i + k) % NW, u = l + 64 * at, r = u / VB, b = (u % VB) ^ swz(r, VB);
-          if (AHEAD > 1 || SERVICE * i + k < NW) to_lds(vb, (unsigned)min(r, nv - 1) * ld + 16u * b, va + 1024u * at);
-        }
-#pragma unroll
-        for (int i = 0; i < (B::CN + SERVICE - 1) / SERVICE; ++i) {
+        for (int i = 0; i < B::CN / SERVICE; ++i) {
           const int at = SERVICE * i + k;
-          if (at < B::CN) to_lds(cb, 16u * min(l + 64 * at, B::CU - 1), ca + 1024u * at);
+          to_lds(cb, 16u * min(l + 64 * at, B::CU - 1), ca + 1024u * at);
         }
         kb += (long long)C * ld; qb += (long long)C * ld; vb += (long long)C * ld;
         cb += (long long)p.HV * sizeof(Coef);
@@ -457,8 +440,8 @@ struct Walk {
         out[0] = first4(hi);
         out[128] = first4(lo);
       }
-      // what the next step needs has landed: with AHEAD = 2 this step's request may still be on its way
-      if (AHEAD > 1 && j < nc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(B::LOADS) : "memory");
+      // what the next step needs has landed; this step's request may still be on its way
+      if (j < nc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(B::LOADS) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (s < nc) end_step();
     }
@@ -467,10 +450,10 @@ struct Walk {
   // ---- a wave that keeps 16 rows of the state, half of their channels ----
   // S as result tiles of K^T U: lane (n, g) the row v = n, channels 32 x + 8 g .. + 7 in the registers (x, 0), (x, 1), which
   // are also the operand of K S and Q S.
-  __device__ __forceinline__ void state(int w, int half, int src, int dst) const {
+  __device__ __forceinline__ void state(int half, int src, int dst) const {
     constexpr int KH = KS / 2;
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4, qrow = 4 * g + (n >> 2);
-    const long long head = (long long)hv * V * K + (long long)((part * NW + w) * 16 + n) * K + 32 * KH * half + 8 * g;
+    const long long head = (long long)hv * V * K + (long long)(part * 16 + n) * K + 32 * KH * half + 8 * g;
     f32x4 S[KH][2] = {};
     if (src != 0) {
 #pragma unroll
@@ -492,8 +475,8 @@ struct Walk {
     auto step = [&](int t, bool update) {
       const lds_t ko = base + 16u * ((unsigned)(t - 1 + B::KN) % B::KN * TU), kn = base + 16u * ((unsigned)(t + 1) % B::KN * TU);
       const lds_t qt = base + 16u * (B::QAT + (unsigned)(t + B::QN) % B::QN * TU);
-      const Pass& in = pass(w, t + 1);
-      Pass& out = pass(w, t);
+      const Pass& in = pass(t + 1);
+      Pass& out = pass(t);
       const float next = t < 0 || t == nc ? 1.f : coef(t).last[0];
       bf16x8 uh, ul, kf[2][2], qf[2][2], sh[2], sl[2];
       auto fetch = [&](int x) {
@@ -581,13 +564,13 @@ struct Walk {
   }
 
   // ---- the wave that walks the chain R -> T' R -> R of these rows ----
-  __device__ __forceinline__ void chain(int w) const {
+  __device__ __forceinline__ void chain() const {
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4, qrow = 4 * g + (n >> 2);
     bf16x8 uh = {}, ul = {};
     auto step = [&](int t, bool first) {
       const Coef& ck = coef(t);
-      const Pass& in = pass(w, t + 1);
-      Pass& out = pass(w, t);
+      const Pass& in = pass(t + 1);
+      Pass& out = pass(t);
       f32x4 ks[2], r[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) ks[i] = in.kp[0][i][l] + in.kp[1][i][l];
@@ -604,7 +587,7 @@ struct Walk {
       const lds_t vt = (lds_t)(char*)lds + 16u * (B::VAT + (unsigned)t % B::VN * B::VU);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const s16x4 q = quad(vt + 16u * ((16 * i + qrow) * VB + ((2 * w + ((n & 3) >> 1)) ^ swz(16 * i + qrow, VB))) + 8u * (n & 1));
+        const s16x4 q = quad(vt + 16u * ((16 * i + qrow) * VB + (((n & 3) >> 1) ^ swz(16 * i + qrow, VB))) + 8u * (n & 1));
         const f32x4 cc = *(const f32x4*)&ck.c[16 * i + 4 * g];
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[i][e] = fmaf(-cc[e], ks[i][e], bf2f((bf16_t)q[e]));
@@ -630,15 +613,15 @@ struct Walk {
   }
 
   // ---- the wave that forms their outputs, a step after the chain ----
-  __device__ __forceinline__ void outputs(int w) const {
+  __device__ __forceinline__ void outputs() const {
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
     const unsigned old = 2u * p.HV * V;          // bytes from token to token
-    char* out = (char*)p.out + (long long)lo * old + 2u * (hv * V + (part * NW + w) * 16 + n);
+    char* out = (char*)p.out + (long long)lo * old + 2u * (hv * V + part * 16 + n);
 #pragma unroll
     for (int s = 0; s < AHEAD + 2; ++s) end_step();
     for (int t = 0; t < nc; ++t) {
       const Coef& ck = coef(t);
-      const Pass& in = pass(w, t);
+      const Pass& in = pass(t);
       f32x4 o[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) o[i] = (in.qs[0][i][l] + in.qs[1][i][l]) * *(const f32x4*)&ck.d[16 * i + 4 * g];
@@ -650,13 +633,13 @@ struct Walk {
   }
 };
 
-template <int K, int V, int NW, int AHEAD>
-__global__ __launch_bounds__(64 * (ROLES * NW + SERVICE)) __attribute__((amdgpu_waves_per_eu(2)))
+template <int K, int V>
+__global__ __launch_bounds__(64 * (ROLES + SERVICE)) __attribute__((amdgpu_waves_per_eu(2)))
 void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int* __restrict__ order) {
   // the size at launch: the compiler would take LDS as a bound of the waves on a SIMD, and hand out more registers than
   // a wave can use without moves between their two halves
   extern __shared__ u32x4 lds[];
-  constexpr int COLS = 16 * NW, PARTS = V / COLS;
+  constexpr int COLS = 16, PARTS = V / COLS;
   const int M = p.HV / p.H * PARTS;
   const Place at = place_of(blockIdx.x, s.N * p.H, M);
   if (at.item >= s.N * p.H) return;
@@ -667,23 +650,23 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
   if (dst == 0) {                                // a padding sequence
     const long long old = (long long)p.HV * V;
     bf16_t* out = (bf16_t*)p.out + lo * old + (long long)hv * V + part * COLS;
-    for (long long i = threadIdx.x; i < (long long)len * COLS; i += 64 * (ROLES * NW + SERVICE)) out[i / COLS * old + i % COLS] = 0;
+    for (long long i = threadIdx.x; i < (long long)len * COLS; i += 64 * (ROLES + SERVICE)) out[i / COLS * old + i % COLS] = 0;
     return;
   }
   if (len == 0) {                                // no tokens: the state moves on
     const long long rows = (long long)hv * V * K + (long long)part * COLS * K;
-    for (int i = 4 * threadIdx.x; i < COLS * K; i += 4 * 64 * (ROLES * NW + SERVICE)) {
+    for (int i = 4 * threadIdx.x; i < COLS * K; i += 4 * 64 * (ROLES + SERVICE)) {
       f32x4 x = {};
       if (src != 0) x = *(const f32x4*)(p.S + src * p.slot_stride + rows + i);
       *(f32x4*)(p.S + dst * p.slot_stride + rows + i) = x;
     }
     return;
   }
-  const Walk<K, V, NW, AHEAD> walk = {p, lds, lo, len, (len + C - 1) / C, hv, part};
-  if (w < NW) walk.chain(w);
-  else if (w < 3 * NW) walk.state((w - NW) % NW, (w - NW) / NW, src, dst);
-  else if (w < 4 * NW) walk.outputs(w - 3 * NW);
-  else walk.service(w - 4 * NW, work + ((long long)(lo / C + sn) * p.HV + hv));
+  const Walk<K, V> walk = {p, lds, lo, len, (len + C - 1) / C, hv, part};
+  if (w == 0) walk.chain();
+  else if (w < 3) walk.state(w - 1, src, dst);
+  else if (w == 3) walk.outputs();
+  else walk.service(w - ROLES, work + ((long long)(lo / C + sn) * p.HV + hv));
 }
 
 // ---- the walk with a wave alone for 16 rows ------------------------------------------------------------------------------------
@@ -826,23 +809,11 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
     for (int h = 0; h < 2; ++h) *(f32x4*)(p.S + dst * p.slot_stride + head + 32 * x + 4 * h) = S[x][h];
 }
 
-int num_cus() {
-  static int cache[64] = {0};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-  if (cache[dev] == 0) {
-    int n = 0;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
-    cache[dev] = n;
-  }
-  return cache[dev];
-}
-
 template <int K, int V>
 int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
-  typedef Tiles<K, 1, 2> T;
+  typedef Tiles<K> T;
   typedef Pair<K, 4> P;
-  static const hipError_t set = hipFuncSetAttribute((const void*)walk_kernel<K, V, 1, 2>,
+  static const hipError_t set = hipFuncSetAttribute((const void*)walk_kernel<K, V>,
                                                     hipFuncAttributeMaxDynamicSharedMemorySize, T::BYTES);
   if (set != hipSuccess) return LQ_ERR_HIP;
   int* order = (int*)(work + seq_runs<C>(s) * d->HV);
@@ -851,8 +822,8 @@ int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
   auto grid = [&](int parts) { return (unsigned)place_grid((long long)s->N * d->H, d->HV / d->H * parts); };
   // Up to a CU for every 16 rows the walk spreads each over eight waves; with more of them, one.  Eight | one, 2048
   // tokens each, 32 heads: 1 sequence (256 times 16 rows) 55 | 89 us, 2 sequences 108 | 92, 4 208 | 99.
-  if ((long long)s->N * d->HV * (V / 16) <= num_cus())
-    walk_kernel<K, V, 1, 2><<<grid(V / 16), 64 * (ROLES + SERVICE), T::BYTES, st>>>(*d, *s, work, order);
+  if ((long long)s->N * d->HV * (V / 16) <= lq_seq_cus())
+    walk_kernel<K, V><<<grid(V / 16), 64 * (ROLES + SERVICE), T::BYTES, st>>>(*d, *s, work, order);
   else
     lone_kernel<K, V, 4><<<grid(V / 64), 256, P::BYTES, st>>>(*d, *s, work, order);
   return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;

@@ -13,21 +13,18 @@
 
 namespace {
 
-// the log-gate of a token: GDN and KDA's unbounded form, or KDA's bounded one.  Below -128 its exponential is zero in fp32
-// either way.  A NaN stays one.
-__device__ __forceinline__ float log_gate(float x, float ea, float glb) {
-  return glb != 0.f ? glb / (1.0f + expf(-ea * x)) : -ea * softplus20f(x);
+// the gate of a token: GDN and KDA's unbounded form, or KDA's bounded one.  A NaN stays one.
+__device__ __forceinline__ float gate_of(float x, float ea, float glb) {
+  return exp_f(glb != 0.f ? glb * __builtin_amdgcn_rcpf(1.0f + exp_f(-ea * x)) : -ea * softplus_f(x));
 }
 
-template <int K, bool KDA> struct Token {        // a token's inputs as loaded
-  uint2 q[K / 32], k[K / 32], a[KDA ? K / 32 : 1];
-  bf16_t b, ag;
-};
+constexpr int BLOCK = 8;                         // tokens whose KDA gates a workgroup forms at once
 
 template <int K, int V, int ROWS, bool KDA>
 __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
   constexpr int E = K / 32;                      // float4 groups a lane
   constexpr int PARTS = V / (32 * ROWS);         // workgroups a head
+  __shared__ f32x4 gates[KDA ? BLOCK : 1][KDA ? K / 4 : 1];
   const int part = blockIdx.x % PARTS, hn = blockIdx.x / PARTS, n = hn / p.HV, hv = hn - n * p.HV;
   const int hk = hv / (p.HV / p.H);
   const int lane = threadIdx.x & 7, row0 = part * 32 * ROWS + (threadIdx.x >> 3) * ROWS;
@@ -40,6 +37,23 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
       for (int t = lo; t < hi; ++t) out[t * old + lane] = 0;
     return;
   }
+  const bf16_t* mixed = (const bf16_t*)p.mixed + 4 * lane + hk * K;
+  const bf16_t* vrow = (const bf16_t*)p.mixed + 2ll * p.H * K + (long long)hv * V + row0;
+  u32x2 qn[E], kn[E];                            // the next token's inputs as loaded
+  bf16_t vn[ROWS], bn = 0, an = 0;
+  auto request = [&](int t) {
+    const bf16_t* m = mixed + t * p.mixed_ld;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      qn[e] = *(const u32x2*)(m + 32 * e);
+      kn[e] = *(const u32x2*)(m + p.H * K + 32 * e);
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) vn[r] = vrow[t * p.mixed_ld + r];
+    if (!KDA) an = ((const bf16_t*)p.a)[t * p.a_ld + hv];
+    bn = ((const bf16_t*)p.b)[t * p.b_ld + hv];
+  };
+  if (lo < hi) request(lo);
   const long long head = (long long)hv * V * K + (long long)row0 * K + 4 * lane;
   float S[ROWS][4 * E];
   {
@@ -48,53 +62,45 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
     for (int r = 0; r < ROWS; ++r)
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float4 x = src ? *(const float4*)(f + r * K + 32 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
-        S[r][4 * e] = x.x; S[r][4 * e + 1] = x.y; S[r][4 * e + 2] = x.z; S[r][4 * e + 3] = x.w;
+        f32x4 x = {};
+        if (src) x = *(const f32x4*)(f + r * K + 32 * e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[r][4 * e + i] = x[i];
       }
   }
   const float ea = expf(gate_param(p.A_log, p.gate_bf16 & 1, hv));
-  float dt[KDA ? 4 * E : 1];
-  if (KDA) {
-#pragma unroll
-    for (int i = 0; i < 4 * E; ++i)
-      dt[KDA ? i : 0] = gate_param(p.dt_bias, p.gate_bf16 & 2, (long long)hv * K + 4 * lane + 32 * (i >> 2) + (i & 3));
-  } else {
-    dt[0] = gate_param(p.dt_bias, p.gate_bf16 & 2, hv);
-  }
-  const bf16_t* mixed = (const bf16_t*)p.mixed + 4 * lane;
-  const bf16_t* vrow = (const bf16_t*)p.mixed + 2ll * p.H * K + (long long)hv * V + row0;
-  Token<K, KDA> next;
-  bf16_t vnext[ROWS];
-  auto request = [&](int t) {
-    const bf16_t* m = mixed + t * p.mixed_ld + hk * K;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      next.q[e] = *(const uint2*)(m + 32 * e);
-      next.k[e] = *(const uint2*)(m + p.H * K + 32 * e);
-      if (KDA) next.a[KDA ? e : 0] = *(const uint2*)((const bf16_t*)p.a + t * p.a_ld + hv * K + 4 * lane + 32 * e);
-    }
-    if (!KDA) next.ag = ((const bf16_t*)p.a)[t * p.a_ld + hv];
-    next.b = ((const bf16_t*)p.b)[t * p.b_ld + hv];
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r) vnext[r] = vrow[t * p.mixed_ld + r];
-  };
-  if (lo < hi) request(lo);
+  const int channel = threadIdx.x % K;
+  const float dt = gate_param(p.dt_bias, p.gate_bf16 & 2, KDA ? (long long)hv * K + channel : hv);
+  float scale = 1.f;                             // GDN: the state is scale S
   for (int t = lo; t < hi; ++t) {
-    const Token<K, KDA> now = next;
-    float v[ROWS];
+    if (KDA && (t - lo) % BLOCK == 0) {
+      const bf16_t* a = (const bf16_t*)p.a + hv * K + channel;
+      if (t > lo) __syncthreads();
+      for (int i = threadIdx.x / K; i < min(BLOCK, hi - t); i += 256 / K)
+        ((float*)gates[i])[channel] = gate_of(bf2f(a[(t + i) * p.a_ld]) + dt, ea, p.glb);
+      __syncthreads();
+    }
+    float q[4 * E], k[4 * E], v[ROWS], nq = 0.f, nk = 0.f, kq = 0.f;
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) v[r] = bf2f(vnext[r]);
-    if (t + 1 < hi) request(t + 1);
-    float q[4 * E], k[4 * E], nq = 0.f, nk = 0.f, kq = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t qw[2] = {now.q[e].x, now.q[e].y}, kw[2] = {now.k[e].x, now.k[e].y};
+    for (int e = 0; e < E; ++e)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        q[4 * e + 2 * i] = bf_lo(qw[i]); q[4 * e + 2 * i + 1] = bf_hi(qw[i]);
-        k[4 * e + 2 * i] = bf_lo(kw[i]); k[4 * e + 2 * i + 1] = bf_hi(kw[i]);
+        q[4 * e + 2 * i] = bf_lo(qn[e][i]); q[4 * e + 2 * i + 1] = bf_hi(qn[e][i]);
+        k[4 * e + 2 * i] = bf_lo(kn[e][i]); k[4 * e + 2 * i + 1] = bf_hi(kn[e][i]);
       }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) v[r] = bf2f(vn[r]);
+    const float beta = __builtin_amdgcn_rcpf(1.0f + exp_f(-bf2f(bn)));
+    float al[KDA ? 4 * E : 1];
+    if (KDA) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) al[KDA ? 4 * e + i : 0] = gates[KDA ? (t - lo) % BLOCK : 0][KDA ? lane + 8 * e : 0][i];
+    } else {
+      scale *= gate_of(bf2f(an) + dt, ea, 0.f);
     }
+    if (t + 1 < hi) request(t + 1);
 #pragma unroll
     for (int i = 0; i < 4 * E; ++i) {
       nq = fmaf(q[i], q[i], nq); nk = fmaf(k[i], k[i], nk); kq = fmaf(k[i], q[i], kq);
@@ -102,32 +108,25 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
     nq = sum8(nq); nk = sum8(nk); kq = sum8(kq);
     const float iq = rsqrtf_rn(nq + 1e-6f) * p.scale, ik = rsqrtf_rn(nk + 1e-6f);
     kq *= iq * ik;
-    const float beta = 1.0f / (1.0f + expf(-bf2f(now.b)));
-    float al[KDA ? 4 * E : 1];
-    if (KDA) {
+    if (!KDA && scale < 0x1p-20f) {              // before 1 / scale grows large
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint32_t aw[2] = {now.a[KDA ? e : 0].x, now.a[KDA ? e : 0].y};
+      for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = (i & 1) ? bf_hi(aw[i >> 1]) : bf_lo(aw[i >> 1]);
-          al[KDA ? 4 * e + i : 0] = expf(log_gate(x + dt[KDA ? 4 * e + i : 0], ea, p.glb));
-        }
-      }
-    } else {
-      al[0] = expf(log_gate(bf2f(now.ag) + dt[0], ea, 0.f));
+        for (int i = 0; i < 4 * E; ++i) S[r][i] *= scale;
+      scale = 1.f;
     }
+    const float up = KDA ? ik : ik * __builtin_amdgcn_rcpf(scale), sk = ik * scale, sq = iq * scale;
     float keep = 0.f;
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
       float m = 0.f, y = 0.f;
 #pragma unroll
       for (int i = 0; i < 4 * E; ++i) {
-        S[r][i] *= al[KDA ? i : 0];
+        if (KDA) S[r][i] *= al[KDA ? i : 0];
         m = fmaf(S[r][i], k[i], m); y = fmaf(S[r][i], q[i], y);
       }
-      m = sum8(m) * ik; y = sum8(y) * iq;
-      const float u = beta * (v[r] - m), uk = u * ik;
+      m = sum8(m) * sk; y = sum8(y) * sq;
+      const float u = beta * (v[r] - m), uk = u * up;
 #pragma unroll
       for (int i = 0; i < 4 * E; ++i) S[r][i] = fmaf(uk, k[i], S[r][i]);
       y = fmaf(kq, u, y);
@@ -139,19 +138,38 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      *(float4*)(f + r * K + 32 * e) = make_float4(S[r][4 * e], S[r][4 * e + 1], S[r][4 * e + 2], S[r][4 * e + 3]);
+    for (int e = 0; e < E; ++e) {
+      const float* x = &S[r][4 * e];
+      *(f32x4*)(f + r * K + 32 * e) = f32x4{x[0], x[1], x[2], x[3]} * scale;
+    }
 }
 
 template <int K, int V, int ROWS, bool KDA>
-int launch(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
+int launch_rows(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
   const long long grid = (long long)s->N * d->HV * (V / (32 * ROWS));
   if (grid > 0x7fffffffll) return LQ_ERR_ARG;
   steps_kernel<K, V, ROWS, KDA><<<(unsigned)grid, 256, 0, st>>>(*d, *s);
   return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
 }
+template <int K, int V, bool KDA>
+int launch(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
+  if (s->T <= s->N || (long long)s->N * d->HV * (V / 32) <= 2 * lq_seq_cus()) return launch_rows<K, V, 1, KDA>(d, s, st);
+  return launch_rows<K, V, V / 32, KDA>(d, s, st);
+}
 
 }  // namespace
+
+__attribute__((visibility("hidden"))) int lq_seq_cus() {
+  static int cache[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (cache[dev] == 0) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cache[dev] = n;
+  }
+  return cache[dev];
+}
 
 __attribute__((visibility("hidden"))) int lq_check_delta(const lq_delta* d, const lq_seqs* s) {
   if (!d || !seqs_ok(s)) return LQ_ERR_ARG;
@@ -174,8 +192,8 @@ extern "C" int lq_delta_steps(const lq_delta* d, const lq_seqs* s, void* stream)
   if (int rc = lq_check_delta(d, s)) return rc;
   if (s->N == 0) return LQ_OK;
   hipStream_t st = (hipStream_t)stream;
-  if (d->kda) return launch<128, 128, 4, true>(d, s, st);
-  if (d->K == 128) return launch<128, 128, 4, false>(d, s, st);
-  if (d->V == 128) return launch<64, 128, 4, false>(d, s, st);
-  return launch<64, 64, 2, false>(d, s, st);
+  if (d->kda) return launch<128, 128, true>(d, s, st);
+  if (d->K == 128) return launch<128, 128, false>(d, s, st);
+  if (d->V == 128) return launch<64, 128, false>(d, s, st);
+  return launch<64, 64, false>(d, s, st);
 }

@@ -271,6 +271,24 @@ def test_empty_calls(seq):
         run_delta(fn, none, 2)
 
 
+@pytest.mark.parametrize("fn,first", [("delta_prefill", 1), ("delta_prefill", 100), ("delta_steps", 5)])
+def test_rows_before_the_first_sequence(seq, fn, first):
+    """Packed rows before loc[0] belong to nobody: not read, not written."""
+    d = R.delta_inputs(16, [first, 40, 0, 33], 4, 2, 64, 64)
+    for k in ("loc", "src", "idx"):
+        d[k] = d[k][1:]
+    for k in ("mixed", "a", "b"):
+        d[k][:first] = float("nan")
+    want, S = R.delta_ref(d, 2)
+    g = gpu(d)
+    out = torch.full((first + 73, 4, 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    getattr(seq, fn)(g["S"], g["mixed"], g["a"], g["b"], g["A_log"], g["dt_bias"], g["idx"], g["loc"], out, 2, src=g["src"])
+    torch.cuda.synchronize()
+    assert bool((out[:first] == 7).all())
+    near_prefill(out[first:], want[first:])
+    assert rel(g["S"], S) <= 1e-5
+
+
 # ---- the conv ---------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("C,bias,silu", [(256, True, True), (1000, False, True), (70, True, False), (33, False, True)])
 @pytest.mark.parametrize("lens", [[1], [2, 0, 3, 1], [16, 17, 50, 4]], ids=str)
@@ -325,6 +343,64 @@ def test_conv_of_one_token_equals_the_decode_update(seq):
     assert torch.equal(s1, s2)
     a, b = R.f64(o1), R.f64(o2)                           # both round the same sum: at most a unit apart
     assert (np.abs(a - b) <= 2.0 ** -7 * np.abs(a) + 1e-5).all()
+
+
+@pytest.mark.parametrize("first", [1, 8, 21, 40])
+def test_conv_rows_before_the_first_sequence(seq, first):
+    """Packed rows before loc[0] belong to nobody: not read, not written."""
+    C, lens = 64, [9, 0, 30]
+    g = torch.Generator().manual_seed(23)
+    T = first + sum(lens)
+    x, st, w = (torch.randn(*s, generator=g).to(R.BF16) for s in ((T, C), (7, C, 3), (C, 4)))
+    x[:first] = float("nan")
+    loc = torch.tensor(first + np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32)
+    src, idx = torch.tensor([1, 2, 3], dtype=torch.int32), torch.tensor([4, 5, 6], dtype=torch.int32)
+    want, state = R.conv(R.f64(x), R.f64(st), R.f64(w), None, idx.tolist(), loc.tolist(), src.tolist())
+    s, out = st.to(DEV), torch.full((T, C), 7.0, dtype=torch.bfloat16, device=DEV)
+    seq.conv_prefill(x.to(DEV), s, w.to(DEV), None, idx.to(DEV), loc.to(DEV), out, src=src.to(DEV))
+    torch.cuda.synchronize()
+    assert bool((out[:first] == 7).all())
+    close_bf16(out[first:], want[first:], scale=1.0)
+    assert np.array_equal(R.f64(s), state)
+
+
+@pytest.mark.parametrize("N", [64, 65, 300, 4500])
+def test_conv_of_many_sequences(seq, N):
+    """The search for a run's sequence, in one step, two and three."""
+    C, rng = 2, np.random.default_rng(N)
+    lens = rng.integers(0, 4, N)
+    lens[N // 2] = 100
+    g = torch.Generator().manual_seed(24)
+    T = int(lens.sum())
+    x, st, w = (torch.randn(*s, generator=g).to(R.BF16) for s in ((T, C), (N + 1, C, 3), (C, 4)))
+    loc = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32)
+    idx = torch.tensor(rng.permutation(N) + 1, dtype=torch.int32)
+    want, state = R.conv(R.f64(x), R.f64(st), R.f64(w), None, idx.tolist(), loc.tolist())
+    s, out = st.to(DEV), torch.empty(T, C, dtype=torch.bfloat16, device=DEV)
+    seq.conv_prefill(x.to(DEV), s, w.to(DEV), None, idx.to(DEV), loc.to(DEV), out)
+    torch.cuda.synchronize()
+    close_bf16(out, want, scale=1.0)
+    assert np.array_equal(R.f64(s), state)
+
+
+def test_conv_large_call_equals_its_sequences(seq):
+    """A call of 2^27 elements against each of its sequences in a call of its own (narrower accesses): the same bits."""
+    C, lens = 8192, [9000, 1, 0, 5, 7411]
+    N, T = len(lens), sum(lens)
+    g = torch.Generator(device=DEV).manual_seed(25)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)      # noqa: E731
+    assert T * C >= 1 << 27
+    x, w, b, st = rn(T, C), rn(C, 4), rn(C), rn(2 * N + 1, C, 3)
+    at = np.concatenate([[0], np.cumsum(lens)])
+    loc = torch.tensor(at, dtype=torch.int32, device=DEV)
+    src = torch.arange(1, N + 1, dtype=torch.int32, device=DEV)
+    s1, s2, o1, o2 = st.clone(), st.clone(), torch.empty_like(x), torch.empty_like(x)
+    seq.conv_prefill(x, s1, w, b, src + N, loc, o1, src=src)
+    for n in range(N):
+        own = slice(int(at[n]), int(at[n + 1]))
+        seq.conv_prefill(x[own], s2, w, b, src[n:n + 1] + N, loc[n:n + 2] - loc[n], o2[own], src=src[n:n + 1])
+    torch.cuda.synchronize()
+    assert torch.equal(o1, o2) and torch.equal(s1, s2)
 
 
 # ---- the norms --------------------------------------------------------------------------------------------------------
