@@ -205,6 +205,6 @@ def gated_norm(x, z, weight, out, eps=1e-6, gate="silu", offset=0.0):
 def add_norm(x, y, weight, res, out, eps=1e-6, scale=1.0, offset=0.0):
     """The residual add and the norm before the next block: res = x + scale y, out = res rsqrt(mean(res^2) + eps)
     (offset + weight), of the sum before it is rounded to bf16.  Shapes as `gated_norm`; res and out are laid out alike; res
-    may be x (in place)."""
+    may be x or y (in place)."""
     n = _norm(x, y, weight, out, res, eps, scale, offset, 0)
     _lib.check(_lib.seq_lib().lq_add_norm(n, _raw_stream(x)), "lq_add_norm")

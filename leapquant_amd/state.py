@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from . import kernels as KN
+from . import seq
 
 WINDOW = 16          # tokens per window (L), state.py:16
 RANK = 4             # Compensator Tokens per head (R), state.py:17
@@ -67,6 +68,10 @@ class LeapQuantState:
     head that a call fills, the second is flushed at the start of the next call that steps its slot (the outputs are
     the same; a due row costs its call one head flush instead of two).  dequantize settles such heads first.
     """
+
+    # tokens a sequence up to which a GDN prefill goes token by token: at 8 both take 75 us (64 sequences of 32 heads of 128 x
+    # 128) or 15 against 17 (8 sequences), at 4 55 against 74 and 11 against 17, at 16 118 against 75 and 23 against 17
+    STEPS = 8
 
     def __init__(self, ssm, H, kda=False, gate_lower_bound=0.0, nmax=0, L=WINDOW, R=RANK, qmax=KN.QMAX,
                  defer_flush=False):
@@ -175,6 +180,27 @@ class LeapQuantState:
         else:                        # step + flush of the heads it fills (one launch)
             fn = L.lq_gdn_decode_deferred if self.defer_flush else L.lq_gdn_decode
             _lib.check(fn(ctypes.byref(st), ctypes.byref(io), None, dev(self.Q0), stream), "lq_gdn_decode")
+
+    def prefill(self, ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, has_state=None):
+        """The prompts of a ragged batch, or their next pieces: tokens loc[n] .. loc[n + 1] - 1 of the packed mixed [T, 2HK +
+        HV V], a, b and out [T, HV, V] belong to slot idx[n] (an idx outside 1 .. NS - 1: padding).  has_state [N]: which
+        sequences go on from the checkpoint of their slot; the others start from zero, as all do by default.  The states
+        are fp32 for the call and end as the 8-bit checkpoints that decode reads, with empty windows.
+        GDN prompts go through `seq.delta_prefill`; KDA, and calls of at most STEPS tokens a sequence, token by token."""
+        if idx.dim() != 1:
+            raise ValueError("idx: 1-D expected, got shape %s" % (tuple(idx.shape),))
+        if has_state is not None and has_state.shape != idx.shape:
+            raise ValueError("has_state: one of each idx expected, got shape %s" % (tuple(has_state.shape),))
+        src = torch.zeros_like(idx) if has_state is None else idx * has_state.to(torch.bool)
+        if has_state is not None:
+            self.dequantize(ssm, src)
+        if self.kda:
+            seq.delta_steps(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src=src, scale=self._scale, kda=True,
+                            gate_lower_bound=self.glb)
+        else:
+            fn = seq.delta_steps if mixed.shape[0] <= self.STEPS * idx.shape[0] else seq.delta_prefill
+            fn(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src=src, scale=self._scale)
+        self.quantize(ssm, idx)
 
     def decode_conv(self, ssm, x, conv_state, conv_weight, conv_bias, silu, a, b, A_log, dt_bias, idx, out):
         """GDN decode with the conv1d update fused into the step (lq_gdn_step_conv): x is the raw projection
