@@ -80,7 +80,7 @@ def _param(t, n, name):
     return t if t.is_contiguous() else t.detach().contiguous()
 
 
-def _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, glb):
+def _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, glb, chunks=False):
     """Bytes of lq_delta and lq_seqs, and the tensors that have to live until the launch."""
     if S.dtype is not _F32 or S.dim() != 4:
         raise TypeError("S: fp32 [NS, HV, V, K] expected, got %s %s" % (S.dtype, tuple(S.shape)))
@@ -106,7 +106,7 @@ def _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, gl
     a_ld, b_ld = _rows(a, T, HV * KA, "a", 4 if kda else 1), _rows(b, T, HV, "b", 1)
     if out.dtype is not _BF16 or out.shape != (T, HV, V) or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out: contiguous 16-byte aligned bf16 [T, HV, V] expected")
-    if T * HV > 1 << 30 or mixed_ld > 1 << 24:
+    if chunks and (T * HV > 1 << 30 or mixed_ld > 1 << 24):
         raise ValueError("at most 2^30 tokens times value heads and rows of 2^24 elements in a call, got %d and %d"
                          % (T * HV, mixed_ld))
     A_log, dt_bias = _param(A_log, HV, "A_log"), _param(dt_bias, HV * KA, "dt_bias")
@@ -125,7 +125,7 @@ def delta_prefill(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, sc
     [T, 2HK + HV V] after the conv, q | k | v; a, b: bf16 [T, HV] raw gates.  The three may be column ranges of wider rows.
     A_log, dt_bias: [HV].  out: bf16 [T, HV, V].  scale: of the queries, K^-1/2 by default.  Gates, norms and state as the
     decode step's, with beta = sigmoid(b) not rounded.  A NaN or infinity in a token reaches all tokens of its chunk of 32."""
-    d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, False, 0.0)
+    d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, False, 0.0, chunks=True)
     L = _lib.seq_lib()
     n = L.lq_delta_workspace(d, seqs)
     work = torch.empty(n, dtype=torch.uint8, device=S.device) if n > 0 else None

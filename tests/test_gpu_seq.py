@@ -465,3 +465,78 @@ def test_norm_graph(seq):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(r, r2) and torch.equal(o, o2)
+
+
+# ---- together -----------------------------------------------------------------------------------------------------------
+def test_graph_of_conv_and_norms(seq):
+    """Replays of the conv and both norms equal the eager results, with other work between."""
+    g = torch.Generator(device=DEV).manual_seed(40)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)      # noqa: E731
+    x, st, w, nw = rn(77, 256), rn(7, 256, 3), rn(256, 4), rn(256)
+    loc = torch.tensor([0, 40, 41, 77], dtype=torch.int32, device=DEV)
+    src = torch.arange(1, 4, dtype=torch.int32, device=DEV)
+    y, n, r, o = (torch.zeros_like(x) for _ in range(4))
+
+    def run():
+        seq.conv_prefill(x, st, w, None, src + 3, loc, y, src=src)
+        seq.gated_norm(y, x, nw, n)
+        seq.add_norm(x, n, nw, r, o, scale=0.5)
+
+    run()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (st, y, n, r, o)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for _ in range(4):
+        for t in (y, n, r, o, st[4:]):
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((st, y, n, r, o), want))
+        torch.matmul(x, w)
+        torch.cuda.synchronize()
+
+
+def _far(rows, cols, ld):
+    """bf16 [rows, cols] whose last rows lie past 2^32 elements."""
+    return torch.empty((rows - 1) * ld + cols, dtype=torch.bfloat16, device=DEV).as_strided((rows, cols), (ld, 1))
+
+
+@pytest.mark.parametrize("fn", ["delta_prefill", "delta_steps"])
+def test_delta_offsets_past_32_bits(seq, fn):
+    """Slots past 2^31 floats of the state cache and tokens past 2^32 elements: the bits of the same call on small tensors."""
+    d = R.delta_inputs(41, [40, 30], 2, 1, 128, 128)
+    g = gpu(d)
+    want = run_delta(getattr(seq, fn), g, 1)
+    NS = (1 << 31) // (2 * 128 * 128) + 8
+    S = torch.empty(NS, 2, 128, 128, device=DEV)
+    far = [NS - 4, NS - 3, NS - 2, NS - 1]
+    S[far[0]], S[far[1]] = d["S"][1].to(DEV), d["S"][2].to(DEV)
+    mixed = _far(70, d["mixed"].shape[1], 1 << 24 if fn == "delta_prefill" else 1 << 26)
+    mixed.copy_(g["mixed"])
+    out = torch.zeros_like(want)
+    getattr(seq, fn)(S, mixed, g["a"], g["b"], g["A_log"], g["dt_bias"], torch.tensor(far[2:], device=DEV), g["loc"], out, 1,
+                     src=torch.tensor(far[:2], device=DEV))
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(S[far[2]], g["S"][3]) and torch.equal(S[far[3]], g["S"][4])
+
+
+def test_conv_and_norm_offsets_past_32_bits(seq):
+    g = torch.Generator(device=DEV).manual_seed(42)
+    rn = lambda *s: torch.randn(*s, generator=g, device=DEV).to(torch.bfloat16)      # noqa: E731
+    T, C, ld = 70, 64, 1 << 26
+    x, w, st, nw = rn(T, C), rn(C, 4), rn(3, C, 3), rn(C)
+    far = _far(T, C, ld)
+    far.copy_(x)
+    loc = torch.tensor([0, 60, T], dtype=torch.int32, device=DEV)
+    idx = torch.tensor([1, 2], dtype=torch.int32, device=DEV)
+    s1, s2, a, b = st.clone(), st.clone(), torch.empty_like(x), torch.empty_like(x)
+    seq.conv_prefill(x, s1, w, None, idx, loc, a)
+    seq.conv_prefill(far, s2, w, None, idx, loc, b)
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and torch.equal(s1, s2)
+    seq.gated_norm(x, x, nw, a)
+    seq.gated_norm(far, x, nw, far)                       # in place
+    torch.cuda.synchronize()
+    assert torch.equal(far, a)
