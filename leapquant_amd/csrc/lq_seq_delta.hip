@@ -19,6 +19,8 @@
 // carried as two bf16 halves (hi + lo, 2^-17 of an element is lost), their products as the two or three significant ones: the
 // state is accurate to a few 1e-6, where single bf16 operands would leave 3e-3, and the outputs keep their digits where
 // their terms cancel (a query nearly orthogonal to the state, equal keys in a chunk).
+#include <type_traits>
+
 #include "lq_seq.h"
 
 __attribute__((visibility("hidden"))) int lq_check_delta(const lq_delta* d, const lq_seqs* s);
@@ -77,7 +79,7 @@ __device__ __forceinline__ int swz(int r, int blocks) { return (r / (16 / blocks
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds(const void* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
                : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -738,15 +740,16 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
     col_at[x] = 16u * (qrow * RB + ((4 * x + (n & 3)) ^ swz(qrow, RB)));
   }
   if (nc > 0) request(min(C, len), 0);
-  for (int c = 0; c < nc; ++c) {
+  auto step = [&](int c, auto half) {             // the buffer a constant: every place in LDS is a register and an offset
+    constexpr int BUF = decltype(half)::value;
     const int left = len - c * C;
     // chunk c has landed: after its loads came the stores of the chunk before
     if (c > 0) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     end_step();
-    if (left > C) request(min(C, left - C), (c + 1) & 1);
-    const lds_t kt = base + 16u * B::BUF * (c & 1), qt = kt + 16u * TU;
-    const Coef& ck = *(const Coef*)(lds + B::BUF * (c & 1) + B::CAT);
+    if (left > C) request(min(C, left - C), 1 - BUF);
+    const lds_t kt = base + 16u * B::BUF * BUF, qt = kt + 16u * TU;
+    const Coef& ck = *(const Coef*)(lds + B::BUF * BUF + B::CAT);
     f32x4 ks[2] = {}, qs[2] = {};
 #pragma unroll
     for (int x = 0; x < KS; ++x) {
@@ -797,11 +800,20 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
       }
     if (left > C) {                              // eight stores, which the next step's wait counts
 #pragma unroll
-      for (int i = 0; i < 8; ++i) *(bf16_t*)(out + (16 * (i >> 2) + 4 * g + (i & 3)) * old) = f2bf(qs[i >> 2][i & 3]);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t two = pk_bf16_kept(qs[i >> 1][2 * (i & 1)], qs[i >> 1][2 * (i & 1) + 1]);
+        bf16_t* to = (bf16_t*)(out + (16 * (i >> 1) + 4 * g + 2 * (i & 1)) * old);
+        to[0] = (bf16_t)two;
+        *(bf16_t*)((char*)to + old) = (bf16_t)(two >> 16);
+      }
     } else {
       store_chunk(out, old, qs, g, left);
     }
     out += (long long)C * old;
+  };
+  for (int c = 0; c < nc; c += 2) {
+    step(c, std::integral_constant<int, 0>());
+    if (c + 1 < nc) step(c + 1, std::integral_constant<int, 1>());
   }
 #pragma unroll
   for (int x = 0; x < KS; ++x)
