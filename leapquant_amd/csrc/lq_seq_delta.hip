@@ -41,7 +41,17 @@ __device__ __forceinline__ f32x4 mf(const bf16x4& a, const bf16x4& b, const f32x
   return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ bf16x4 first4(const bf16x8& a) { return __builtin_shufflevector(a, a, 0, 1, 2, 3); }
-// eight fp32 values as two bf16 halves
+// four or eight fp32 values as two bf16 halves
+__device__ __forceinline__ void split4(const f32x4& x, bf16x4& hi, bf16x4& lo) {
+  u32x2 h, l;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    h[i] = pk_bf16_kept(x[2 * i], x[2 * i + 1]);
+    l[i] = pk_bf16(x[2 * i] - bf_lo(h[i]), x[2 * i + 1] - bf_hi(h[i]));
+  }
+  hi = __builtin_bit_cast(bf16x4, h);
+  lo = __builtin_bit_cast(bf16x4, l);
+}
 __device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, bf16x8& hi, bf16x8& lo) {
   const float f[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
   u32x4 h, l;
@@ -321,15 +331,12 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
     const f32x4 b0 = *(const f32x4*)&my.bet[4 * g], b1 = *(const f32x4*)&my.bet[16 + 4 * g];
     const float e0 = exp_f((gh - my.ghi[n]) + (gl - my.glo[n])) * my.rk[n];
     const float e1 = exp_f((gh - my.ghi[16 + n]) + (gl - my.glo[16 + n])) * my.rk[16 + n];
-    const f32x4 zero = {};
     bf16x8 hi, lo;
-    split8(*(const f32x4*)&my.m[n][4 * g] * b0 * e0, zero, hi, lo);
-    out.t0[0][l] = first4(hi); out.t0[1][l] = first4(lo);
+    split4(*(const f32x4*)&my.m[n][4 * g] * b0 * e0, out.t0[0][l], out.t0[1][l]);
     split8(*(const f32x4*)&my.m[16 + n][4 * g] * b0 * e1, *(const f32x4*)&my.m[16 + n][16 + 4 * g] * b1 * e1, hi, lo);
     out.t1[0][l] = hi; out.t1[1][l] = lo;
     spread(ww[0], ww[1], ww[2]);
-    split8(*(const f32x4*)&my.m[n][4 * g] * b0, zero, hi, lo);
-    out.w0[0][l] = first4(hi); out.w0[1][l] = first4(lo);
+    split4(*(const f32x4*)&my.m[n][4 * g] * b0, out.w0[0][l], out.w0[1][l]);
     split8(*(const f32x4*)&my.m[16 + n][4 * g] * b0, *(const f32x4*)&my.m[16 + n][16 + 4 * g] * b1, hi, lo);
     out.w1[0][l] = hi; out.w1[1][l] = lo;
     if (l < C) {
@@ -359,8 +366,7 @@ struct Tiles {                         // places in LDS, in 16-byte blocks
   static constexpr int CU = (int)sizeof(Coef) / 16, CN = 8;
   static constexpr int KN = AHEAD + 3, QN = AHEAD + 2, VN = AHEAD + 2;
   static constexpr int QAT = KN * TU, VAT = QAT + QN * TU, CAT = VAT + VN * VU, XAT = CAT + KN * CN * 64;
-  static constexpr int PAT = XAT + 2 * 4 * 64, SAT = PAT + 2 * PASS;          // what the waves pass on; scratch
-  static constexpr int END = SAT + SERVICE * 16 * 5, BYTES = 16 * END;
+  static constexpr int PAT = XAT + 2 * 4 * 64, END = PAT + 2 * PASS, BYTES = 16 * END;      // PAT: what the waves pass on
   // loads of a service wave for a chunk, the same for each: all four load V, and Coef's last blocks more than once, so that
   // one count says what is still on its way
   static constexpr int LOADS = 2 * TU / 64 / SERVICE + 1 + CN / SERVICE;
@@ -400,7 +406,6 @@ struct Walk {
     const char *kb = rows + 2u * (p.H + hk) * K, *qb = rows + 2u * hk * K;
     const char* vb = rows + 2u * (2 * p.H * K + hv * V + part * 16);
     const char* cb = (const char*)work;
-    float(*m)[20] = (float(*)[20])(lds + B::SAT + 80 * k);
     const int xi = k >> 1, xe = k & 1;           // rows of this chunk, of the one before
     for (int s = -1 - AHEAD; s <= nc; ++s) {
       const int j = s + 1 + AHEAD;
@@ -431,16 +436,14 @@ struct Walk {
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
           const int at = (4 * x + g) ^ swz(n, RB);
-          xx = mf(__builtin_bit_cast(bf16x8, kt[at]), __builtin_bit_cast(bf16x8, ko[at]), xx);
+          xx = mf(__builtin_bit_cast(bf16x8, ko[at]), __builtin_bit_cast(bf16x8, kt[at]), xx);
         }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m[4 * g + r][n] = xx[r];
-        wave_sync();
-        bf16x8 hi, lo;
-        split8(*(const f32x4*)&m[n][4 * g], f32x4{}, hi, lo);
+        // X's transpose as a result: a lane has row n of X at the columns 4 g .., as the chain takes it
+        bf16x4 hi, lo;
+        split4(xx, hi, lo);
         bf16x4* out = (bf16x4*)(xtile(s + 1) + 128 * xi + l) + xe;
-        out[0] = first4(hi);
-        out[128] = first4(lo);
+        out[0] = hi;
+        out[128] = lo;
       }
       // what the next step needs has landed; this step's request may still be on its way
       if (j < nc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(B::LOADS) : "memory");
