@@ -137,12 +137,22 @@ __device__ __forceinline__ void chunk_product(const bf16x4 (&m0)[2][64], const b
   y[0] = mf(m0[1][l], first4(rh), y0);
   y[1] = mf(m1[1][l], rh, y1);
 }
-// a result's rows, tokens, that there are
-__device__ __forceinline__ void store_chunk(char* out, unsigned old, const f32x4 (&o)[2], int g, int left) {
+// a result's rows, tokens, that there are: this lane's offsets from the chunk's first token, and their stores
+__device__ __forceinline__ void store_places(unsigned (&at)[8], unsigned old, int n, int g) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 16 * (i >> 2) + 4 * g + (i & 3);
-    if (r < left) *(bf16_t*)(out + r * old) = f2bf(o[i >> 2][i & 3]);
+  for (int i = 0; i < 8; ++i) at[i] = (16 * (i >> 2) + 4 * g + (i & 3)) * old + 2u * n;
+}
+__device__ __forceinline__ void store_chunk(char* out, const unsigned (&at)[8], const f32x4 (&o)[2], int g, int left) {
+  uint32_t two[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) two[i] = pk_bf16_kept(o[i >> 1][2 * (i & 1)], o[i >> 1][2 * (i & 1) + 1]);
+  if (left >= C) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) *(bf16_t*)(out + at[i]) = (bf16_t)(i & 1 ? two[i >> 1] >> 16 : two[i >> 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (16 * (i >> 2) + 4 * g + (i & 3) < left) *(bf16_t*)(out + at[i]) = (bf16_t)(i & 1 ? two[i >> 1] >> 16 : two[i >> 1]);
   }
 }
 
@@ -363,14 +373,14 @@ template <int K>
 struct Tiles {                         // places in LDS, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB;                    // blocks of a row of K, of a tile
   static constexpr int VB = 2, VU = C * VB;                        // the same of the workgroup's columns of V
-  static constexpr int CU = (int)sizeof(Coef) / 16, CN = 8;
+  static constexpr int CU = (int)sizeof(Coef) / 16, CN = 7;
   static constexpr int KN = AHEAD + 3, QN = AHEAD + 2, VN = AHEAD + 2;
   static constexpr int QAT = KN * TU, VAT = QAT + QN * TU, CAT = VAT + VN * VU, XAT = CAT + KN * CN * 64;
   static constexpr int PAT = XAT + 2 * 4 * 64, END = PAT + 2 * PASS, BYTES = 16 * END;      // PAT: what the waves pass on
-  // loads of a service wave for a chunk, the same for each: all four load V, and Coef's last blocks more than once, so that
-  // one count says what is still on its way
-  static constexpr int LOADS = 2 * TU / 64 / SERVICE + 1 + CN / SERVICE;
-  static_assert(VU == 64 && CN * 64 >= CU && CN % SERVICE == 0, "loads of a chunk");
+  // loads of a service wave for a chunk, the same for each (the last one of the last wave is V), so that one count says what
+  // is still on its way
+  static constexpr int LOADS = 2 * TU / 64 / SERVICE + (CN + 1) / SERVICE;
+  static_assert(VU == 64 && CN * 64 >= CU && (CN + 1) % SERVICE == 0, "loads of a chunk");
   static_assert(BYTES <= 160 * 1024, "LDS of a CU");
   static_assert(LOADS < 64, "what a wave may have outstanding");
 };
@@ -383,8 +393,11 @@ struct Walk {
   u32x4* lds;
   int lo, len, nc, hv, part;
 
-  __device__ __forceinline__ const u32x4* ktile(int c) const { return lds + (unsigned)c % B::KN * TU; }
-  __device__ __forceinline__ const Coef& coef(int c) const { return *(const Coef*)(lds + B::CAT + (unsigned)c % B::KN * B::CN * 64); }
+  // the tiles of K and the Coefs go round KN places: a chunk's place, the next one's, the one's before
+  static __device__ __forceinline__ int after(int at) { return at == B::KN - 1 ? 0 : at + 1; }
+  static __device__ __forceinline__ int before(int at) { return at == 0 ? B::KN - 1 : at - 1; }
+  __device__ __forceinline__ const u32x4* ktile(int at) const { return lds + at * TU; }
+  __device__ __forceinline__ const Coef& coef(int at) const { return *(const Coef*)(lds + B::CAT + at * B::CN * 64); }
   __device__ __forceinline__ bf16x8* xtile(int c) const { return (bf16x8*)(lds + B::XAT + (c & 1) * 256); }
   __device__ __forceinline__ Pass& pass(int c) const { return ((Pass*)(lds + B::PAT))[c & 1]; }
 
@@ -407,31 +420,40 @@ struct Walk {
     const char* vb = rows + 2u * (2 * p.H * K + hv * V + part * 16);
     const char* cb = (const char*)work;
     const int xi = k >> 1, xe = k & 1;           // rows of this chunk, of the one before
+    constexpr int TL = TU / 64 / SERVICE, CL = (B::CN + 1) / SERVICE;
+    unsigned toff[TL], coff[CL];                 // this lane's offsets from a chunk's first row; rows past its end: the last again
+    auto place = [&](int count) {
+#pragma unroll
+      for (int i = 0; i < TL; ++i) {
+        const int u = l + 64 * (SERVICE * i + k), r = u / RB;
+        toff[i] = (unsigned)min(r, count - 1) * ld + 16u * ((u % RB) ^ swz(r, RB));
+      }
+      if (k == SERVICE - 1) coff[CL - 1] = (unsigned)min(l / VB, count - 1) * ld + 16u * ((l % VB) ^ swz(l / VB, VB));
+    };
+#pragma unroll
+    for (int i = 0; i < CL; ++i) coff[i] = 16u * min(l + 64 * (CL * k + i), B::CU - 1);
+    place(C);
+    int jk = 0, sk = B::KN - 1 - AHEAD;          // places of the chunks j and s
     for (int s = -1 - AHEAD; s <= nc; ++s) {
       const int j = s + 1 + AHEAD;
-      if (j < nc) {                              // request chunk j; rows past the end: the last one again
-        const int nv = min(C, len - j * C);
-        const unsigned ka = lds0 + 16u * ((unsigned)j % B::KN * TU), qa = lds0 + 16u * (B::QAT + (unsigned)j % B::QN * TU);
+      if (j < nc) {                              // request chunk j
+        if (len - j * C < C) place(len - j * C);
+        const unsigned ka = lds0 + 16u * jk * TU + 1024u * k, qa = lds0 + 16u * (B::QAT + (unsigned)j % B::QN * TU) + 1024u * k;
         const unsigned va = lds0 + 16u * (B::VAT + (unsigned)j % B::VN * B::VU);
-        const unsigned ca = lds0 + 16u * (B::CAT + (unsigned)j % B::KN * B::CN * 64);
+        const unsigned ca = lds0 + 16u * (B::CAT + jk * B::CN * 64) + 1024u * CL * k;
 #pragma unroll
-        for (int i = 0; i < TU / 64 / SERVICE; ++i) {
-          const int at = SERVICE * i + k, u = l + 64 * at, r = u / RB, b = (u % RB) ^ swz(r, RB);
-          const unsigned off = (unsigned)min(r, nv - 1) * ld + 16u * b;
-          to_lds(kb, off, ka + 1024u * at);
-          to_lds(qb, off, qa + 1024u * at);
+        for (int i = 0; i < TL; ++i) {
+          to_lds(kb, toff[i], ka + 1024u * SERVICE * i);
+          to_lds(qb, toff[i], qa + 1024u * SERVICE * i);
         }
-        to_lds(vb, (unsigned)min(l / VB, nv - 1) * ld + 16u * ((l % VB) ^ swz(l / VB, VB)), va);
 #pragma unroll
-        for (int i = 0; i < B::CN / SERVICE; ++i) {
-          const int at = SERVICE * i + k;
-          to_lds(cb, 16u * min(l + 64 * at, B::CU - 1), ca + 1024u * at);
-        }
+        for (int i = 0; i < CL - 1; ++i) to_lds(cb, coff[i], ca + 1024u * i);
+        to_lds(k < SERVICE - 1 ? cb : vb, coff[CL - 1], k < SERVICE - 1 ? ca + 1024u * (CL - 1) : va);
         kb += (long long)C * ld; qb += (long long)C * ld; vb += (long long)C * ld;
         cb += (long long)p.HV * sizeof(Coef);
       }
       if (s >= 0 && s + 1 < nc) {                // X of chunk s + 1
-        const u32x4 *kt = ktile(s + 1) + (16 * xi + n) * RB, *ko = ktile(s) + (16 * xe + n) * RB;
+        const u32x4 *kt = ktile(after(sk)) + (16 * xi + n) * RB, *ko = ktile(sk) + (16 * xe + n) * RB;
         f32x4 xx = {};
 #pragma unroll
         for (int x = 0; x < KS; ++x) {
@@ -449,6 +471,8 @@ struct Walk {
       if (j < nc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(B::LOADS) : "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (s < nc) end_step();
+      jk = after(jk);
+      sk = after(sk);
     }
   }
 
@@ -477,12 +501,14 @@ struct Walk {
     // step t: S_t, then K_{t+1} S_t and Q_t S_t (of whatever is in LDS where there is no such chunk: nobody reads that), and
     // S_t e^{G_C} for the next step.  In the order in which it is to issue: 32 channels' halves are formed and scaled between
     // the matrix instructions of the 32 before, behind the update of the 32 after.
+    int tk = B::KN - 1;                          // place of chunk t
     auto step = [&](int t, bool update) {
-      const lds_t ko = base + 16u * ((unsigned)(t - 1 + B::KN) % B::KN * TU), kn = base + 16u * ((unsigned)(t + 1) % B::KN * TU);
+      const lds_t ko = base + 16u * before(tk) * TU, kn = base + 16u * after(tk) * TU;
       const lds_t qt = base + 16u * (B::QAT + (unsigned)(t + B::QN) % B::QN * TU);
       const Pass& in = pass(t + 1);
       Pass& out = pass(t);
-      const float next = t < 0 || t == nc ? 1.f : coef(t).last[0];
+      const float next = t < 0 || t == nc ? 1.f : coef(tk).last[0];
+      tk = after(tk);
       bf16x8 uh, ul, kf[2][2], qf[2][2], sh[2], sl[2];
       auto fetch = [&](int x) {
 #pragma unroll
@@ -572,8 +598,9 @@ struct Walk {
   __device__ __forceinline__ void chain() const {
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4, qrow = 4 * g + (n >> 2);
     bf16x8 uh = {}, ul = {};
+    int tk = 0;                                  // place of chunk t
     auto step = [&](int t, bool first) {
-      const Coef& ck = coef(t);
+      const Coef& ck = coef(tk);
       const Pass& in = pass(t + 1);
       Pass& out = pass(t);
       f32x4 ks[2], r[2];
@@ -581,7 +608,7 @@ struct Walk {
       for (int i = 0; i < 2; ++i) ks[i] = in.kp[0][i][l] + in.kp[1][i][l];
       if (!first) {
         const bf16x8* xt = xtile(t);
-        const float last = coef(t - 1).last[0];
+        const float last = coef(before(tk)).last[0];
 #pragma unroll
         for (int i = 0; i < 2; ++i) ks[i] *= last;
 #pragma unroll
@@ -606,6 +633,7 @@ struct Walk {
       split8(U[0], U[1], uh, ul);
       out.u[0][l] = uh;
       out.u[1][l] = ul;
+      tk = after(tk);
     };
 #pragma unroll
     for (int s = 0; s < AHEAD + 1; ++s) end_step();
@@ -621,17 +649,19 @@ struct Walk {
   __device__ __forceinline__ void outputs() const {
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
     const unsigned old = 2u * p.HV * V;          // bytes from token to token
-    char* out = (char*)p.out + (long long)lo * old + 2u * (hv * V + part * 16 + n);
+    char* out = (char*)p.out + (long long)lo * old + 2u * (hv * V + part * 16);
+    unsigned at[8];
+    store_places(at, old, n, g);
 #pragma unroll
     for (int s = 0; s < AHEAD + 2; ++s) end_step();
-    for (int t = 0; t < nc; ++t) {
-      const Coef& ck = coef(t);
+    for (int t = 0, tk = 0; t < nc; ++t, tk = after(tk)) {
+      const Coef& ck = coef(tk);
       const Pass& in = pass(t);
       f32x4 o[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) o[i] = (in.qs[0][i][l] + in.qs[1][i][l]) * *(const f32x4*)&ck.d[16 * i + 4 * g];
       chunk_product(ck.w0, ck.w1, in.r[0][l], in.r[1][l], l, o[0], o[1], o);
-      store_chunk(out, old, o, g, len - t * C);
+      store_chunk(out, at, o, g, len - t * C);
       out += (long long)C * old;
       if (t + 1 < nc) end_step();
     }
@@ -810,7 +840,9 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
         *(bf16_t*)((char*)to + old) = (bf16_t)(two >> 16);
       }
     } else {
-      store_chunk(out, old, qs, g, left);
+      unsigned at[8];
+      store_places(at, old, 0, g);
+      store_chunk(out, at, qs, g, left);
     }
     out += (long long)C * old;
   };
