@@ -7,7 +7,8 @@
 // workgroup touches them, so a call can run in place.
 //
 // VEC = 8 where the call is large (WIDE): a workgroup's rows are then 4 KiB pieces, and 32768 tokens of 8192 channels take
-// 215 us (1.07 GB: 5.0 TB/s, a large copy's rate), against 276 us with VEC = 2.  VEC = 2 below: a thread moves 2 channels'
+// 212 us (1.07 GB: 5.1 TB/s, past a large copy's rate; 218 without the outputs' hint, 223 with one on the inputs, which
+// other runs read again), against 276 us with VEC = 2.  VEC = 2 below: a thread moves 2 channels'
 // taps and not 8, and there are four times the waves: 64 tokens 4.5 us against 9.4, 333 tokens 6.4 against 10.8, 8000
 // tokens 66 against 70, which is about where they meet.  Small calls are bound by their chain of loads: the run's
 // sequence, its slots, the taps.
@@ -112,7 +113,12 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(lq_conv cv, lq_seqs s, co
       if (silu) y[e] *= fast_sigmoid(y[e]);
       h[0][e] = h[1][e]; h[1][e] = h[2][e]; h[2][e] = f[e];
     }
-    if (i < n) *(raw_t*)(o + (long long)i * C) = dst ? E::pack(y) : E::zero();
+    if (i < n) {
+      const raw_t r = dst ? E::pack(y) : E::zero();
+      raw_t* to = (raw_t*)(o + (long long)i * C);
+      if (VEC == 8) __builtin_nontemporal_store(r, to);      // more than the caches hold
+      else *to = r;
+    }
   }
 }
 

@@ -16,11 +16,11 @@
 //
 // Rounding.  The raw keys, queries and values are bf16 and enter the products as they are; their norms, decays and beta are
 // fp32 factors of rows and columns of fp32 sums, never folded into an operand.  fp32 operands (S, R, T', W, X, T' R) are
-// carried as two bf16 halves (hi + lo, 2^-17 of an element is lost), their products as the two or three significant ones: the
-// state is accurate to a few 1e-6, where single bf16 operands would leave 3e-3, and the outputs keep their digits where
-// their terms cancel (a query nearly orthogonal to the state, equal keys in a chunk).  A third half would bring the state to
-// the 2e-7 of fp32 sums for half as many matrix instructions again; what reads it rounds it to 8 bits (6e-3) or the outputs
-// to bf16 (2e-3).
+// carried as two bf16 halves (hi + lo: at most 2^-16 of an element is lost, 2.8e-6 in the mean), their products as the two or
+// three significant ones: the state ends within 5e-6 of its norm, where single bf16 operands would leave 3e-3, and the
+// outputs keep their digits where their terms cancel (a query nearly orthogonal to the state, equal keys in a chunk).  A
+// third half would bring the state to the 2e-7 of fp32 sums for half as many matrix instructions again; what reads it
+// rounds it to 8 bits (5e-3 of the outputs), and the outputs are bf16 (1.7e-3).
 //
 // Measured (both kernels, heads of 128 x 128, 16 key and 32 value heads): one prompt of 8192 tokens 206 us (201 MB of tokens
 // and outputs; its 256 steps of 0.68 us are the time), 13 prompts of 32768 tokens 430-470 us (805 MB: 1.8 TB/s; matrix
@@ -204,7 +204,7 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
   if (number >= s.T / C + s.N) return;
   const SeqRun run = seq_run<C>(s, number);
   const int t0 = run.lo + run.j * C, nv = min(C, run.hi - t0);
-  if (nv <= 0 || seq_dst(s, run.n, p.NS) == 0) return;
+  if (nv <= 0) return;
   const int l = threadIdx.x & 63, n = l & 15, g = l >> 4;
   bf16x8 kf[2][KS], qf[2][KS];
 #pragma unroll

@@ -5,29 +5,37 @@
 // A row is held by LANES threads (8 to 256), CH groups of VEC elements each, groups of one thread LANES * VEC apart so that a
 // load instruction covers consecutive bytes.  LANES <= 64 reduces by lane exchanges, above that through LDS.
 //
-// Measured: gated, 32768 rows of 32 heads of 128, 145 us (805 MB: 5.5 TB/s); add, 16385 rows of 2048, 50 us (268 MB:
-// 5.4 TB/s), both past a large copy's 4.9.  64 rows take 3.4 us, a launch and a load.
+// Measured: gated, 32768 rows of 32 heads of 128, 146 us (805 MB: 5.5 TB/s); add, 16385 rows of 2048, 47 us (268 MB:
+// 5.7 TB/s), both past a large copy's 4.9; without the hints that calls larger than the shared cache give (ONCE) 150 and
+// 49.5.  64 rows take 3.4 us, a launch and a load.
 #include "lq_seq.h"
 
 namespace {
 
 constexpr int TH = 256;
 
-template <int VEC> __device__ __forceinline__ void load_elems(const bf16_t* p, float* f) {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// ONCE: by the hint that nothing here or soon reads these bytes again
+template <int VEC, bool ONCE> __device__ __forceinline__ void load_elems(const bf16_t* p, float* f) {
   if constexpr (VEC == 8) {
-    const uint4 u = *(const uint4*)p;
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    u32x4 w;
+    if (ONCE) w = __builtin_nontemporal_load((const u32x4*)p);
+    else w = *(const u32x4*)p;
 #pragma unroll
     for (int i = 0; i < 4; ++i) { f[2 * i] = bf_lo(w[i]); f[2 * i + 1] = bf_hi(w[i]); }
   } else {
     f[0] = bf2f(*p);
   }
 }
-template <int VEC> __device__ __forceinline__ void store_elems(bf16_t* p, const float* f) {
-  if constexpr (VEC == 8)
-    *(uint4*)p = make_uint4(pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7]));
-  else
+template <int VEC, bool ONCE> __device__ __forceinline__ void store_elems(bf16_t* p, const float* f) {
+  if constexpr (VEC == 8) {
+    const u32x4 w = {pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7])};
+    if (ONCE) __builtin_nontemporal_store(w, (u32x4*)p);
+    else *(u32x4*)p = w;
+  } else {
     *p = f2bf(f[0]);
+  }
 }
 
 // sum over the LANES threads of a row; every thread of the workgroup calls it
@@ -44,7 +52,7 @@ template <int LANES> __device__ __forceinline__ float row_sum(float x, float* ld
   return x;
 }
 
-template <int VEC, int LANES, int CH, bool ADD>
+template <int VEC, int LANES, int CH, bool ADD, bool ONCE>
 __global__ __launch_bounds__(TH) void norm_kernel(lq_norm p) {
   __shared__ float lds[TH / 64];
   const long long v = (long long)blockIdx.x * (TH / LANES) + threadIdx.x / LANES;     // vector: row * heads + head
@@ -59,8 +67,8 @@ __global__ __launch_bounds__(TH) void norm_kernel(lq_norm p) {
   for (int i = 0; i < CH; ++i) {
     const int d = (i * LANES + lane) * VEC;
     if (live && d < p.D) {
-      load_elems<VEC>(x + d, f[i]);
-      load_elems<VEC>(z + d, g[i]);
+      load_elems<VEC, ONCE>(x + d, f[i]);
+      load_elems<VEC, ONCE>(z + d, g[i]);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[i][e] = g[i][e] = 0.f;
@@ -82,7 +90,7 @@ __global__ __launch_bounds__(TH) void norm_kernel(lq_norm p) {
     if (d >= p.D) break;
     float w[VEC], y[VEC];
     if (p.weight_bf16) {
-      load_elems<VEC>((const bf16_t*)p.weight + d, w);
+      load_elems<VEC, false>((const bf16_t*)p.weight + d, w);
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) w[e] = ((const float*)p.weight)[d + e];
@@ -92,17 +100,32 @@ __global__ __launch_bounds__(TH) void norm_kernel(lq_norm p) {
       y[e] = f[i][e] * inv * (p.offset + w[e]);
       if (!ADD) y[e] *= p.act ? fast_sigmoid(g[i][e]) : g[i][e] * fast_sigmoid(g[i][e]);
     }
-    if (ADD) store_elems<VEC>((bf16_t*)p.res + o + d, f[i]);
-    store_elems<VEC>((bf16_t*)p.out + o + d, y);
+    if (ADD) store_elems<VEC, ONCE>((bf16_t*)p.res + o + d, f[i]);
+    store_elems<VEC, ONCE>((bf16_t*)p.out + o + d, y);
   }
 }
 
-template <int VEC, int LANES, int CH, bool ADD>
+template <int VEC, int LANES, int CH, bool ADD, bool ONCE>
 int launch(const lq_norm* p, hipStream_t s) {
   const long long vecs = (long long)p->rows * p->heads, per = TH / LANES, grid = (vecs + per - 1) / per;
   if (grid > 0x7fffffffll) return LQ_ERR_ARG;
-  norm_kernel<VEC, LANES, CH, ADD><<<(unsigned)grid, TH, 0, s>>>(*p);
+  norm_kernel<VEC, LANES, CH, ADD, ONCE><<<(unsigned)grid, TH, 0, s>>>(*p);
   return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
+}
+
+constexpr long long CACHED = 256ll << 20;        // of the cache that all XCDs share
+
+template <bool ADD, bool ONCE>
+int rows_of_8(const lq_norm* p, hipStream_t s) {
+  const int D = p->D;
+  if (D <= 64) return launch<8, 8, 1, ADD, ONCE>(p, s);
+  if (D <= 128) return launch<8, 16, 1, ADD, ONCE>(p, s);
+  if (D <= 256) return launch<8, 32, 1, ADD, ONCE>(p, s);
+  if (D <= 512) return launch<8, 64, 1, ADD, ONCE>(p, s);
+  if (D <= 2048) return launch<8, 256, 1, ADD, ONCE>(p, s);
+  if (D <= 4096) return launch<8, 256, 2, ADD, ONCE>(p, s);
+  if (D <= 8192) return launch<8, 256, 4, ADD, ONCE>(p, s);
+  return launch<8, 256, 8, ADD, ONCE>(p, s);
 }
 
 template <bool ADD>
@@ -116,20 +139,14 @@ int norm(const lq_norm* p, hipStream_t s) {
                        (uintptr_t)(p->weight_bf16 ? p->weight : nullptr);
   const int D = p->D;
   if (D % 8 == 0 && ld % 8 == 0 && (at & 15) == 0) {     // 16-byte loads
-    if (D <= 64) return launch<8, 8, 1, ADD>(p, s);
-    if (D <= 128) return launch<8, 16, 1, ADD>(p, s);
-    if (D <= 256) return launch<8, 32, 1, ADD>(p, s);
-    if (D <= 512) return launch<8, 64, 1, ADD>(p, s);
-    if (D <= 2048) return launch<8, 256, 1, ADD>(p, s);
-    if (D <= 4096) return launch<8, 256, 2, ADD>(p, s);
-    if (D <= 8192) return launch<8, 256, 4, ADD>(p, s);
-    return launch<8, 256, 8, ADD>(p, s);
+    const long long bytes = 2ll * p->rows * p->heads * D * (ADD ? 4 : 3);
+    return bytes > CACHED ? rows_of_8<ADD, true>(p, s) : rows_of_8<ADD, false>(p, s);
   }
-  if (D <= 64) return launch<1, 16, 4, ADD>(p, s);
-  if (D <= 256) return launch<1, 64, 4, ADD>(p, s);
-  if (D <= 1024) return launch<1, 256, 4, ADD>(p, s);
-  if (D <= 4096) return launch<1, 256, 16, ADD>(p, s);
-  return launch<1, 256, 64, ADD>(p, s);
+  if (D <= 64) return launch<1, 16, 4, ADD, false>(p, s);
+  if (D <= 256) return launch<1, 64, 4, ADD, false>(p, s);
+  if (D <= 1024) return launch<1, 256, 4, ADD, false>(p, s);
+  if (D <= 4096) return launch<1, 256, 16, ADD, false>(p, s);
+  return launch<1, 256, 64, ADD, false>(p, s);
 }
 
 }  // namespace

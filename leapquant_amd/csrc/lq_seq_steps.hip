@@ -142,13 +142,15 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
     }
     if (lane < ROWS) out[t * old + lane] = f2bf(keep);
   }
+  // A layer's state is next read after the other layers': 31.8 us instead of 39.4 for KDA, 32 sequences of up to 4 tokens,
+  // 65 instead of 67 for GDN, 64 of up to 8 (with the hint on the loads too 33.6 and 63).
   float* f = p.S + dst * p.slot_stride + head;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float* x = &S[r][4 * e];
-      *(f32x4*)(f + r * K + 32 * e) = f32x4{x[0], x[1], x[2], x[3]} * scale;
+      __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]} * scale, (f32x4*)(f + r * K + 32 * e));
     }
 }
 

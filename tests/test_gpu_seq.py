@@ -467,6 +467,29 @@ def test_norm_graph(seq):
         assert torch.equal(r, r2) and torch.equal(o, o2)
 
 
+@pytest.mark.parametrize("op", ["gated", "add"])
+def test_norm_large_call_equals_its_parts(seq, op):
+    """A call of more bytes than the caches hold against the same rows in smaller calls: the same bits."""
+    rows, D = 23000, 2048
+    g = torch.Generator(device=DEV).manual_seed(39)
+    x, y = (torch.randn(rows, D, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    w = torch.randn(D, generator=g, device=DEV)
+    assert 3 * x.numel() * 2 > 256 << 20
+    a, b = ([torch.empty_like(x) for _ in range(2)] for _ in range(2))
+
+    def run(to, part):
+        if op == "gated":
+            seq.gated_norm(x[part], y[part], w, to[0][part])
+        else:
+            seq.add_norm(x[part], y[part], w, to[0][part], to[1][part], scale=0.5)
+
+    run(a, slice(None))
+    for lo in range(0, rows, 6000):
+        run(b, slice(lo, lo + 6000))
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b[0]) and (op == "gated" or torch.equal(a[1], b[1]))
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 def test_graph_of_conv_and_norms(seq):
     """Replays of the conv and both norms equal the eager results, with other work between."""
