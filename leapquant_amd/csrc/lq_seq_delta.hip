@@ -22,9 +22,10 @@
 // third half would bring the state to the 2e-7 of fp32 sums for half as many matrix instructions again; what reads it
 // rounds it to 8 bits (5e-3 of the outputs), and the outputs are bf16 (1.7e-3).
 //
-// Measured (both kernels, heads of 128 x 128, 16 key and 32 value heads): one prompt of 8192 tokens 206 us (201 MB of tokens
-// and outputs; its 256 steps of 0.68 us are the time), 13 prompts of 32768 tokens 430-470 us (805 MB: 1.8 TB/s; matrix
-// instructions busy 42% of the walk's cycles, vector ones 50%, LDS 45%, at the 1.7 GHz that this mix leaves of the clock).
+// Measured (both kernels, heads of 128 x 128, 16 key and 32 value heads, a call among others): one prompt of 8192 tokens
+// 184 us (201 MB of tokens and outputs; its 256 steps of 0.6 us are the time), 13 prompts of 32768 tokens 413 us (850 MB:
+// 2.1 TB/s; matrix instructions busy 42% of the walk's cycles, vector ones 50%, LDS 45%, at the 1.7 GHz that this mix
+// leaves of the clock).  The kernels' own times below are a profiler's, which stretches the short ones.
 #include <type_traits>
 
 #include "lq_seq.h"
