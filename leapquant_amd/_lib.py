@@ -1,12 +1,15 @@
 """ctypes binding of liblq.so (include/lq.h) and liblq_seq.so (include/lq_seq.h).  The product path has no fallback: if a
 library is missing or a call fails, this raises."""
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_build", "liblq.so")
 SEQ_LIB_PATH = os.path.join(_HERE, "_build", "liblq_seq.so")
+SEQ_CALL_PATH = os.path.join(_HERE, "_build", "lq_seq_call.so")
 ABI_VERSION = 6
 SCHED_INTS = 512           # include/lq.h: LQ_SCHED_INTS
 
@@ -119,6 +122,21 @@ def seq_lib():
     if _SEQ_LIB[0] is None:
         _SEQ_LIB[0] = _load(SEQ_LIB_PATH, SEQ_SIGNATURES)
     return _SEQ_LIB[0]
+
+
+_SEQ_CALL = [None]
+
+
+def seq_call():
+    """The loaded lq_seq_call.so, a Python extension (raises if it has not been built)."""
+    if _SEQ_CALL[0] is None:
+        if not os.path.exists(SEQ_CALL_PATH):
+            raise RuntimeError("%s is missing: build it with python -m leapquant_amd.build" % SEQ_CALL_PATH)
+        loader = importlib.machinery.ExtensionFileLoader("lq_seq_call", SEQ_CALL_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("lq_seq_call", SEQ_CALL_PATH, loader=loader))
+        loader.exec_module(module)
+        _SEQ_CALL[0] = module
+    return _SEQ_CALL[0]
 
 
 _ERR = {-1: "bad argument (unsupported shape / size / pointer)", -2: "HIP launch error",

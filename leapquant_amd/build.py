@@ -1,8 +1,8 @@
 """Builds liblq.so (the HIP kernels + C ABI of include/lq.h) in-tree for gfx950, liblq_seq.so (the operators on whole
-sequences, include/lq_seq.h), and liblq_probe.so (a streaming-read probe that bench.py times as the memory system's ceiling;
-not part of the API).
+sequences, include/lq_seq.h) with lq_seq_call.so (their calls from Python), and liblq_probe.so (a streaming-read probe that
+bench.py times as the memory system's ceiling; not part of the API).
 
-    python -m leapquant_amd.build          # -> leapquant_amd/_build/liblq.so, liblq_seq.so, liblq_probe.so
+    python -m leapquant_amd.build          # -> leapquant_amd/_build/liblq.so, liblq_seq.so, lq_seq_call.so, liblq_probe.so
 
 hipcc cross-compiles without a GPU.  Every HIP file gets `-Xclang -target-feature -Xclang -packed-fp32-ops` (no
 packed FP32 instructions in the device code).
@@ -11,6 +11,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -19,6 +20,7 @@ LIB = os.path.join(OUT, "liblq.so")
 SOURCES = ("lq_step.hip", "lq_step_bf16.hip", "lq_flush.hip", "lq_dequant.hip", "lq_dense.hip", "lq_noalloc.hip")
 SEQ_LIB = os.path.join(OUT, "liblq_seq.so")
 SEQ_SOURCES = ("lq_seq_conv.hip", "lq_seq_norm.hip", "lq_seq_steps.hip", "lq_seq_delta.hip")
+SEQ_CALL = os.path.join(OUT, "lq_seq_call.so")
 PROBE_LIB = os.path.join(OUT, "liblq_probe.so")
 PROBE_SOURCES = ("lq_probe.hip",)
 ARCH = os.environ.get("LQ_OFFLOAD_ARCH", "gfx950")
@@ -57,6 +59,24 @@ def _compile_link(cc, flags, sources, lib, verbose):
     os.replace(tmp, lib)
 
 
+def _build_call():
+    """The Python extension in front of liblq_seq.so: host C++ on torch's tensors, found beside the library it calls."""
+    import torch
+    t = os.path.dirname(torch.__file__)
+    rocm = os.path.dirname(os.path.dirname(hipcc())) if os.path.sep in hipcc() else "/opt/rocm"
+    tmp = SEQ_CALL + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           os.path.join(CSRC, "lq_seq_call.cpp"), "-o", tmp]
+    cmd += ["-isystem" + d for d in (os.path.join(t, "include"), os.path.join(t, "include", "torch", "csrc", "api", "include"),
+                                     os.path.join(rocm, "include"), sysconfig.get_paths()["include"])]
+    cmd += ["-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10", "-L" + OUT, "-llq_seq",
+            "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("building lq_seq_call.so failed:\n%s" % r.stderr)
+    os.replace(tmp, SEQ_CALL)
+
+
 def build(verbose=False):
     os.makedirs(OUT, exist_ok=True)
     cc = hipcc()
@@ -68,6 +88,7 @@ def build(verbose=False):
              "-mllvm", "-amdgpu-atomic-optimizer-strategy=None"]
     _compile_link(cc, flags, SOURCES, LIB, verbose)
     _compile_link(cc, flags, SEQ_SOURCES, SEQ_LIB, verbose)
+    _build_call()
     _compile_link(cc, flags, PROBE_SOURCES, PROBE_LIB, verbose)
     return LIB
 

@@ -24,6 +24,7 @@ from .kernels import GDN_DIMS, _raw_stream, conv_struct
 _ACT = {"silu": 0, "sigmoid": 1}
 _F32, _BF16, _I32 = torch.float32, torch.bfloat16, torch.int32
 _KDA_DIMS = ((128, 128),)
+_NOT_PLAIN = 1           # lq_seq_call: arguments to be converted or refused below; nothing was launched
 
 
 def _on(dev, **tensors):
@@ -125,6 +126,9 @@ def delta_prefill(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, sc
     [T, 2HK + HV V] after the conv, q | k | v; a, b: bf16 [T, HV] raw gates.  The three may be column ranges of wider rows.
     A_log, dt_bias: [HV].  out: bf16 [T, HV, V].  scale: of the queries, K^-1/2 by default.  Gates, norms and state as the
     decode step's, with beta = sigmoid(b) not rounded.  A NaN or infinity in a token reaches all tokens of its chunk of 32."""
+    rc = _lib.seq_call().delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, False, 0.0, True)
+    if rc != _NOT_PLAIN:
+        return _lib.check(rc, "lq_delta_prefill")
     d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, False, 0.0, chunks=True)
     L = _lib.seq_lib()
     n = L.lq_delta_workspace(d, seqs)
@@ -138,6 +142,9 @@ def delta_steps(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, scal
     0, its bounded gate gate_lower_bound * sigmoid(exp(A_log) (a + dt_bias))."""
     if gate_lower_bound and not kda:
         raise ValueError("gate_lower_bound: KDA only")
+    rc = _lib.seq_call().delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, bool(kda), gate_lower_bound, False)
+    if rc != _NOT_PLAIN:
+        return _lib.check(rc, "lq_delta_steps")
     d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, bool(kda), gate_lower_bound)
     _lib.check(_lib.seq_lib().lq_delta_steps(d, seqs, _raw_stream(S)), "lq_delta_steps")
 
@@ -146,6 +153,9 @@ def conv_prefill(x, conv_state, weight, bias, idx, loc, out, src=None, silu=True
     """The depthwise causal conv1d of width 4 over a ragged batch: out [T, C] (bf16) from the packed tokens x [T, C] (bf16,
     possibly a column range of wider rows), out_t = act(sum_j w_j x_{t-3+j} + bias).  conv_state [NS, C, 3] (any strides): the
     inputs before a sequence's first token come from its slot src, its last three are left in slot idx."""
+    rc = _lib.seq_call().conv(x, conv_state, weight, bias, idx, loc, out, src, bool(silu))
+    if rc != _NOT_PLAIN:
+        return _lib.check(rc, "lq_conv_seq")
     if x.dim() != 2:
         raise ValueError("x: [T, C] expected, got shape %s" % (tuple(x.shape),))
     T, C = x.shape
@@ -198,6 +208,9 @@ def gated_norm(x, z, weight, out, eps=1e-6, gate="silu", offset=0.0):
     bf16 [D]; offset 1 for weights stored around zero.  out may be x."""
     if gate not in _ACT:
         raise ValueError("gate: 'silu' or 'sigmoid' expected, got %r" % (gate,))
+    rc = _lib.seq_call().norm(x, z, weight, out, None, eps, 0.0, offset, _ACT[gate], False)
+    if rc != _NOT_PLAIN:
+        return _lib.check(rc, "lq_gated_norm")
     n = _norm(x, z, weight, out, None, eps, 0.0, offset, _ACT[gate])
     _lib.check(_lib.seq_lib().lq_gated_norm(n, _raw_stream(x)), "lq_gated_norm")
 
@@ -206,5 +219,8 @@ def add_norm(x, y, weight, res, out, eps=1e-6, scale=1.0, offset=0.0):
     """The residual add and the norm before the next block: res = x + scale y, out = res rsqrt(mean(res^2) + eps)
     (offset + weight), of the sum before it is rounded to bf16.  Shapes as `gated_norm`; res and out are laid out alike; res
     may be x or y (in place)."""
+    rc = _lib.seq_call().norm(x, y, weight, out, res, eps, scale, offset, 0, True)
+    if rc != _NOT_PLAIN:
+        return _lib.check(rc, "lq_add_norm")
     n = _norm(x, y, weight, out, res, eps, scale, offset, 0)
     _lib.check(_lib.seq_lib().lq_add_norm(n, _raw_stream(x)), "lq_add_norm")

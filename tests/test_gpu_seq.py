@@ -490,6 +490,35 @@ def test_norm_large_call_equals_its_parts(seq, op):
     assert torch.equal(a[0], b[0]) and (op == "gated" or torch.equal(a[1], b[1]))
 
 
+def test_direct_and_checked_calls_agree(seq, monkeypatch):
+    """Arguments as the kernels read them go straight to the library; the same call through the Python checks (64-bit indexes,
+    half-precision gates' copies) leaves the same bits."""
+    d = R.delta_inputs(43, [40, 3], 4, 2, 128, 128)
+    d["A_log"] = d["A_log"].half().float()
+    g = gpu(d)
+    x, w = g["mixed"], torch.randn(g["mixed"].shape[1], 4, device=DEV).to(torch.bfloat16)
+    taps = torch.randn(5, x.shape[1], 3, device=DEV).to(torch.bfloat16)
+    nw = torch.nn.Parameter(torch.randn(x.shape[1], device=DEV))
+
+    def run(**kw):
+        e = dict(g, **kw)
+        out = [run_delta(fn, e, 2) for fn in (seq.delta_prefill, seq.delta_steps)] + [e["S"].clone()]
+        y, t = torch.empty_like(x), taps.clone()
+        seq.conv_prefill(x, t, w, None, e["idx"], e["loc"], y, src=e["src"])
+        n, r, o = (torch.empty_like(x) for _ in range(3))
+        seq.gated_norm(y, x, nw, n)
+        seq.add_norm(x, n, nw, r, o, scale=0.5)
+        torch.cuda.synchronize()
+        return out + [y, t, n, r, o]
+
+    checked = run(idx=g["idx"].long(), loc=g["loc"].long(), A_log=g["A_log"].half())
+    with monkeypatch.context() as m:
+        for name in ("_delta", "_norm", "_batch"):
+            m.setattr(seq, name, None)                    # not to be reached
+        direct = run()
+    assert all(torch.equal(a, b) for a, b in zip(checked, direct))
+
+
 # ---- together -----------------------------------------------------------------------------------------------------------
 def test_graph_of_conv_and_norms(seq):
     """Replays of the conv and both norms equal the eager results, with other work between."""

@@ -178,3 +178,20 @@ def test_norm_and_conv_arguments():
                  lambda: seq.conv_prefill(x, st, cw, None, i, l[:1], x)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_direct_calls_leave_all_else_to_the_operators():
+    """What the extension in front of the library does not take as it is, it hands back without a launch or an error."""
+    from leapquant_amd import _lib
+    c = _lib.seq_call()
+    t, n = torch.zeros(2, 8, dtype=torch.bfloat16), c.NOT_PLAIN
+    idx = torch.zeros(2, dtype=torch.int32)
+    for bad in (t, None, 3, "x"):
+        assert c.norm(bad, t, t[0], t, None, 1e-6, 0.0, 0.0, 0, False) == n
+        assert c.norm(t, t, t[0], t, bad, 1e-6, 0.0, 0.0, 0, True) == n
+        assert c.conv(bad, t, t, None, idx, idx, t, None, True) == n
+        assert c.delta(bad, t, t, t, t, t, idx, idx, t, None, 2, None, False, 0.0, True) == n
+    assert c.norm() == c.conv() == c.delta() == n
+    from leapquant_amd import seq
+    with pytest.raises(ValueError):
+        seq.gated_norm(t, t, torch.ones(8), t)
