@@ -195,3 +195,20 @@ def test_direct_calls_leave_all_else_to_the_operators():
     from leapquant_amd import seq
     with pytest.raises(ValueError):
         seq.gated_norm(t, t, torch.ones(8), t)
+
+
+def test_state_prefill_refuses():
+    from leapquant_amd.state import LeapQuantState
+    ssm = torch.zeros(3, 4, 128, 128)
+    st = LeapQuantState(ssm, 2)
+    mixed, a = torch.zeros(5, 1024, dtype=torch.bfloat16), torch.zeros(5, 4, dtype=torch.bfloat16)
+    out, p = torch.zeros(5, 4, 128, dtype=torch.bfloat16), torch.zeros(4)
+    idx, loc = torch.tensor([1, 2], dtype=torch.int32), torch.tensor([0, 2, 5], dtype=torch.int32)
+    with pytest.raises(ValueError, match="idx"):
+        st.prefill(ssm, mixed, a, a, p, p, idx[None], loc, out)
+    with pytest.raises(ValueError, match="has_state"):
+        st.prefill(ssm, mixed, a, a, p, p, idx, loc, out, has_state=torch.ones(3, dtype=torch.bool))
+    with pytest.raises(ValueError, match="GPU"):
+        st.prefill(ssm, mixed, a, a, p, p, idx, loc, out)
+    with pytest.raises(ValueError, match="mixed"):
+        st.prefill(ssm, mixed[:, 1:], a, a, p, p, idx, loc, out)
