@@ -371,7 +371,8 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
 //
 // A step ends when the slowest wave has done its part.  Of its 1500 cycles the state's waves work 1390, the chain 1110, the
 // others 820 to 1190, and LDS moves 125 KB, 970 cycles' worth.  8192 tokens take 173 us; with X through LDS between 185 to
-// 199.  Not kept: X from the first kernel (166, but 8 more there), X by one wave (183), 32 channels a state wave (218: LDS).
+// 199.  Not kept: X from the first kernel (166, but 8 more there), X by one wave (183), 32 channels a state wave (218: LDS),
+// a step's tiles read into registers a step ahead (177 to 189: the reads then stand before the step's end).
 constexpr int AHEAD = 2;               // chunks requested before the step that first needs one
 constexpr int SERVICE = 4;             // service waves of a workgroup
 constexpr int ROLES = 4;               // waves of 16 rows of the state: chain, two halves of the channels, outputs
@@ -717,7 +718,7 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
   else walk.service(w - ROLES, work + ((long long)(lo / C + sn) * p.HV + hv));
 }
 
-// ---- the walk with a wave alone for 16 rows ------------------------------------------------------------------------------------
+// ---- the walk with a wave alone for 16 rows --------------------------------------------------------------------------------
 // All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all (351 a chunk, 60 of them matrix
 // ones), and LDS for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768
 // tokens: 348 us.  A third workgroup a CU (LDS 32 bytes smaller) gains 2%, 32 columns a wave lose 18% (registers).

@@ -28,7 +28,7 @@ __device__ __forceinline__ float gate_of(float x, float ea, float glb) {
 
 constexpr int BLOCK = 8;                         // tokens whose KDA gates a workgroup forms at once
 
-template <int K, int V, int ROWS, bool KDA>
+template <int K, int V, int ROWS, bool KDA, bool PAST>
 __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
   constexpr int E = K / 32;                      // float4 groups a lane
   constexpr int PARTS = V / (32 * ROWS);         // workgroups a head
@@ -142,15 +142,16 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
     }
     if (lane < ROWS) out[t * old + lane] = f2bf(keep);
   }
-  // A layer's state is next read after the other layers': 31.8 us instead of 39.4 for KDA, 32 sequences of up to 4 tokens,
-  // 65 instead of 67 for GDN, 64 of up to 8 (with the hint on the loads too 33.6 and 63).
   float* f = p.S + dst * p.slot_stride + head;
 #pragma unroll
   for (int r = 0; r < ROWS; ++r)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float* x = &S[r][4 * e];
-      __builtin_nontemporal_store(f32x4{x[0], x[1], x[2], x[3]} * scale, (f32x4*)(f + r * K + 32 * e));
+      const f32x4 y = f32x4{x[0], x[1], x[2], x[3]} * scale;
+      f32x4* to = (f32x4*)(f + r * K + 32 * e);
+      if (PAST) __builtin_nontemporal_store(y, to);
+      else *to = y;
     }
 }
 
@@ -158,7 +159,11 @@ template <int K, int V, int ROWS, bool KDA>
 int launch_rows(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
   const long long grid = (long long)s->N * d->HV * (V / (32 * ROWS));
   if (grid > 0x7fffffffll) return LQ_ERR_ARG;
-  steps_kernel<K, V, ROWS, KDA><<<(unsigned)grid, 256, 0, st>>>(*d, *s);
+  // States that fit the shared cache are written past it, which leaves it to those that are read: where one layer's states take
+  // turns in it, 64 sequences of 8 tokens take 68 us instead of 77, 32 of 4 (KDA) 35 instead of 39; where other data fill
+  // it, the same.  Beyond its size that gains nothing, and after other writes 256 sequences lose 18%.
+  if (4ll * s->N * d->HV * V * K <= 256ll << 20) steps_kernel<K, V, ROWS, KDA, true><<<(unsigned)grid, 256, 0, st>>>(*d, *s);
+  else steps_kernel<K, V, ROWS, KDA, false><<<(unsigned)grid, 256, 0, st>>>(*d, *s);
   return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
 }
 template <int K, int V, bool KDA>
