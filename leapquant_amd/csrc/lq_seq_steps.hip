@@ -15,8 +15,10 @@
 // exponentials and a reciprocal for each key channel, are the same for all rows: the workgroup forms those of 8 tokens at once.
 //
 // Measured, heads of 128 x 128: 256 sequences of one token and 32 heads 205 us (1.07 GB: 5.2 TB/s, a copy's rate), 64 of one
-// 69 us (3.9 TB/s), 64 of 8 tokens 94 us, where the vector units take over (2.7 us a token); one sequence of one token 5 us,
-// the chain of its loads.
+// 68 us (3.9 TB/s), 64 of 8 tokens 90 us, where the vector units take over (2 us a token); one sequence of one token 5 us, the
+// chain of its loads, of 32 tokens 26 us.  (Caches full of other data; 40, 61 and 21 us where they hold states.)  Norms, gates
+// and beta come from the hardware's reciprocal square root, exp2, log and reciprocal, 1 ulp each: with the library's 7 to
+// 10% of a token's time more.
 #include "lq_seq.h"
 
 namespace {
@@ -114,7 +116,7 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
       nq = fmaf(q[i], q[i], nq); nk = fmaf(k[i], k[i], nk); kq = fmaf(k[i], q[i], kq);
     }
     nq = sum8(nq); nk = sum8(nk); kq = sum8(kq);
-    const float iq = rsqrtf_rn(nq + 1e-6f) * p.scale, ik = rsqrtf_rn(nk + 1e-6f);
+    const float iq = __builtin_amdgcn_rsqf(nq + 1e-6f) * p.scale, ik = __builtin_amdgcn_rsqf(nk + 1e-6f);
     kq *= iq * ik;
     if (!KDA && scale < 0x1p-20f) {              // before 1 / scale grows large
 #pragma unroll
