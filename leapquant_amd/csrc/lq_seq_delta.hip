@@ -15,17 +15,19 @@
 // X_c = K_c K_{c-1}^T: the product with the state is a chunk old when it is needed, and a second wave keeps the state.
 //
 // Rounding.  The raw keys, queries and values are bf16 and enter the products as they are; their norms, decays and beta are
-// fp32 factors of rows and columns of fp32 sums, never folded into an operand.  fp32 operands (S, R, T', W, X, T' R) are
-// carried as two bf16 halves (hi + lo: at most 2^-16 of an element is lost, 2.8e-6 in the mean), their products as the two or
-// three significant ones: the state ends within 5e-6 of its norm, where single bf16 operands would leave 3e-3, and the
-// outputs keep their digits where their terms cancel (a query nearly orthogonal to the state, equal keys in a chunk).  A
-// third half would bring the state to the 2e-7 of fp32 sums for half as many matrix instructions again; what reads it
-// rounds it to 8 bits (5e-3 of the outputs), and the outputs are bf16 (1.7e-3).
+// fp32 factors of rows and columns of fp32 sums, never folded into an operand.  fp32 operands are carried in bf16 parts, each
+// 2.8e-6 (two parts) or 5e-9 (three) of the operand short in the mean.  What is appended to the state and leads to it (T', R,
+// T' R, X) has three: errors of its terms do not cancel where the terms do, as with equal keys in a chunk.  The state ends
+// within 8e-7 of its norm, 2e-7 in the median (fp32 sums: 2e-7); with two parts within 6e-6, and 2e-5 where appended values
+// cancel, for 12% less time.  What is read of the state (S in K S and Q S) and W have two: a third in K S takes 12% more time
+// for the rest of the difference, and the outputs are bf16 (1.7e-3); single bf16 operands would lose digits where their
+// terms cancel (a query nearly orthogonal to the state, equal keys).
 //
 // Measured (both kernels, heads of 128 x 128, 16 key and 32 value heads, a call among others): one prompt of 8192 tokens
-// 184 us (201 MB of tokens and outputs; its 256 steps of 0.6 us are the time), 13 prompts of 32768 tokens 413 us (850 MB:
-// 2.1 TB/s; matrix instructions busy 42% of the walk's cycles, vector ones 50%, LDS 45%, at the 1.7 GHz that this mix
-// leaves of the clock).  The kernels' own times below are a profiler's, which stretches the short ones.
+// 204 us (201 MB of tokens and outputs; its 256 steps of 0.65 us are the time), 13 prompts of 32768 tokens 476 us (850 MB:
+// 1.8 TB/s; with two parts everywhere, 414 us, matrix instructions were busy 42% of the walk's cycles, vector ones 50%, LDS
+// 45%, at the 1.7 GHz that this mix leaves of the clock).  The kernels' own times below are a profiler's, which stretches
+// the short ones.
 #include <type_traits>
 
 #include "lq_seq.h"
@@ -48,36 +50,49 @@ __device__ __forceinline__ f32x4 mf(const bf16x4& a, const bf16x4& b, const f32x
   return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ bf16x4 first4(const bf16x8& a) { return __builtin_shufflevector(a, a, 0, 1, 2, 3); }
-// four or eight fp32 values as two bf16 halves
-__device__ __forceinline__ void split4(const f32x4& x, bf16x4& hi, bf16x4& lo) {
-  u32x2 h, l;
+// four or eight fp32 values as two or three bf16 parts
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pk_bf16_kept(x, y);
+  lo = pk_bf16_kept(x - bf_lo(hi), y - bf_hi(hi));
+}
+__device__ __forceinline__ uint32_t third2(float x, float y, uint32_t hi, uint32_t lo) {
+  return pk_bf16(x - bf_lo(hi) - bf_lo(lo), y - bf_hi(hi) - bf_hi(lo));
+}
+__device__ __forceinline__ void split4(const f32x4& x, bf16x4& hi, bf16x4& lo, bf16x4* third = nullptr) {
+  u32x2 h, l, t;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    h[i] = pk_bf16_kept(x[2 * i], x[2 * i + 1]);
-    l[i] = pk_bf16(x[2 * i] - bf_lo(h[i]), x[2 * i + 1] - bf_hi(h[i]));
+    uint32_t a, b;
+    split2(x[2 * i], x[2 * i + 1], a, b);
+    h[i] = a; l[i] = b;
+    if (third) t[i] = third2(x[2 * i], x[2 * i + 1], a, b);
   }
   hi = __builtin_bit_cast(bf16x4, h);
   lo = __builtin_bit_cast(bf16x4, l);
+  if (third) *third = __builtin_bit_cast(bf16x4, t);
 }
-__device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, bf16x8& hi, bf16x8& lo) {
+__device__ __forceinline__ void split8(const f32x4& x, const f32x4& y, bf16x8& hi, bf16x8& lo, bf16x8* third = nullptr) {
   const float f[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-  u32x4 h, l;
+  u32x4 h, l, t;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    h[i] = pk_bf16_kept(f[2 * i], f[2 * i + 1]);
-    l[i] = pk_bf16(f[2 * i] - bf_lo(h[i]), f[2 * i + 1] - bf_hi(h[i]));
+    uint32_t a, b;
+    split2(f[2 * i], f[2 * i + 1], a, b);
+    h[i] = a; l[i] = b;
+    if (third) t[i] = third2(f[2 * i], f[2 * i + 1], a, b);
   }
   hi = __builtin_bit_cast(bf16x8, h);
   lo = __builtin_bit_cast(bf16x8, l);
+  if (third) *third = __builtin_bit_cast(bf16x8, t);
 }
 
 // What the first kernel leaves for a chunk of a value head.  The matrices are operands as a lane takes them: lane l of a row
 // tile holds row l % 16 at the columns 4 g .. 4 g + 3 and 16 + 4 g .. (g = l / 16), the order in which a lane of a product's
 // result holds its rows, so that results are the next product's operands without moving between lanes.  The first row tile's
-// columns 16 .. are zero and left out.  High and low half of each.
+// columns 16 .. are zero and left out.  T' in three parts, W in two.
 struct alignas(16) Coef {
-  bf16x4 t0[2][64], w0[2][64];
-  bf16x8 t1[2][64], w1[2][64];
+  bf16x4 t0[3][64], w0[2][64];
+  bf16x8 t1[3][64], w1[2][64];
   float c[C];                          // e^G / |k|: of the rows of K S
   float d[C];                          // scale e^G / |q|: of the rows of Q S
   float last[4];                       // e^{G_C}
@@ -133,16 +148,26 @@ __device__ __forceinline__ Place place_of(int b, int items, int M) {
 }
 inline long long place_grid(long long items, int M) { return (items < 8 ? items : (items + 7) / 8 * 8) * M; }
 
-// T' or W of a chunk times R (or any 32 rows held as their halves), onto acc
-__device__ __forceinline__ void chunk_product(const bf16x4 (&m0)[2][64], const bf16x8 (&m1)[2][64], const bf16x8& rh,
-                                              const bf16x8& rl, int l, const f32x4& a0, const f32x4& a1, f32x4 (&y)[2]) {
-  f32x4 y0 = a0, y1 = a1;
-  y0 = mf(m0[0][l], first4(rh), y0);
-  y1 = mf(m1[0][l], rh, y1);
-  y0 = mf(m0[0][l], first4(rl), y0);
-  y1 = mf(m1[0][l], rl, y1);
-  y[0] = mf(m0[1][l], first4(rh), y0);
-  y[1] = mf(m1[1][l], rh, y1);
+// T' or W of a chunk, in N parts, times R, onto y: the products that reach the N-th part's digits
+template <int N> struct Operand { bf16x4 m0[N]; bf16x8 m1[N]; };
+template <int N> __device__ __forceinline__ Operand<N> operand(const bf16x4 (&m0)[N][64], const bf16x8 (&m1)[N][64], int l) {
+  Operand<N> m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    m.m0[i] = m0[i][l];
+    m.m1[i] = m1[i][l];
+  }
+  return m;
+}
+template <int N>
+__device__ __forceinline__ void chunk_product(const Operand<N>& m, const bf16x8 (&r)[N], f32x4 (&y)[2]) {
+#pragma unroll
+  for (int a = 0; a < N; ++a)
+#pragma unroll
+    for (int b = 0; a + b < N; ++b) {
+      y[0] = mf(m.m0[a], first4(r[b]), y[0]);
+      y[1] = mf(m.m1[a], r[b], y[1]);
+    }
 }
 // a result's rows, tokens, that there are: this lane's offsets from the chunk's first token, and their stores
 __device__ __forceinline__ void store_places(unsigned (&at)[8], unsigned old, int n, int g) {
@@ -164,7 +189,7 @@ __device__ __forceinline__ void store_chunk(char* out, const unsigned (&at)[8], 
 }
 
 // ---- T' and W of every chunk ---------------------------------------------------------------------------------------------
-// 33 us for 8192 tokens (256 chunks, 32 heads), 125 us for 32768: 500 MB of keys, queries and results, 4 TB/s, and 53% of the
+// 35 us for 8192 tokens (256 chunks, 32 heads), 130 us for 32768: 530 MB of keys, queries and results, 4 TB/s, and 53% of the
 // vector units' cycles.  One wave a chunk and value head.  (I + A)^-1 by forward substitution in its two diagonal blocks of 16
 // (a column a lane) and -T11 A10 T00 below them by fp32 matrix instructions: substitution stays accurate where powers of A
 // would not (equal keys without decay make them grow like binomials).
@@ -350,8 +375,9 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
     const float e0 = exp_f((gh - my.ghi[n]) + (gl - my.glo[n])) * my.rk[n];
     const float e1 = exp_f((gh - my.ghi[16 + n]) + (gl - my.glo[16 + n])) * my.rk[16 + n];
     bf16x8 hi, lo;
-    split4(*(const f32x4*)&my.m[n][4 * g] * b0 * e0, out.t0[0][l], out.t0[1][l]);
-    split8(*(const f32x4*)&my.m[16 + n][4 * g] * b0 * e1, *(const f32x4*)&my.m[16 + n][16 + 4 * g] * b1 * e1, hi, lo);
+    split4(*(const f32x4*)&my.m[n][4 * g] * b0 * e0, out.t0[0][l], out.t0[1][l], &out.t0[2][l]);
+    split8(*(const f32x4*)&my.m[16 + n][4 * g] * b0 * e1,
+           *(const f32x4*)&my.m[16 + n][16 + 4 * g] * b1 * e1, hi, lo, &out.t1[2][l]);
     out.t1[0][l] = hi; out.t1[1][l] = lo;
     spread(ww[0], ww[1], ww[2]);
     split4(*(const f32x4*)&my.m[n][4 * g] * b0, out.w0[0][l], out.w0[1][l]);
@@ -369,16 +395,17 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
 // Chunk c is requested in step c - 1 - AHEAD, has landed when step c - 1 begins, and meets the waves in the steps c - 1 (K in
 // K_c S_{c-1} and X), c (Q, V, T', c, ..) and c + 1 (K^T in the state's update, W, d, e^{G_C}).
 //
-// A step ends when the slowest wave has done its part.  Of its 1500 cycles the state's waves work 1390, the chain 1110, the
-// others 820 to 1190, and LDS moves 125 KB, 970 cycles' worth.  8192 tokens take 173 us; with X through LDS between 185 to
-// 199.  Not kept: X from the first kernel (166, but 8 more there), X by one wave (183), 32 channels a state wave (218: LDS),
-// a step's tiles read into registers a step ahead (177 to 189: the reads then stand before the step's end).
+// A step ends when the slowest wave has done its part.  8192 tokens take 202 us.  With two parts everywhere it was 173: of a
+// step's 1500 cycles the state's waves worked 1390, the chain 1110, the others 820 to 1190, and LDS moved 125 KB, 970 cycles'
+// worth.  X by way of LDS to its operand's layout took 12 us more.  Not kept (of 173): X from the first kernel (166, but 8 more
+// there), X by one wave (183), 32 channels a state wave (218: LDS), a step's tiles read into registers a step ahead (177 to
+// 189: the reads then stand before the step's end).
 constexpr int AHEAD = 2;               // chunks requested before the step that first needs one
 constexpr int SERVICE = 4;             // service waves of a workgroup
 constexpr int ROLES = 4;               // waves of 16 rows of the state: chain, two halves of the channels, outputs
 struct Pass {                          // between the waves of 16 rows, of one step
   f32x4 kp[2][2][64], qs[2][2][64];    // K S, Q S of a half of the channels: row tile
-  bf16x8 r[2][64], u[2][64];           // R, T' R: high and low half
+  bf16x8 r[2][64], u[3][64];           // R, T' R in parts, the highest first
 };
 constexpr int PASS = (int)sizeof(Pass) / 16;
 
@@ -386,14 +413,13 @@ template <int K>
 struct Tiles {                         // places in LDS, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB;                    // blocks of a row of K, of a tile
   static constexpr int VB = 2, VU = C * VB;                        // the same of the workgroup's columns of V
-  static constexpr int CU = (int)sizeof(Coef) / 16, CN = 7;
+  static constexpr int CU = (int)sizeof(Coef) / 16, CN = 8;
   static constexpr int KN = AHEAD + 3, QN = AHEAD + 2, VN = AHEAD + 2;
   static constexpr int QAT = KN * TU, VAT = QAT + QN * TU, CAT = VAT + VN * VU, XAT = CAT + KN * CN * 64;
-  static constexpr int PAT = XAT + 2 * 4 * 64, END = PAT + 2 * PASS, BYTES = 16 * END;      // PAT: what the waves pass on
-  // loads of a service wave for a chunk, the same for each (the last one of the last wave is V), so that one count says what
-  // is still on its way
-  static constexpr int LOADS = 2 * TU / 64 / SERVICE + (CN + 1) / SERVICE;
-  static_assert(VU == 64 && CN * 64 >= CU && (CN + 1) % SERVICE == 0, "loads of a chunk");
+  static constexpr int PAT = XAT + 2 * 6 * 64, END = PAT + 2 * PASS, BYTES = 16 * END;      // PAT: what the waves pass on
+  // loads of a service wave for a chunk, the same for each (all four load V), so that one count says what is still on its way
+  static constexpr int LOADS = 2 * TU / 64 / SERVICE + CN / SERVICE + 1;
+  static_assert(VU == 64 && CN * 64 >= CU && CN % SERVICE == 0, "loads of a chunk");
   static_assert(BYTES <= 160 * 1024, "LDS of a CU");
   static_assert(LOADS < 64, "what a wave may have outstanding");
 };
@@ -411,7 +437,7 @@ struct Walk {
   static __device__ __forceinline__ int before(int at) { return at == 0 ? B::KN - 1 : at - 1; }
   __device__ __forceinline__ const u32x4* ktile(int at) const { return lds + at * TU; }
   __device__ __forceinline__ const Coef& coef(int at) const { return *(const Coef*)(lds + B::CAT + at * B::CN * 64); }
-  __device__ __forceinline__ bf16x8* xtile(int c) const { return (bf16x8*)(lds + B::XAT + (c & 1) * 256); }
+  __device__ __forceinline__ bf16x8* xtile(int c) const { return (bf16x8*)(lds + B::XAT + (c & 1) * 384); }
   __device__ __forceinline__ Pass& pass(int c) const { return ((Pass*)(lds + B::PAT))[c & 1]; }
 
   // the order of what comes before: N matrix instructions with M vector ones under each, and LDS reads among the first
@@ -433,15 +459,15 @@ struct Walk {
     const char* vb = rows + 2u * (2 * p.H * K + hv * V + part * 16);
     const char* cb = (const char*)work;
     const int xi = k >> 1, xe = k & 1;           // rows of this chunk, of the one before
-    constexpr int TL = TU / 64 / SERVICE, CL = (B::CN + 1) / SERVICE;
-    unsigned toff[TL], coff[CL];                 // this lane's offsets from a chunk's first row, past its last row that row's
+    constexpr int TL = TU / 64 / SERVICE, CL = B::CN / SERVICE;
+    unsigned toff[TL], coff[CL], voff;               // this lane's offsets from a chunk's first row, past its last row that row's
     auto place = [&](int count) {
 #pragma unroll
       for (int i = 0; i < TL; ++i) {
         const int u = l + 64 * (SERVICE * i + k), r = u / RB;
         toff[i] = (unsigned)min(r, count - 1) * ld + 16u * ((u % RB) ^ swz(r, RB));
       }
-      if (k == SERVICE - 1) coff[CL - 1] = (unsigned)min(l / VB, count - 1) * ld + 16u * ((l % VB) ^ swz(l / VB, VB));
+      voff = (unsigned)min(l / VB, count - 1) * ld + 16u * ((l % VB) ^ swz(l / VB, VB));
     };
 #pragma unroll
     for (int i = 0; i < CL; ++i) coff[i] = 16u * min(l + 64 * (CL * k + i), B::CU - 1);
@@ -460,8 +486,8 @@ struct Walk {
           to_lds(qb, toff[i], qa + 1024u * SERVICE * i);
         }
 #pragma unroll
-        for (int i = 0; i < CL - 1; ++i) to_lds(cb, coff[i], ca + 1024u * i);
-        to_lds(k < SERVICE - 1 ? cb : vb, coff[CL - 1], k < SERVICE - 1 ? ca + 1024u * (CL - 1) : va);
+        for (int i = 0; i < CL; ++i) to_lds(cb, coff[i], ca + 1024u * i);
+        to_lds(vb, voff, va);
         kb += (long long)C * ld; qb += (long long)C * ld; vb += (long long)C * ld;
         cb += (long long)p.HV * sizeof(Coef);
       }
@@ -474,11 +500,8 @@ struct Walk {
           xx = mf(__builtin_bit_cast(bf16x8, ko[at]), __builtin_bit_cast(bf16x8, kt[at]), xx);
         }
         // X's transpose as a result: a lane has row n of X at the columns 4 g .., as the chain takes it
-        bf16x4 hi, lo;
-        split4(xx, hi, lo);
-        bf16x4* out = (bf16x4*)(xtile(s + 1) + 128 * xi + l) + xe;
-        out[0] = hi;
-        out[128] = lo;
+        bf16x4* out = (bf16x4*)(xtile(s + 1) + 192 * xi + l) + xe;
+        split4(xx, out[0], out[128], &out[256]);
       }
       // what the next step needs has landed; this step's request may still be on its way
       if (j < nc) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(B::LOADS) : "memory");
@@ -522,7 +545,7 @@ struct Walk {
       Pass& out = pass(t);
       const float next = t < 0 || t == nc ? 1.f : coef(tk).last[0];
       tk = after(tk);
-      bf16x8 uh, ul, kf[2][2], qf[2][2], sh[2], sl[2];
+      bf16x8 u[3], kf[2][2], qf[2][2], sh[2], sl[2];
       auto fetch = [&](int x) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -532,7 +555,8 @@ struct Walk {
       };
       s16x4 k2[KH][2][2];                        // channels 32 x + 8 q + 4 h ..; row 16 + .. has the same column place
       if (update) {
-        uh = in.u[0][l]; ul = in.u[1][l];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) u[i] = in.u[i][l];
 #pragma unroll
         for (int x = 0; x < KH; ++x)
 #pragma unroll
@@ -546,12 +570,12 @@ struct Walk {
       auto advance = [&](int x) {
         bf16x8 kT[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
           kT[h] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(k2[x][h][0], k2[x][h][1], 0, 1, 2, 3, 4, 5, 6, 7));
-          S[x][h] = mf(kT[h], uh, S[x][h]);
-        }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) S[x][h] = mf(kT[h], ul, S[x][h]);
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) S[x][h] = mf(kT[h], u[i], S[x][h]);
       };
       f32x4 kp[2] = {}, qs[2] = {};
       auto products = [&](int x) {
@@ -610,7 +634,7 @@ struct Walk {
   // ---- the wave that walks the chain R -> T' R -> R of these rows ----
   __device__ __forceinline__ void chain() const {
     const int l = threadIdx.x & 63, n = l & 15, g = l >> 4, qrow = 4 * g + (n >> 2);
-    bf16x8 uh = {}, ul = {};
+    bf16x8 u[3] = {};
     int tk = 0;                                  // place of chunk t
     auto step = [&](int t, bool first) {
       const Coef& ck = coef(tk);
@@ -625,9 +649,11 @@ struct Walk {
 #pragma unroll
         for (int i = 0; i < 2; ++i) ks[i] *= last;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)              // low times low too: equal keys cancel all but a 32nd of the sum
+        for (int a = 0; a < 3; ++a)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) ks[i] = mf(xt[128 * i + 64 * (k >> 1) + l], k & 1 ? ul : uh, ks[i]);
+          for (int b = 0; a + b < 3; ++b)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) ks[i] = mf(xt[192 * i + 64 * a + l], u[b], ks[i]);
       }
       const lds_t vt = (lds_t)(char*)lds + 16u * (B::VAT + (unsigned)t % B::VN * B::VU);
 #pragma unroll
@@ -637,15 +663,15 @@ struct Walk {
 #pragma unroll
         for (int e = 0; e < 4; ++e) r[i][e] = fmaf(-cc[e], ks[i][e], bf2f((bf16_t)q[e]));
       }
-      bf16x8 rh, rl;
-      split8(r[0], r[1], rh, rl);
-      f32x4 U[2];
-      chunk_product(ck.t0, ck.t1, rh, rl, l, f32x4{}, f32x4{}, U);
-      out.r[0][l] = rh;
-      out.r[1][l] = rl;
-      split8(U[0], U[1], uh, ul);
-      out.u[0][l] = uh;
-      out.u[1][l] = ul;
+      bf16x8 rp[3];
+      split8(r[0], r[1], rp[0], rp[1], &rp[2]);
+      f32x4 U[2] = {};
+      chunk_product(operand(ck.t0, ck.t1, l), rp, U);
+      out.r[0][l] = rp[0];
+      out.r[1][l] = rp[1];
+      split8(U[0], U[1], u[0], u[1], &u[2]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) out.u[i][l] = u[i];
       tk = after(tk);
     };
 #pragma unroll
@@ -673,7 +699,8 @@ struct Walk {
       f32x4 o[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) o[i] = (in.qs[0][i][l] + in.qs[1][i][l]) * *(const f32x4*)&ck.d[16 * i + 4 * g];
-      chunk_product(ck.w0, ck.w1, in.r[0][l], in.r[1][l], l, o[0], o[1], o);
+      const bf16x8 rp[2] = {in.r[0][l], in.r[1][l]};
+      chunk_product(operand(ck.w0, ck.w1, l), rp, o);
       store_chunk(out, at, o, g, len - t * C);
       out += (long long)C * old;
       if (t + 1 < nc) end_step();
@@ -719,9 +746,9 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
 }
 
 // ---- the walk with a wave alone for 16 rows --------------------------------------------------------------------------------
-// All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all (351 a chunk, 60 of them matrix
-// ones), and LDS for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768
-// tokens: 348 us.  A third workgroup a CU (LDS 32 bytes smaller) gains 2%, 32 columns a wave lose 18% (registers).
+// All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all (74 matrix ones a chunk), and LDS
+// for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768 tokens: 406 us.
+// With two parts everywhere (348): a third workgroup a CU gained 2%, 32 columns a wave lost 18% (registers).
 template <int K, int NW>
 struct Pair {                          // places in LDS of the two chunks, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB, VB = 2 * NW, VU = C * VB;
@@ -820,9 +847,9 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
         qs[i] = mf(qf[i], sl, qs[i]);
       }
     }
-    bf16x8 rh, rl, uh, ul;
+    bf16x8 u[3];
     {
-      f32x4 r[2], U[2];
+      f32x4 r[2], U[2] = {};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int row = 16 * i + qrow;
@@ -832,10 +859,12 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
         for (int e = 0; e < 4; ++e) r[i][e] = fmaf(-cc[e], ks[i][e], bf2f((bf16_t)q[e]));
         qs[i] *= *(const f32x4*)&ck.d[16 * i + 4 * g];
       }
-      split8(r[0], r[1], rh, rl);
-      chunk_product(ck.t0, ck.t1, rh, rl, l, f32x4{}, f32x4{}, U);
-      split8(U[0], U[1], uh, ul);
-      chunk_product(ck.w0, ck.w1, rh, rl, l, qs[0], qs[1], qs);
+      bf16x8 rp[3];
+      split8(r[0], r[1], rp[0], rp[1], &rp[2]);
+      chunk_product(operand(ck.t0, ck.t1, l), rp, U);
+      split8(U[0], U[1], u[0], u[1], &u[2]);
+      const bf16x8 rw[2] = {rp[0], rp[1]};
+      chunk_product(operand(ck.w0, ck.w1, l), rw, qs);
     }
     const float last = ck.last[0];
 #pragma unroll
@@ -844,8 +873,9 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
       for (int h = 0; h < 2; ++h) {
         const s16x4 k0 = quad(kt + col_at[x] + 8u * h), k1 = quad(kt + col_at[x] + 256u * RB + 8u * h);
         const bf16x8 kT = __builtin_bit_cast(bf16x8, __builtin_shufflevector(k0, k1, 0, 1, 2, 3, 4, 5, 6, 7));
-        S[x][h] = mf(kT, uh, S[x][h] * last);
-        S[x][h] = mf(kT, ul, S[x][h]);
+        S[x][h] *= last;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) S[x][h] = mf(kT, u[i], S[x][h]);
       }
     if (left > C) {                              // eight stores, which the next step's wait counts
 #pragma unroll
@@ -883,10 +913,15 @@ int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
   chunk_kernel<K><<<(unsigned)((seq_runs<C>(s) * d->HV + CHUNKS - 1) / CHUNKS) + 1, 64 * CHUNKS, 0, st>>>(*d, *s, work, order);
   if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
   auto grid = [&](int parts) { return (unsigned)place_grid((long long)s->N * d->H, d->HV / d->H * parts); };
-  // Up to a CU for every 16 rows the walk spreads each over eight waves; with more of them, one.  Eight | one, both
-  // kernels, 2048 tokens each, 32 heads of 128 x 128: 1 sequence (256 times 16 rows) 62 | 95 us, 2 sequences 111 | 100,
-  // 4 199 | 125; 16 heads of 64 x 64: 4 sequences (256 times) 54 | 76, 8 97 | 85.
-  if ((long long)s->N * d->HV * (V / 16) <= lq_seq_cus())
+  // Up to half a CU for every 16 rows the walk spreads each over eight waves (0.65 us a chunk, one workgroup a CU); with more
+  // of them, one (1.2 to 2.3 us, several a CU).  Eight | one, both kernels, 2048 tokens a sequence in the mean, 128 x 128,
+  // measured with two parts everywhere (three add 10% to either):
+  //   times 16 rows    256 (1 x 32 heads)    384 (6 x 8)    512 (2 x 32)    512 (8 x 8)    768 (3 x 32)    1024 (4 x 32)
+  //   equal lengths         62 |  95          102 |  99      110 | 104       106 | 101      154 | 115       198 | 131 us
+  //   random cuts           62 |  94          158 | 290      105 | 148       112 | 182      152 | 198       200 | 235
+  // Lengths are known on the device only, and prompts are rarely equal: twice the CUs, where equal ones lose 6%.  16 heads of
+  // 64 x 64: 512 (8 sequences) 99 | 86, 102 | 145; 768 139 | 98, 150 | 179.
+  if ((long long)s->N * d->HV * (V / 16) <= 2 * lq_seq_cus())
     walk_kernel<K, V><<<grid(V / 16), 64 * (ROLES + SERVICE), T::BYTES, st>>>(*d, *s, work, order);
   else
     lone_kernel<K, V, 4><<<grid(V / 64), 256, P::BYTES, st>>>(*d, *s, work, order);

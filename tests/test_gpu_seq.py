@@ -4,7 +4,7 @@ Bars, from what is rounded where:
   * a bf16 output of fp32 arithmetic (conv, norms, delta_steps): half a unit in the last place is 2^-9 of the value; 2^-8 lets
     an fp32 error move a value over a rounding edge.  Plus 1e-5 of the row's scale where terms cancel.
   * fp32 states of delta_steps: a few roundings of 2^-24 a token, 24 tokens: 1e-5 of the norm.
-  * delta_prefill's states: operands of the matrix cores carried as two bf16 halves, 2^-17 of each element at most, four
+  * delta_prefill's states: operands of the matrix cores carried in two or three bf16 parts, 2^-17 of each element at most, four
     products in a chain, errors of random sign: 1e-5 of the norm.  Its outputs besides their own rounding take the
     attention weights in bf16 (2^-9 each, random signs): 4e-3 of the norm, and 2^-6 of the larger of value and rms."""
 import numpy as np
@@ -106,6 +106,39 @@ def test_prefill_head_layouts(seq, HV, H):
     g = gpu(d)
     near_prefill(run_delta(seq.delta_prefill, g, H), want)
     assert rel(g["S"][3:], S[3:]) <= 1e-5
+
+
+MANY = [0, 70, 31, 1, 96, 64, 33, 2, 45, 32, 5, 130, 20, 17, 63, 65, 3, 40]
+
+
+@pytest.mark.parametrize("case", ["trained", "equal keys", "no decay", "strong decay", "zero and large"])
+@pytest.mark.parametrize("K,V", DIMS)
+def test_prefill_of_many_sequences(seq, K, V, case):
+    """More heads and sequences than the compute units take 16 rows a time of (the walk with a wave alone for them), at the
+    values and gates where the other one is tested too; a padding sequence among them, every third from zero."""
+    HV, H, N = 8, 2, len(MANY)
+    d = R.delta_inputs(17, MANY, HV, H, K, V, gate={"equal keys": -40.0, "no decay": -40.0, "strong decay": 60.0}.get(case))
+    if case == "equal keys":
+        d["mixed"][:, H * K:2 * H * K] = d["mixed"][0, H * K:2 * H * K]
+        d["b"][:] = 9.0
+    if case == "zero and large":
+        d["mixed"][100:110] = 0
+        d["mixed"][200:204] *= 1e4
+    d["src"][::3] = 0
+    d["idx"][4] = 0
+    want, S = R.delta_ref(d, H)
+    g = gpu(d)
+    out = run_delta(seq.delta_prefill, g, H)
+    at = d["loc"].tolist()
+    for n in range(N):
+        if n == 4:
+            assert not out[at[n]:at[n + 1]].any()
+        elif MANY[n]:
+            near_prefill(out[at[n]:at[n + 1]], want[at[n]:at[n + 1]])
+        if n != 4:
+            assert rel(g["S"][N + 1 + n], S[N + 1 + n]) <= 1e-5, n
+    assert torch.equal(g["S"][:N + 1].cpu(), d["S"][:N + 1])
+    assert torch.equal(g["S"][N + 5].cpu(), d["S"][N + 5])            # the padding sequence's
 
 
 @pytest.mark.parametrize("fn", ["delta_prefill", "delta_steps"])
