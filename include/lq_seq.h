@@ -55,8 +55,9 @@ int lq_delta_steps(const lq_delta* d, const lq_seqs* s, void* stream);
 int lq_delta_prefill(const lq_delta* d, const lq_seqs* s, void* work, long long work_bytes, void* stream);
 long long lq_delta_workspace(const lq_delta* d, const lq_seqs* s);
 
-/* Depthwise causal conv1d (W = 4) of the packed tokens x (bf16, rows x_ld elements apart) into out (bf16 [T][C]): the conv of lq.h's
- * lq_conv for each token, the taps before a sequence's first token read from its slot, its last three inputs left there. */
+/* Depthwise causal conv1d (W = 4) of the packed tokens x (bf16, rows x_ld elements apart) into out (bf16 [T][C], not
+ * overlapping x): the conv of lq.h's lq_conv for each token, the taps before a sequence's first token read from its slot, its
+ * last three inputs left there. */
 int lq_conv_seq(const lq_conv* cv, const lq_seqs* s, const void* x, long long x_ld, void* out, int C, void* stream);
 
 /* Norm of the rows of D <= 16384 elements, of `heads` consecutive vectors each: element (row, h, d) of x at
@@ -76,7 +77,8 @@ typedef struct lq_norm {
 
 /* out = x rsqrt(mean(x^2) + eps) (offset + weight) act(z) */
 int lq_gated_norm(const lq_norm* n, void* stream);
-/* res = x + scale z;  out = res rsqrt(mean(res^2) + eps) (offset + weight), of the sum before it is rounded.  res may be x. */
+/* res = x + scale z;  out = res rsqrt(mean(res^2) + eps) (offset + weight), of the sum before it is rounded.  res may be
+ * x or z. */
 int lq_add_norm(const lq_norm* n, void* stream);
 
 #ifdef __cplusplus

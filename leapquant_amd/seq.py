@@ -152,7 +152,7 @@ def delta_steps(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, scal
 def conv_prefill(x, conv_state, weight, bias, idx, loc, out, src=None, silu=True):
     """The depthwise causal conv1d of width 4 over a ragged batch: out [T, C] (bf16) from the packed tokens x [T, C] (bf16,
     possibly a column range of wider rows), out_t = act(sum_j w_j x_{t-3+j} + bias).  conv_state [NS, C, 3] (any strides): the
-    inputs before a sequence's first token come from its slot src, its last three are left in slot idx."""
+    inputs before a sequence's first token come from its slot src, its last three are left in slot idx.  out may not overlap x."""
     rc = _lib.seq_call().conv(x, conv_state, weight, bias, idx, loc, out, src, bool(silu))
     if rc != _NOT_PLAIN:
         return _lib.check(rc, "lq_conv_seq")
