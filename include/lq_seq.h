@@ -55,6 +55,10 @@ int lq_delta_steps(const lq_delta* d, const lq_seqs* s, void* stream);
 int lq_delta_prefill(const lq_delta* d, const lq_seqs* s, void* work, long long work_bytes, void* stream);
 long long lq_delta_workspace(const lq_delta* d, const lq_seqs* s);
 
+/* What lq_delta_steps (chunks = 0) or lq_delta_prefill (chunks = 1) answers to these arguments, workspace aside, without a
+ * launch: for a caller with work to do before the call that must not be done if the call is refused. */
+int lq_delta_check(const lq_delta* d, const lq_seqs* s, int chunks);
+
 /* Depthwise causal conv1d (W = 4) of the packed tokens x (bf16, rows x_ld elements apart) into out (bf16 [T][C], not
  * overlapping x): the conv of lq.h's lq_conv for each token, the taps before a sequence's first token read from its slot, its
  * last three inputs left there. */

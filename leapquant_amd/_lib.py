@@ -81,6 +81,7 @@ SEQ_SIGNATURES = {
     "lq_delta_steps": (c_int, [c_void_p, c_void_p, c_void_p]),
     "lq_delta_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p]),
     "lq_delta_workspace": (c_ll, [c_void_p, c_void_p]),
+    "lq_delta_check": (c_int, [c_void_p, c_void_p, c_int]),
     "lq_conv_seq": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
     "lq_gated_norm": (c_int, [c_void_p, c_void_p]),
     "lq_add_norm": (c_int, [c_void_p, c_void_p]),

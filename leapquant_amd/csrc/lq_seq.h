@@ -7,6 +7,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 __attribute__((visibility("hidden"))) int lq_seq_cus();      // compute units of the current GPU
+// a prefill's grids and 32-bit offsets hold what it is given
+__attribute__((visibility("hidden"))) bool lq_prefill_fits(const lq_delta* d, const lq_seqs* s);
 
 struct SeqRun {      // a run of a sequence's tokens, as its workgroup finds it
   int n, j;          // sequence, run of it

@@ -3,7 +3,7 @@
 // norm).
 // Each function checks all that the Python operator checks.  It returns the C entry's status, or NOT_PLAIN, having done
 // nothing: the operator then goes on in Python, which converts what may be converted and says what is wrong with the rest.
-// Nothing is thrown out of here.
+// No C++ exception leaves; the only Python one is that of the callable that `delta` calls.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
@@ -19,6 +19,7 @@ namespace {
 
 constexpr int NOT_PLAIN = 1;
 struct NotPlain {};
+struct Raised {};                        // a Python exception is set
 void need(bool ok) { if (!ok) throw NotPlain(); }
 
 const at::Tensor& tensor(PyObject* o) {
@@ -74,16 +75,19 @@ template <typename F> PyObject* status(F call) {
   int rc = NOT_PLAIN;
   try {
     rc = call();
+  } catch (const Raised&) {
+    return nullptr;
   } catch (...) {
     PyErr_Clear();
   }
   return PyLong_FromLong(rc);
 }
 
-// (S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, kda, glb, chunks)
+// (S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, kda, glb, chunks, before): `before`, None or a callable, is
+// called once nothing is left that refuses the call, right before the launch
 PyObject* delta(PyObject*, PyObject* const* arg, Py_ssize_t count) {
   return status([&] {
-    need(count == 15);
+    need(count == 16);
     const at::Tensor& S = tensor(arg[0]);
     need(S.is_cuda() && S.scalar_type() == at::kFloat && S.dim() == 4);
     const int dev = S.get_device();
@@ -117,11 +121,17 @@ PyObject* delta(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const lq_delta d = {(float*)S.data_ptr(), SS, (int)NS, (int)HV, (int)H, (int)K, (int)V, mixed.data_ptr(), a.data_ptr(),
                         b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), out.data_ptr(), mixed_ld, a_ld, b_ld, scale,
                         gate_bf16, kda, (float)number(arg[13])};
-    if (!chunks) return lq_delta_steps(&d, &s, stream(dev));
-    const long long n = lq_delta_workspace(&d, &s);
+    if (int rc = lq_delta_check(&d, &s, chunks)) return rc;
+    const long long n = chunks ? lq_delta_workspace(&d, &s) : 0;
     at::Tensor work;
     if (n > 0) work = at::empty({n}, at::TensorOptions().dtype(at::kByte).device(S.device()));
-    return lq_delta_prefill(&d, &s, n > 0 ? work.data_ptr() : nullptr, n, stream(dev));
+    void* const st = stream(dev);
+    if (arg[15] != Py_None) {
+      PyObject* r = PyObject_CallNoArgs(arg[15]);
+      if (!r) throw Raised();
+      Py_DECREF(r);
+    }
+    return chunks ? lq_delta_prefill(&d, &s, n > 0 ? work.data_ptr() : nullptr, n, st) : lq_delta_steps(&d, &s, st);
   });
 }
 

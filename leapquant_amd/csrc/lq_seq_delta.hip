@@ -32,8 +32,6 @@
 
 #include "lq_seq.h"
 
-__attribute__((visibility("hidden"))) int lq_check_delta(const lq_delta* d, const lq_seqs* s);
-
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -930,17 +928,18 @@ int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
 
 }  // namespace
 
+__attribute__((visibility("hidden"))) bool lq_prefill_fits(const lq_delta* d, const lq_seqs* s) {
+  return (seq_runs<C>(s) + 8) * d->HV <= 0x7fffffffll && ((long long)s->N * d->HV + 8) * 8 <= 0x7fffffffll && d->mixed_ld <= (1 << 24);
+}
+
 extern "C" long long lq_delta_workspace(const lq_delta* d, const lq_seqs* s) {
-  if (!d || d->kda || lq_check_delta(d, s) || s->N == 0) return 0;
+  if (lq_delta_check(d, s, 1) || s->N == 0) return 0;
   return seq_runs<C>(s) * d->HV * (long long)sizeof(Coef) + 4ll * s->N;
 }
 
 extern "C" int lq_delta_prefill(const lq_delta* d, const lq_seqs* s, void* work, long long work_bytes, void* stream) {
-  if (int rc = lq_check_delta(d, s)) return rc;
-  if (d->kda) return LQ_ERR_ARG;
+  if (int rc = lq_delta_check(d, s, 1)) return rc;
   if (s->N == 0) return LQ_OK;
-  if ((seq_runs<C>(s) + 8) * d->HV > 0x7fffffffll || ((long long)s->N * d->HV + 8) * 8 > 0x7fffffffll || d->mixed_ld > (1 << 24))
-    return LQ_ERR_ARG;
   const long long need = lq_delta_workspace(d, s);
   if (need > 0 && (!work || ((uintptr_t)work & 15) || work_bytes < need)) return LQ_ERR_ARG;
   hipStream_t st = (hipStream_t)stream;

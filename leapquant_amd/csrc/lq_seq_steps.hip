@@ -157,10 +157,17 @@ __global__ __launch_bounds__(256) void steps_kernel(lq_delta p, lq_seqs s) {
     }
 }
 
+// Rows a lane.  One asks for the state in the shortest chain of loads; all rows of a head's workgroup in one share a token's
+// norms and sums among 4.  One | four rows, 32 heads of 128 x 128: 1 x 1 token 5.4 | 6.8 us, 64 x 1 69 | 75, 1 x 4
+// 7.9 | 9.7, 1 x 32 28 | 41, 8 x 4 17.8 | 15.3, 64 x 8 143 | 94.
+int rows_of(const lq_delta* d, const lq_seqs* s) {
+  return s->T <= s->N || (long long)s->N * d->HV * (d->V / 32) <= 2 * lq_seq_cus() ? 1 : d->V / 32;
+}
+long long grid_of(const lq_delta* d, const lq_seqs* s) { return (long long)s->N * d->HV * (d->V / (32 * rows_of(d, s))); }
+
 template <int K, int V, int ROWS, bool KDA>
 int launch_rows(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
-  const long long grid = (long long)s->N * d->HV * (V / (32 * ROWS));
-  if (grid > 0x7fffffffll) return LQ_ERR_ARG;
+  const long long grid = grid_of(d, s);
   // States that fit the shared cache are written past it, which leaves it to those that are read: where one layer's states take
   // turns in it, 64 sequences of 8 tokens take 68 us instead of 77, 32 of 4 (KDA) 35 instead of 39; where other data fill
   // it, the same.  Beyond its size that gains nothing, and after other writes 256 sequences lose 18%.
@@ -170,11 +177,7 @@ int launch_rows(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
 }
 template <int K, int V, bool KDA>
 int launch(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
-  // One row a lane asks for the state in the shortest chain of loads; all rows of a head's workgroup in one share a token's
-  // norms and sums among 4.  One | four rows, 32 heads of 128 x 128: 1 x 1 token 5.4 | 6.8 us, 64 x 1 69 | 75, 1 x 4
-  // 7.9 | 9.7, 1 x 32 28 | 41, 8 x 4 17.8 | 15.3, 64 x 8 143 | 94.
-  if (s->T <= s->N || (long long)s->N * d->HV * (V / 32) <= 2 * lq_seq_cus()) return launch_rows<K, V, 1, KDA>(d, s, st);
-  return launch_rows<K, V, V / 32, KDA>(d, s, st);
+  return rows_of(d, s) == 1 ? launch_rows<K, V, 1, KDA>(d, s, st) : launch_rows<K, V, V / 32, KDA>(d, s, st);
 }
 
 }  // namespace
@@ -191,8 +194,8 @@ __attribute__((visibility("hidden"))) int lq_seq_cus() {
   return cache[dev];
 }
 
-__attribute__((visibility("hidden"))) int lq_check_delta(const lq_delta* d, const lq_seqs* s) {
-  if (!d || !seqs_ok(s)) return LQ_ERR_ARG;
+extern "C" int lq_delta_check(const lq_delta* d, const lq_seqs* s, int chunks) {
+  if (!d || !seqs_ok(s) || (chunks != 0 && (chunks != 1 || d->kda))) return LQ_ERR_ARG;
   const bool dims = (d->K == 128 && d->V == 128) || (!d->kda && d->K == 64 && (d->V == 128 || d->V == 64));
   if (!dims || d->NS <= 0 || d->H <= 0 || d->HV <= 0 || d->HV % d->H != 0) return LQ_ERR_ARG;
   if ((d->kda != 0 && d->kda != 1) || d->gate_bf16 < 0 || d->gate_bf16 > 3 || (!d->kda && d->glb != 0.f)) return LQ_ERR_ARG;
@@ -205,11 +208,13 @@ __attribute__((visibility("hidden"))) int lq_check_delta(const lq_delta* d, cons
   if (((uintptr_t)d->mixed & 15) || ((uintptr_t)d->out & 15) || (d->kda && ((uintptr_t)d->a & 7))) return LQ_ERR_ARG;
   if (!d->A_log || !d->dt_bias) return LQ_ERR_ARG;
   if (s->N > 0 && s->T > 0 && (!d->mixed || !d->a || !d->b || !d->out)) return LQ_ERR_ARG;
-  return LQ_OK;
+  if (s->N == 0) return LQ_OK;
+  if (chunks) return lq_prefill_fits(d, s) ? LQ_OK : LQ_ERR_ARG;
+  return grid_of(d, s) > 0x7fffffffll ? LQ_ERR_ARG : LQ_OK;
 }
 
 extern "C" int lq_delta_steps(const lq_delta* d, const lq_seqs* s, void* stream) {
-  if (int rc = lq_check_delta(d, s)) return rc;
+  if (int rc = lq_delta_check(d, s, 0)) return rc;
   if (s->N == 0) return LQ_OK;
   hipStream_t st = (hipStream_t)stream;
   if (d->kda) return launch<128, 128, true>(d, s, st);

@@ -119,6 +119,26 @@ def _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, gl
     return d, seqs, (live, a, A_log, dt_bias)
 
 
+def _rule(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, glb, chunks, before=None):
+    """The gated delta rule in chunks or token by token.  `before`, a callable, is called when nothing is left that refuses
+    the call (arguments checked, workspace taken), right before the launch."""
+    name = "lq_delta_prefill" if chunks else "lq_delta_steps"
+    rc = _lib.seq_call().delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, kda, glb, chunks, before)
+    if rc != _NOT_PLAIN:
+        return _lib.check(rc, name)
+    d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, glb, chunks=chunks)
+    L = _lib.seq_lib()
+    _lib.check(L.lq_delta_check(d, seqs, chunks), name)
+    n = L.lq_delta_workspace(d, seqs) if chunks else 0
+    work = torch.empty(n, dtype=torch.uint8, device=S.device) if n > 0 else None
+    if before is not None:
+        before()
+    if chunks:
+        _lib.check(L.lq_delta_prefill(d, seqs, work.data_ptr() if n > 0 else None, n, _raw_stream(S)), name)
+    else:
+        _lib.check(L.lq_delta_steps(d, seqs, _raw_stream(S)), name)
+
+
 def delta_prefill(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, scale=None):
     """The gated delta rule of Gated DeltaNet over the prompts of a ragged batch, in chunks on the matrix cores.
 
@@ -126,14 +146,7 @@ def delta_prefill(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, sc
     [T, 2HK + HV V] after the conv, q | k | v; a, b: bf16 [T, HV] raw gates.  The three may be column ranges of wider rows.
     A_log, dt_bias: [HV].  out: bf16 [T, HV, V].  scale: of the queries, K^-1/2 by default.  Gates, norms and state as the
     decode step's, with beta = sigmoid(b) not rounded.  A NaN or infinity in a token reaches all tokens of its chunk of 32."""
-    rc = _lib.seq_call().delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, False, 0.0, True)
-    if rc != _NOT_PLAIN:
-        return _lib.check(rc, "lq_delta_prefill")
-    d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, False, 0.0, chunks=True)
-    L = _lib.seq_lib()
-    n = L.lq_delta_workspace(d, seqs)
-    work = torch.empty(n, dtype=torch.uint8, device=S.device) if n > 0 else None
-    _lib.check(L.lq_delta_prefill(d, seqs, work.data_ptr() if n > 0 else None, n, _raw_stream(S)), "lq_delta_prefill")
+    _rule(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, False, 0.0, True)
 
 
 def delta_steps(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, scale=None, kda=False, gate_lower_bound=0.0):
@@ -142,11 +155,7 @@ def delta_steps(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, scal
     0, its bounded gate gate_lower_bound * sigmoid(exp(A_log) (a + dt_bias))."""
     if gate_lower_bound and not kda:
         raise ValueError("gate_lower_bound: KDA only")
-    rc = _lib.seq_call().delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, src, H, scale, bool(kda), gate_lower_bound, False)
-    if rc != _NOT_PLAIN:
-        return _lib.check(rc, "lq_delta_steps")
-    d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, bool(kda), gate_lower_bound)
-    _lib.check(_lib.seq_lib().lq_delta_steps(d, seqs, _raw_stream(S)), "lq_delta_steps")
+    _rule(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, bool(kda), gate_lower_bound, False)
 
 
 def conv_prefill(x, conv_state, weight, bias, idx, loc, out, src=None, silu=True):

@@ -191,15 +191,14 @@ class LeapQuantState:
             raise ValueError("idx: 1-D expected, got shape %s" % (tuple(idx.shape),))
         if has_state is not None and has_state.shape != idx.shape:
             raise ValueError("has_state: one of each idx expected, got shape %s" % (tuple(has_state.shape),))
+        # the checkpoints become fp32 states only once nothing refuses the call any more: a refused one leaves them as they are
+        self._check_round_trip(ssm, idx)
+        idx = seq._index(idx, idx.shape[0], "idx")
         src = torch.zeros_like(idx) if has_state is None else idx * has_state.to(torch.bool)
-        if has_state is not None:
-            self.dequantize(ssm, src)
-        if self.kda:
-            seq.delta_steps(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src=src, scale=self._scale, kda=True,
-                            gate_lower_bound=self.glb)
-        else:
-            fn = seq.delta_steps if mixed.shape[0] <= self.STEPS * idx.shape[0] else seq.delta_prefill
-            fn(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src=src, scale=self._scale)
+        before = None if has_state is None else functools.partial(self.dequantize, ssm, src)
+        chunks = not self.kda and mixed.shape[0] > self.STEPS * idx.shape[0]
+        seq._rule(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src, self._scale, bool(self.kda),
+                  self.glb if self.kda else 0.0, chunks, before)
         self.quantize(ssm, idx)
 
     def decode_conv(self, ssm, x, conv_state, conv_weight, conv_bias, silu, a, b, A_log, dt_bias, idx, out):
