@@ -50,14 +50,14 @@ class GDNBlock:
         seq.add_norm(x, y, self.norm_next, y, h)
         return y, h
 
-    def prefill(self, x, h, idx, loc, has_state=None):
-        """x, h [T, hidden]: the residual stream and its norm, the packed tokens of the sequences in slots idx."""
+    def prefill(self, x, h, idx, loc, has_state=None, longest=None):
+        """x, h [T, hidden]: the residual stream and its norm, the packed tokens of the sequences in slots idx, at most `longest` each."""
         mixed, z, b, a = self._project(h)
         src = torch.zeros_like(idx) if has_state is None else idx * has_state
         m = torch.empty(x.shape[0], self.C, device=x.device, dtype=BF16)
         seq.conv_prefill(mixed, self.conv, self.w_conv, None, idx, loc, m, src=src)
         o = torch.empty(x.shape[0], self.HV, self.D, device=x.device, dtype=BF16)
-        self.state.prefill(self.ssm, m, a, b, self.A_log, self.dt_bias, idx, loc, o, has_state=has_state)
+        self.state.prefill(self.ssm, m, a, b, self.A_log, self.dt_bias, idx, loc, o, has_state=has_state, longest=longest)
         return self._close(x, o, z)
 
     def decode(self, x, h, idx):
@@ -85,7 +85,7 @@ def main():
     for timed in (False, True):
         t0, t1, t2 = ev(), ev(), ev()
         t0.record()
-        y, h = block.prefill(x, x, idx, loc)
+        y, h = block.prefill(x, x, idx, loc, longest=max(lens))
         t1.record()
         last = (loc[1:] - 1).long()
         y, h = y[last], h[last]

@@ -69,8 +69,9 @@ class LeapQuantState:
     the same; a due row costs its call one head flush instead of two).  dequantize settles such heads first.
     """
 
-    # tokens a sequence up to which a GDN prefill goes token by token: at 8 both take 75 us (64 sequences of 32 heads of 128 x
-    # 128) or 15 against 17 (8 sequences), at 4 55 against 74 and 11 against 17, at 16 118 against 75 and 23 against 17
+    # Tokens of its longest sequence up to which a GDN prefill goes token by token.  Token by token | in chunks, 32 heads of 128 x
+    # 128: 64 sequences of 4 tokens 46 | 75 us, of 8 60 | 75, of 12 77 | 76, of 16 96 | 74; 8 of 4 9.3 | 17.5, of 8 12.9 | 17.5,
+    # of 12 15.9 | 17.6, of 16 19.5 | 17.5.  63 single tokens beside a prompt of 449: 403 | 79, 255 beside 1790: 1623 | 282.
     STEPS = 8
 
     def __init__(self, ssm, H, kda=False, gate_lower_bound=0.0, nmax=0, L=WINDOW, R=RANK, qmax=KN.QMAX,
@@ -181,12 +182,16 @@ class LeapQuantState:
             fn = L.lq_gdn_decode_deferred if self.defer_flush else L.lq_gdn_decode
             _lib.check(fn(ctypes.byref(st), ctypes.byref(io), None, dev(self.Q0), stream), "lq_gdn_decode")
 
-    def prefill(self, ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, has_state=None):
+    def prefill(self, ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, has_state=None, longest=None):
         """The prompts of a ragged batch, or their next pieces: tokens loc[n] .. loc[n + 1] - 1 of the packed mixed [T, 2HK +
         HV V], a, b and out [T, HV, V] belong to slot idx[n] (an idx outside 1 .. NS - 1: padding).  has_state [N]: which
         sequences go on from the checkpoint of their slot; the others start from zero, as all do by default.  The states
         are fp32 for the call and end as the 8-bit checkpoints that decode reads, with empty windows.
-        GDN prompts go through `seq.delta_prefill`; KDA, and calls of at most STEPS tokens a sequence, token by token."""
+        longest: tokens of the longest sequence where the host knows them (a host integer, which decides on speed only).
+        GDN goes in chunks (`seq.delta_prefill`), or token by token where no sequence has more than STEPS tokens, by `longest`
+        or, without it, because the call has no more; KDA goes token by token."""
+        if isinstance(longest, torch.Tensor):
+            raise TypeError("longest: a host integer expected, got a tensor")
         if idx.dim() != 1:
             raise ValueError("idx: 1-D expected, got shape %s" % (tuple(idx.shape),))
         if has_state is not None and has_state.shape != idx.shape:
@@ -196,7 +201,7 @@ class LeapQuantState:
         idx = seq._index(idx, idx.shape[0], "idx")
         src = torch.zeros_like(idx) if has_state is None else idx * has_state.to(torch.bool)
         before = None if has_state is None else functools.partial(self.dequantize, ssm, src)
-        chunks = not self.kda and mixed.shape[0] > self.STEPS * idx.shape[0]
+        chunks = not self.kda and (mixed.shape[0] if longest is None else longest) > self.STEPS
         seq._rule(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src, self._scale, bool(self.kda),
                   self.glb if self.kda else 0.0, chunks, before)
         self.quantize(ssm, idx)

@@ -53,6 +53,27 @@ def test_a_failed_workspace_leaves_the_checkpoints(monkeypatch):
         st.prefill(**d)
 
 
+@pytest.mark.parametrize("N,T,longest,chunks", [
+    (64, 512, None, True), (64, 512, 449, True), (64, 512, 8, False), (64, 512, 9, True), (1, 8, None, False), (1, 9, None, True),
+    (3, 8, None, False), (256, 256, None, True), (256, 256, 1, False), (0, 0, None, False)])
+def test_prefill_goes_by_the_longest_sequence(monkeypatch, N, T, longest, chunks):
+    """Token by token takes as long as the longest sequence: 63 single tokens beside a prompt of 449 go in chunks."""
+    st, d = call(N=N, T=T, HV=2, H=1, loc=torch.zeros(N + 1, dtype=torch.int32)) if N else call(N=1, T=0)
+    if not N:
+        d.update(idx=d["idx"][:0], loc=d["loc"][:1], has_state=d["has_state"][:0])
+    took = []
+    monkeypatch.setattr(seq, "_rule", lambda *a: took.append(a[14]))
+    for name in ("dequantize", "quantize"):
+        monkeypatch.setattr(st, name, lambda *a: None)
+    st.prefill(**d, longest=longest)
+    assert took == [chunks]
+    st.kda = True
+    st.prefill(**d, longest=longest)
+    assert took == [chunks, False]
+    with pytest.raises(TypeError, match="longest"):
+        st.prefill(**d, longest=torch.tensor(3))
+
+
 def test_check_entry_answers_as_the_calls():
     """lq_delta_check without a launch: the grids' limits and the forms that each call takes."""
     import ctypes
