@@ -14,6 +14,10 @@
 extern "C" {
 #endif
 
+/* Raised with every change of a structure's layout or an entry point's arguments, as LQ_ABI_VERSION of lq.h. */
+#define LQ_SEQ_ABI_VERSION 1
+int lq_seq_abi_version(void);
+
 /* A ragged batch: sequence n holds the packed tokens loc[n] .. loc[n + 1] - 1 of T.  The kernels hold every offset to
  * 0 <= loc[n] <= loc[n + 1] <= T.  It starts from slot src[n] of the state (or conv) cache and leaves its last state in slot
  * idx[n]; a src outside 1 .. NS - 1 starts from zero, an idx outside makes a padding sequence: its outputs are zero and

@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "_build", "liblq.so")
 SEQ_LIB_PATH = os.path.join(_HERE, "_build", "liblq_seq.so")
 SEQ_CALL_PATH = os.path.join(_HERE, "_build", "lq_seq_call.so")
 ABI_VERSION = 6
+SEQ_ABI_VERSION = 1
 SCHED_INTS = 512           # include/lq.h: LQ_SCHED_INTS
 
 c_void_p, c_int, c_float, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
@@ -78,6 +79,7 @@ SIGNATURES = {
 # the same of include/lq_seq.h; the structures go as addresses, so that a caller may hand over their bytes (PACK_*), which a
 # call from Python builds in a quarter of a structure's time
 SEQ_SIGNATURES = {
+    "lq_seq_abi_version": (c_int, []),
     "lq_delta_steps": (c_int, [c_void_p, c_void_p, c_void_p]),
     "lq_delta_prefill": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p]),
     "lq_delta_workspace": (c_ll, [c_void_p, c_void_p]),
@@ -95,11 +97,14 @@ _LIB = [None]
 _SEQ_LIB = [None]
 
 
-def _load(path, signatures):
+def _load(path, signatures, abi, version):
     if not os.path.exists(path):
         raise RuntimeError("%s is missing (%s): build it with `python -m leapquant_amd.build`"
                            % (os.path.basename(path), path))
     L = ctypes.CDLL(path)
+    v = getattr(L, abi)() if hasattr(L, abi) else None
+    if v != version:
+        raise RuntimeError("%s ABI %s, expected %d: rebuild it" % (os.path.basename(path), v, version))
     for name, (res, args) in signatures.items():
         f = getattr(L, name)
         f.restype = res
@@ -110,18 +115,14 @@ def _load(path, signatures):
 def lib():
     """The loaded liblq.so (raises if it has not been built)."""
     if _LIB[0] is None:
-        L = _load(LIB_PATH, SIGNATURES)
-        v = L.lq_abi_version()
-        if v != ABI_VERSION:
-            raise RuntimeError("liblq.so ABI %d, expected %d: rebuild it" % (v, ABI_VERSION))
-        _LIB[0] = L
+        _LIB[0] = _load(LIB_PATH, SIGNATURES, "lq_abi_version", ABI_VERSION)
     return _LIB[0]
 
 
 def seq_lib():
     """The loaded liblq_seq.so (raises if it has not been built)."""
     if _SEQ_LIB[0] is None:
-        _SEQ_LIB[0] = _load(SEQ_LIB_PATH, SEQ_SIGNATURES)
+        _SEQ_LIB[0] = _load(SEQ_LIB_PATH, SEQ_SIGNATURES, "lq_seq_abi_version", SEQ_ABI_VERSION)
     return _SEQ_LIB[0]
 
 
@@ -129,13 +130,20 @@ _SEQ_CALL = [None]
 
 
 def seq_call():
-    """The loaded lq_seq_call.so, a Python extension (raises if it has not been built)."""
+    """The loaded lq_seq_call.so, a Python extension (raises if it has not been built, or for other structures than those of
+    this binding, or against another torch)."""
     if _SEQ_CALL[0] is None:
+        import torch
+        seq_lib()                        # the library behind it, of the same version
         if not os.path.exists(SEQ_CALL_PATH):
             raise RuntimeError("%s is missing: build it with python -m leapquant_amd.build" % SEQ_CALL_PATH)
         loader = importlib.machinery.ExtensionFileLoader("lq_seq_call", SEQ_CALL_PATH)
         module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("lq_seq_call", SEQ_CALL_PATH, loader=loader))
         loader.exec_module(module)
+        built = getattr(module, "ABI", None), getattr(module, "TORCH", None)
+        if built != (SEQ_ABI_VERSION, torch.__version__):
+            raise RuntimeError("lq_seq_call.so: ABI %s with torch %s, expected %d with %s: rebuild it"
+                               % (built + (SEQ_ABI_VERSION, torch.__version__)))
         _SEQ_CALL[0] = module
     return _SEQ_CALL[0]
 

@@ -66,6 +66,7 @@ def _build_call():
     rocm = os.path.dirname(os.path.dirname(hipcc())) if os.path.sep in hipcc() else "/opt/rocm"
     tmp = SEQ_CALL + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           '-DLQ_TORCH_VERSION="%s"' % torch.__version__,
            os.path.join(CSRC, "lq_seq_call.cpp"), "-o", tmp]
     cmd += ["-isystem" + d for d in (os.path.join(t, "include"), os.path.join(t, "include", "torch", "csrc", "api", "include"),
                                      os.path.join(rocm, "include"), sysconfig.get_paths()["include"])]

@@ -202,6 +202,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "lq_seq_call", nullptr, -1, methods
 
 PyMODINIT_FUNC PyInit_lq_seq_call() {
   PyObject* m = PyModule_Create(&module);
-  if (m) PyModule_AddIntConstant(m, "NOT_PLAIN", NOT_PLAIN);
+  if (!m) return nullptr;
+  PyModule_AddIntConstant(m, "NOT_PLAIN", NOT_PLAIN);
+  PyModule_AddIntConstant(m, "ABI", LQ_SEQ_ABI_VERSION);
+  PyModule_AddStringConstant(m, "TORCH", LQ_TORCH_VERSION);      // whose tensors the functions read
   return m;
 }

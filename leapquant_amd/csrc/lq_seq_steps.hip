@@ -194,6 +194,8 @@ __attribute__((visibility("hidden"))) int lq_seq_cus() {
   return cache[dev];
 }
 
+extern "C" int lq_seq_abi_version(void) { return LQ_SEQ_ABI_VERSION; }
+
 extern "C" int lq_delta_check(const lq_delta* d, const lq_seqs* s, int chunks) {
   if (!d || !seqs_ok(s) || (chunks != 0 && (chunks != 1 || d->kda))) return LQ_ERR_ARG;
   const bool dims = (d->K == 128 && d->V == 128) || (!d->kda && d->K == 64 && (d->V == 128 || d->V == 64));
