@@ -1,7 +1,12 @@
 """What is built and shipped of the sequence operators (CPU): stale files are refused before a call."""
+import fnmatch
+import os
+
 import pytest
 
-from leapquant_amd import _lib
+from leapquant_amd import _lib, build as B
+
+ROOT = os.path.dirname(B.HERE)
 
 
 def test_a_library_of_another_version_is_refused(monkeypatch):
@@ -29,3 +34,13 @@ def test_an_extension_of_another_build_is_refused(monkeypatch):
             m.setattr(where, name, value)
             with pytest.raises(RuntimeError, match="rebuild"):
                 _lib.seq_call()
+
+
+def test_the_package_ships_what_it_loads():
+    """An installed package holds the libraries that its modules load, and the sources of each."""
+    tomli = pytest.importorskip("tomli")
+    with open(os.path.join(ROOT, "pyproject.toml"), "rb") as f:
+        globs = tomli.load(f)["tool"]["setuptools"]["package-data"]["leapquant_amd"]
+    files = [_lib.LIB_PATH, _lib.SEQ_LIB_PATH, _lib.SEQ_CALL_PATH] + [os.path.join(B.CSRC, f) for f in os.listdir(B.CSRC)]
+    for f in files:
+        assert any(fnmatch.fnmatch(os.path.relpath(f, B.HERE), g) for g in globs), f
