@@ -8,6 +8,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -71,6 +72,13 @@ int gate(const at::Tensor& t, int dev, long long n) {
 }
 void* stream(int dev) { return (void*)c10::hip::getCurrentHIPStream((c10::DeviceIndex)dev).stream(); }
 
+// `dev` current while this lives: a launch on a default stream goes to the current device, whatever its tensors are on
+struct Current {
+  const c10::DeviceIndex dev, was;
+  explicit Current(int d) : dev((c10::DeviceIndex)d), was(c10::hip::ExchangeDevice(dev)) {}
+  ~Current() { if (was != dev) (void)c10::hip::SetDevice(was); }
+};
+
 template <typename F> PyObject* status(F call) {
   int rc = NOT_PLAIN;
   try {
@@ -121,6 +129,7 @@ PyObject* delta(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const lq_delta d = {(float*)S.data_ptr(), SS, (int)NS, (int)HV, (int)H, (int)K, (int)V, mixed.data_ptr(), a.data_ptr(),
                         b.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), out.data_ptr(), mixed_ld, a_ld, b_ld, scale,
                         gate_bf16, kda, (float)number(arg[13])};
+    const Current current(dev);
     if (int rc = lq_delta_check(&d, &s, chunks)) return rc;
     const long long n = chunks ? lq_delta_workspace(&d, &s) : 0;
     at::Tensor work;
@@ -156,6 +165,7 @@ PyObject* conv(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     need(arg[8] == Py_True || arg[8] == Py_False);
     const lq_conv cv = {st.data_ptr(), w.data_ptr(), bias ? bias->data_ptr() : nullptr, st.stride(0), st.stride(1), st.stride(2),
                         4, arg[8] == Py_True, (int)st.size(0)};
+    const Current current(dev);
     return lq_conv_seq(&cv, &s, x.data_ptr(), ld, out.data_ptr(), (int)C, stream(dev));
   });
 }
@@ -188,6 +198,7 @@ PyObject* norm(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const lq_norm n = {x.data_ptr(), z.data_ptr(), w.data_ptr(), res ? res->data_ptr() : nullptr, out.data_ptr(),
                        row(x), head(x), row(z), head(z), row(out), head(out), (int)rows, (int)heads, (int)D,
                        (float)number(arg[5]), (float)number(arg[6]), (float)number(arg[7]), (int)integer(arg[8]), !wide};
+    const Current current(dev);
     return add ? lq_add_norm(&n, stream(dev)) : lq_gated_norm(&n, stream(dev));
   });
 }

@@ -28,6 +28,7 @@
 // 1.8 TB/s; with two parts everywhere, 414 us, matrix instructions were busy 42% of the walk's cycles, vector ones 50%, LDS
 // 45%, at the 1.7 GHz that this mix leaves of the clock).  The kernels' own times below are a profiler's, which stretches
 // the short ones.
+#include <atomic>
 #include <type_traits>
 
 #include "lq_seq.h"
@@ -900,13 +901,24 @@ void lone_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
     for (int h = 0; h < 2; ++h) *(f32x4*)(p.S + dst * p.slot_stride + head + 32 * x + 4 * h) = S[x][h];
 }
 
+// The walk's LDS is more than a kernel may have unasked: asked for once on each device, and again where that failed.
+template <int K, int V> bool walk_lds() {
+  static std::atomic<bool> had[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && had[dev].load(std::memory_order_relaxed)) return true;
+  if (hipFuncSetAttribute((const void*)walk_kernel<K, V>, hipFuncAttributeMaxDynamicSharedMemorySize, Tiles<K>::BYTES) != hipSuccess)
+    return false;
+  if (known) had[dev].store(true, std::memory_order_relaxed);
+  return true;
+}
+
 template <int K, int V>
 int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
   typedef Tiles<K> T;
   typedef Pair<K, 4> P;
-  static const hipError_t set = hipFuncSetAttribute((const void*)walk_kernel<K, V>,
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, T::BYTES);
-  if (set != hipSuccess) return LQ_ERR_HIP;
+  if (!walk_lds<K, V>()) return LQ_ERR_HIP;
   int* order = (int*)(work + seq_runs<C>(s) * d->HV);
   chunk_kernel<K><<<(unsigned)((seq_runs<C>(s) * d->HV + CHUNKS - 1) / CHUNKS) + 1, 64 * CHUNKS, 0, st>>>(*d, *s, work, order);
   if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;

@@ -11,8 +11,8 @@ A ragged batch is given by `loc` [N + 1] (sequence n holds the packed tokens loc
 that take the sequences' last states, and `src` [N], the slots they start from (None: idx, in place).  A src outside the
 cache's slots 1 .. NS - 1 (0, -1) starts from zero; an idx outside them makes a padding sequence: outputs zero, no slot written.
 As in the decode calls slot 0 is padding.  The caller keeps the slots that one sequence of a call writes apart from those
-that another reads or writes.  Calls launch on torch's current stream, never synchronise and can be captured in a graph;
-they work forward only (no autograd).
+that another reads or writes.  Calls launch on the current stream of their tensors' device, never synchronise and can be
+captured in a graph; they work forward only (no autograd).
 """
 import ctypes
 
@@ -128,15 +128,16 @@ def _rule(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, glb
         return _lib.check(rc, name)
     d, seqs, live = _delta(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src, scale, kda, glb, chunks=chunks)
     L = _lib.seq_lib()
-    _lib.check(L.lq_delta_check(d, seqs, chunks), name)
-    n = L.lq_delta_workspace(d, seqs) if chunks else 0
-    work = torch.empty(n, dtype=torch.uint8, device=S.device) if n > 0 else None
-    if before is not None:
-        before()
-    if chunks:
-        _lib.check(L.lq_delta_prefill(d, seqs, work.data_ptr() if n > 0 else None, n, _raw_stream(S)), name)
-    else:
-        _lib.check(L.lq_delta_steps(d, seqs, _raw_stream(S)), name)
+    with torch.cuda.device(S.get_device()):
+        _lib.check(L.lq_delta_check(d, seqs, chunks), name)
+        n = L.lq_delta_workspace(d, seqs) if chunks else 0
+        work = torch.empty(n, dtype=torch.uint8, device=S.device) if n > 0 else None
+        if before is not None:
+            before()
+        if chunks:
+            _lib.check(L.lq_delta_prefill(d, seqs, work.data_ptr() if n > 0 else None, n, _raw_stream(S)), name)
+        else:
+            _lib.check(L.lq_delta_steps(d, seqs, _raw_stream(S)), name)
 
 
 def delta_prefill(S, mixed, a, b, A_log, dt_bias, idx, loc, out, H, src=None, scale=None):
@@ -176,8 +177,9 @@ def conv_prefill(x, conv_state, weight, bias, idx, loc, out, src=None, silu=True
     seqs, live = _batch(idx, loc, src, T)
     cv = conv_struct(conv_state, weight, bias, silu)
     _on(x.get_device(), conv_state=conv_state, weight=weight, bias=bias, idx=idx, loc=loc, out=out, src=src)
-    _lib.check(_lib.seq_lib().lq_conv_seq(ctypes.byref(cv), seqs, x.data_ptr(), ld, out.data_ptr(), C, _raw_stream(x)),
-               "lq_conv_seq")
+    with torch.cuda.device(x.get_device()):
+        _lib.check(_lib.seq_lib().lq_conv_seq(ctypes.byref(cv), seqs, x.data_ptr(), ld, out.data_ptr(), C, _raw_stream(x)),
+                   "lq_conv_seq")
 
 
 def _norm(x, z, weight, out, res, eps, scale, offset, act):
@@ -221,7 +223,8 @@ def gated_norm(x, z, weight, out, eps=1e-6, gate="silu", offset=0.0):
     if rc != _NOT_PLAIN:
         return _lib.check(rc, "lq_gated_norm")
     n = _norm(x, z, weight, out, None, eps, 0.0, offset, _ACT[gate])
-    _lib.check(_lib.seq_lib().lq_gated_norm(n, _raw_stream(x)), "lq_gated_norm")
+    with torch.cuda.device(x.get_device()):
+        _lib.check(_lib.seq_lib().lq_gated_norm(n, _raw_stream(x)), "lq_gated_norm")
 
 
 def add_norm(x, y, weight, res, out, eps=1e-6, scale=1.0, offset=0.0):
@@ -232,4 +235,5 @@ def add_norm(x, y, weight, res, out, eps=1e-6, scale=1.0, offset=0.0):
     if rc != _NOT_PLAIN:
         return _lib.check(rc, "lq_add_norm")
     n = _norm(x, y, weight, out, res, eps, scale, offset, 0)
-    _lib.check(_lib.seq_lib().lq_add_norm(n, _raw_stream(x)), "lq_add_norm")
+    with torch.cuda.device(x.get_device()):
+        _lib.check(_lib.seq_lib().lq_add_norm(n, _raw_stream(x)), "lq_add_norm")

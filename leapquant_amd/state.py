@@ -204,7 +204,8 @@ class LeapQuantState:
         chunks = not self.kda and (mixed.shape[0] if longest is None else longest) > self.STEPS
         seq._rule(ssm, mixed, a, b, A_log, dt_bias, idx, loc, out, self.H, src, self._scale, bool(self.kda),
                   self.glb if self.kda else 0.0, chunks, before)
-        self.quantize(ssm, idx)
+        with torch.cuda.device(ssm.get_device()):
+            self.quantize(ssm, idx)
 
     def decode_conv(self, ssm, x, conv_state, conv_weight, conv_bias, silu, a, b, A_log, dt_bias, idx, out):
         """GDN decode with the conv1d update fused into the step (lq_gdn_step_conv): x is the raw projection
