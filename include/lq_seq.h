@@ -69,7 +69,8 @@ int lq_delta_check(const lq_delta* d, const lq_seqs* s, int chunks);
 int lq_conv_seq(const lq_conv* cv, const lq_seqs* s, const void* x, long long x_ld, void* out, int C, void* stream);
 
 /* Norm of the rows of D <= 16384 elements, of `heads` consecutive vectors each: element (row, h, d) of x at
- * x[row * x_ld + h * x_hd + d], z and out likewise.  `weight` [D], fp32 or bf16 (weight_bf16). */
+ * x[row * x_ld + h * x_hd + d], z and out likewise; vectors of out (o_ld, o_hd) may not overlap each other.  `weight` [D], fp32
+ * or bf16 (weight_bf16). */
 typedef struct lq_norm {
   const void* x;
   const void* z;          /* lq_gated_norm: the gate; lq_add_norm: what is added */

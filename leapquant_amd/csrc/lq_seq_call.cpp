@@ -187,6 +187,8 @@ PyObject* norm(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     on(dev, z); on(dev, w); on(dev, out);
     need(bf16(z) && bf16(out) && z.sizes() == x.sizes() && out.sizes() == x.sizes());
     need(D == 1 || (x.stride(nd - 1) == 1 && z.stride(nd - 1) == 1 && out.stride(nd - 1) == 1));
+    need(nd < 2 || rows < 2 || out.stride(0) >= D);        // rows and heads of their own
+    need(nd < 3 || heads < 2 || out.stride(1) >= D);
     if (res) {
       on(dev, *res);
       need(bf16(*res) && res->sizes() == x.sizes() && res->strides() == out.strides());

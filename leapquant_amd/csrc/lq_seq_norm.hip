@@ -133,6 +133,7 @@ int norm(const lq_norm* p, hipStream_t s) {
   if (!p || p->rows < 0 || p->heads <= 0 || p->D <= 0 || p->D > 16384) return LQ_ERR_ARG;
   if ((p->act != 0 && p->act != 1) || (p->weight_bf16 != 0 && p->weight_bf16 != 1) || !(p->eps >= 0.f)) return LQ_ERR_ARG;
   if (p->rows == 0) return LQ_OK;
+  if ((p->rows > 1 && p->o_ld < p->D) || (p->heads > 1 && p->o_hd < p->D)) return LQ_ERR_ARG;     // vectors of out overlap
   if (!p->x || !p->z || !p->weight || !p->out || (ADD && !p->res)) return LQ_ERR_ARG;
   const long long ld = p->x_ld | p->x_hd | p->z_ld | p->z_hd | p->o_ld | p->o_hd;
   const uintptr_t at = (uintptr_t)p->x | (uintptr_t)p->z | (uintptr_t)p->out | (uintptr_t)(ADD ? p->res : nullptr) |

@@ -195,6 +195,8 @@ def _norm(x, z, weight, out, res, eps, scale, offset, act):
             raise ValueError("%s: bf16 %s expected, got %s %s" % (name, tuple(shape), t.dtype, tuple(t.shape)))
     if D > 1 and not sx[-1] == sz[-1] == so[-1] == 1:
         raise ValueError("packed elements expected in the last dimension (strides %s, %s, %s)" % (sx, sz, so))
+    if any(n > 1 and s < D for n, s in zip(shape[:-1], so)):
+        raise ValueError("out: rows that overlap each other (strides %s)" % (so,))
     if res is not None and (res.dtype is not _BF16 or res.shape != shape or res.stride() != so):
         raise ValueError("res: bf16 %s laid out as out expected, got %s %s strides %s"
                          % (tuple(shape), res.dtype, tuple(res.shape), res.stride()))
