@@ -1,5 +1,5 @@
 // The calls of leapquant_amd/seq.py whose arguments are as the kernels read them, without the interpreter's time for each
-// attribute of each tensor (a call on small tensors is mostly host time: 10.8 -> 4.9 us for the rule's steps, 6.1 -> 3.2 for a
+// attribute of each tensor (a call on small tensors is mostly host time: 10.8 -> 5.1 us for the rule's steps, 6.1 -> 3.4 for a
 // norm).
 // Each function checks all that the Python operator checks.  It returns the C entry's status, or NOT_PLAIN, having done
 // nothing: the operator then goes on in Python, which converts what may be converted and says what is wrong with the rest.

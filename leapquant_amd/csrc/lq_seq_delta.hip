@@ -19,15 +19,17 @@
 // 2.8e-6 (two parts) or 5e-9 (three) of the operand short in the mean.  What is appended to the state and leads to it (T', R,
 // T' R, X) has three: errors of its terms do not cancel where the terms do, as with equal keys in a chunk.  The state ends
 // within 8e-7 of its norm, 2e-7 in the median (fp32 sums: 2e-7); with two parts within 6e-6, and 2e-5 where appended values
-// cancel, for 12% less time.  What is read of the state (S in K S and Q S) and W have two: a third in K S takes 12% more time
-// for the rest of the difference, and the outputs are bf16 (1.7e-3); single bf16 operands would lose digits where their
-// terms cancel (a query nearly orthogonal to the state, equal keys).
+// cancel, for 12% less time.  What is read of the state (S in K S and Q S), W, and R where it meets W have two: a third in K S
+// takes 12% more time for the rest of the difference, and the outputs are bf16 (1.7e-3; their fp32 values are off by a few 1e-6
+// of their terms, which rounds one in a few thousand the other way than fp32 sums would); single bf16 operands would lose
+// digits where their terms cancel (a query nearly orthogonal to the state, equal keys).  Norms, decays, gates and beta come
+// from the hardware's reciprocal square root, exp2, log and reciprocal, 1 ulp each.
 //
 // Measured (both kernels, heads of 128 x 128, 16 key and 32 value heads, a call among others): one prompt of 8192 tokens
-// 204 us (201 MB of tokens and outputs; its 256 steps of 0.65 us are the time), 13 prompts of 32768 tokens 476 us (850 MB:
-// 1.8 TB/s; with two parts everywhere, 414 us, matrix instructions were busy 42% of the walk's cycles, vector ones 50%, LDS
-// 45%, at the 1.7 GHz that this mix leaves of the clock).  The kernels' own times below are a profiler's, which stretches
-// the short ones.
+// 203 us (201 MB of tokens and outputs; the first kernel 32, then 256 steps of 0.67 us), 13 prompts of 32768 tokens 473 us (850
+// MB: 1.8 TB/s; the first kernel 120; with two parts everywhere, 414 us, matrix instructions were busy 42% of the walk's
+// cycles, vector ones 50%, LDS 45%, at the 1.7 GHz that this mix leaves of the clock).  A profiler has more for the same
+// kernels, 36 + 212 and 131 + 412; where forms of one kernel are compared below, the times are its.
 #include <atomic>
 #include <type_traits>
 
@@ -188,7 +190,7 @@ __device__ __forceinline__ void store_chunk(char* out, const unsigned (&at)[8], 
 }
 
 // ---- T' and W of every chunk ---------------------------------------------------------------------------------------------
-// 35 us for 8192 tokens (256 chunks, 32 heads), 130 us for 32768: 530 MB of keys, queries and results, 4 TB/s, and 53% of the
+// 32 us for 8192 tokens (256 chunks, 32 heads), 120 us for 32768: 530 MB of keys, queries and results, 4.4 TB/s, and 53% of the
 // vector units' cycles.  One wave a chunk and value head.  (I + A)^-1 by forward substitution in its two diagonal blocks of 16
 // (a column a lane) and -T11 A10 T00 below them by fp32 matrix instructions: substitution stays accurate where powers of A
 // would not (equal keys without decay make them grow like binomials).
@@ -394,9 +396,9 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
 // Chunk c is requested in step c - 1 - AHEAD, has landed when step c - 1 begins, and meets the waves in the steps c - 1 (K in
 // K_c S_{c-1} and X), c (Q, V, T', c, ..) and c + 1 (K^T in the state's update, W, d, e^{G_C}).
 //
-// A step ends when the slowest wave has done its part.  8192 tokens take 202 us.  With two parts everywhere it was 173: of a
-// step's 1500 cycles the state's waves worked 1390, the chain 1110, the others 820 to 1190, and LDS moved 125 KB, 970 cycles'
-// worth.  X by way of LDS to its operand's layout took 12 us more.  Not kept (of 173): X from the first kernel (166, but 8 more
+// A step ends when the slowest wave has done its part.  8192 tokens take 171 us.  With two parts everywhere, by the profiler
+// (which has 202 to 212 for three), it was 173: of a step's 1500 cycles the state's waves worked 1390, the chain 1110, the others
+// 820 to 1190, and LDS moved 125 KB, 970 cycles' worth.  X by way of LDS to its operand's layout took 12 us more.  Not kept (of 173): X from the first kernel (166, but 8 more
 // there), X by one wave (183), 32 channels a state wave (218: LDS), a step's tiles read into registers a step ahead (177 to
 // 189: the reads then stand before the step's end).
 constexpr int AHEAD = 2;               // chunks requested before the step that first needs one
@@ -746,8 +748,8 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
 
 // ---- the walk with a wave alone for 16 rows --------------------------------------------------------------------------------
 // All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all (74 matrix ones a chunk), and LDS
-// for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768 tokens: 406 us.
-// With two parts everywhere (348): a third workgroup a CU gained 2%, 32 columns a wave lost 18% (registers).
+// for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768 tokens: 350 us.
+// With two parts everywhere (by the profiler 348, against 406 to 412 with three): a third workgroup a CU gained 2%, 32 columns a wave lost 18% (registers).
 template <int K, int NW>
 struct Pair {                          // places in LDS of the two chunks, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB, VB = 2 * NW, VU = C * VB;
@@ -923,14 +925,17 @@ int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
   chunk_kernel<K><<<(unsigned)((seq_runs<C>(s) * d->HV + CHUNKS - 1) / CHUNKS) + 1, 64 * CHUNKS, 0, st>>>(*d, *s, work, order);
   if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
   auto grid = [&](int parts) { return (unsigned)place_grid((long long)s->N * d->H, d->HV / d->H * parts); };
-  // Up to half a CU for every 16 rows the walk spreads each over eight waves (0.65 us a chunk, one workgroup a CU); with more
-  // of them, one (1.2 to 2.3 us, several a CU).  Eight | one, both kernels, 2048 tokens a sequence in the mean, 128 x 128,
-  // measured with two parts everywhere (three add 10% to either):
-  //   times 16 rows    256 (1 x 32 heads)    384 (6 x 8)    512 (2 x 32)    512 (8 x 8)    768 (3 x 32)    1024 (4 x 32)
-  //   equal lengths         62 |  95          102 |  99      110 | 104       106 | 101      154 | 115       198 | 131 us
-  //   random cuts           62 |  94          158 | 290      105 | 148       112 | 182      152 | 198       200 | 235
-  // Lengths are known on the device only, and prompts are rarely equal: twice the CUs, where equal ones lose 6%.  16 heads of
-  // 64 x 64: 512 (8 sequences) 99 | 86, 102 | 145; 768 139 | 98, 150 | 179.
+  // Up to half a CU for every 16 rows the walk spreads each over eight waves (0.67 us a chunk, one workgroup a CU); with more
+  // of them, one (1.2 to 2.3 us, several a CU).  Eight | one, both kernels, 2048 tokens a sequence in the mean, 128 x 128 (random
+  // cuts: the mean of two draws):
+  //   times 16 rows   256 (1 x 32 heads)  384 (6 x 8)  512 (2 x 32)  512 (8 x 8)  640 (10 x 8)  768 (3 x 32)  1024 (4 x 32)
+  //   equal lengths        70 | 106        112 | 110    118 | 115     114 | 111    162 | 116     167 | 127     213 | 144 us
+  //   random cuts          66 | 105        179 | 328    115 | 164     126 | 204    172 | 294     165 | 222     218 | 264
+  // 16 heads of 64 x 64: 512 (8 sequences) 113 | 94, 121 | 160; 768 160 | 105, 177 | 198; 1024 212 | 127, 230 | 217.
+  // Lengths are known on the device only.  Up to twice the CUs eight waves lose little at equal lengths (3%; 64 x 64: 20%) and
+  // gain more at others.  Above, where a CU takes a third workgroup in turn, neither is right for all: equal lengths lose 31 to
+  // 67% by eight waves, random cuts up to 70% by one.  One it is there: what it loses, the CUs that wait for the longest
+  // sequences, shrinks with more of them (71% at 640, 15 to 21% at 1024).
   if ((long long)s->N * d->HV * (V / 16) <= 2 * lq_seq_cus())
     walk_kernel<K, V><<<grid(V / 16), 64 * (ROLES + SERVICE), T::BYTES, st>>>(*d, *s, work, order);
   else

@@ -5,9 +5,10 @@
 // A row is held by LANES threads (8 to 256), CH groups of VEC elements each, groups of one thread LANES * VEC apart so that a
 // load instruction covers consecutive bytes.  LANES <= 64 reduces by lane exchanges, above that through LDS.
 //
-// Measured: gated, 32768 rows of 32 heads of 128, 146 us (805 MB: 5.5 TB/s); add, 16385 rows of 2048, 47 us (268 MB:
-// 5.7 TB/s), both past a large copy's 4.9; without the hints that calls larger than the shared cache give (ONCE) 150 and
-// 49.5.  64 rows take 3.4 us, a launch and a load.
+// Measured: gated, 32768 rows of 32 heads of 128, 140 us (805 MB: 5.7 TB/s); add, 16385 rows of 2048, 46.6 us (268 MB:
+// 5.8 TB/s), both past a large copy's 4.9; the hints that calls larger than the shared cache give (ONCE) are 2 and 6% of
+// that.  64 rows take 2.9 us, a launch and a load.  Not at that rate: rows of 513 to 1024 elements, where half the threads
+// of a row have none (16384 rows of 1024: 3.8 and 4.6 TB/s), and 2-byte loads (of 2049: 1.9 and 2.2).
 #include "lq_seq.h"
 
 namespace {

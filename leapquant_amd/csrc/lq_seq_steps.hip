@@ -168,9 +168,12 @@ long long grid_of(const lq_delta* d, const lq_seqs* s) { return (long long)s->N 
 template <int K, int V, int ROWS, bool KDA>
 int launch_rows(const lq_delta* d, const lq_seqs* s, hipStream_t st) {
   const long long grid = grid_of(d, s);
-  // States that fit the shared cache are written past it, which leaves it to those that are read: where one layer's states take
-  // turns in it, 64 sequences of 8 tokens take 68 us instead of 77, 32 of 4 (KDA) 35 instead of 39; where other data fill
-  // it, the same.  Beyond its size that gains nothing, and after other writes 256 sequences lose 18%.
+  // States that fit the shared cache are written past it, which leaves it to those that are read.  With the hint | without, 32
+  // heads of 128 x 128, to other slots: 64 sequences of 4 tokens 47 | 54 us, 32 of 4 27 | 29 (where other data fill the cache,
+  // the same).  In place, where the next call reads what this one wrote: four layers in turn, as a model has them, 54 | 61 and
+  // 29.5 | 30; one layer over and over 53 | 48 and 30 | 28; with the 8-bit quantize of all states right after it 98 | 95 and
+  // 53 | 52; single tokens the same either way.  Beyond the cache's size it gains nothing, and after other writes 256
+  // sequences lose 18%.
   if (4ll * s->N * d->HV * V * K <= 256ll << 20) steps_kernel<K, V, ROWS, KDA, true><<<(unsigned)grid, 256, 0, st>>>(*d, *s);
   else steps_kernel<K, V, ROWS, KDA, false><<<(unsigned)grid, 256, 0, st>>>(*d, *s);
   return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
