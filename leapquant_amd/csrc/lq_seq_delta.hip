@@ -398,9 +398,9 @@ void chunk_kernel(lq_delta p, lq_seqs s, Coef* __restrict__ work, int* __restric
 //
 // A step ends when the slowest wave has done its part.  8192 tokens take 171 us.  With two parts everywhere, by the profiler
 // (which has 202 to 212 for three), it was 173: of a step's 1500 cycles the state's waves worked 1390, the chain 1110, the others
-// 820 to 1190, and LDS moved 125 KB, 970 cycles' worth.  X by way of LDS to its operand's layout took 12 us more.  Not kept (of 173): X from the first kernel (166, but 8 more
-// there), X by one wave (183), 32 channels a state wave (218: LDS), a step's tiles read into registers a step ahead (177 to
-// 189: the reads then stand before the step's end).
+// 820 to 1190, and LDS moved 125 KB, 970 cycles' worth.  X by way of LDS to its operand's layout took 12 us more.  Not kept (of
+// 173): X from the first kernel (166, but 8 more there), X by one wave (183), 32 channels a state wave (218: LDS), a step's tiles
+// read into registers a step ahead (177 to 189: the reads then stand before the step's end).
 constexpr int AHEAD = 2;               // chunks requested before the step that first needs one
 constexpr int SERVICE = 4;             // service waves of a workgroup
 constexpr int ROLES = 4;               // waves of 16 rows of the state: chain, two halves of the channels, outputs
@@ -749,7 +749,8 @@ void walk_kernel(lq_delta p, lq_seqs s, const Coef* __restrict__ work, const int
 // ---- the walk with a wave alone for 16 rows --------------------------------------------------------------------------------
 // All of a chunk in one wave, R = V - c K S straight from the state: fewer instructions in all (74 matrix ones a chunk), and LDS
 // for two chunks only, so that two workgroups share a CU and fill each other's waits.  13 sequences of 32768 tokens: 350 us.
-// With two parts everywhere (by the profiler 348, against 406 to 412 with three): a third workgroup a CU gained 2%, 32 columns a wave lost 18% (registers).
+// With two parts everywhere (by the profiler 348, against 406 to 412 with three): a third workgroup a CU gained 2%, 32 columns a
+// wave lost 18% (registers).
 template <int K, int NW>
 struct Pair {                          // places in LDS of the two chunks, in 16-byte blocks
   static constexpr int RB = K / 8, TU = C * RB, VB = 2 * NW, VU = C * VB;
@@ -910,7 +911,8 @@ template <int K, int V> bool walk_lds() {
   if (hipGetDevice(&dev) != hipSuccess) return false;
   const bool known = dev >= 0 && dev < 64;
   if (known && had[dev].load(std::memory_order_relaxed)) return true;
-  if (hipFuncSetAttribute((const void*)walk_kernel<K, V>, hipFuncAttributeMaxDynamicSharedMemorySize, Tiles<K>::BYTES) != hipSuccess)
+  if (hipFuncSetAttribute((const void*)walk_kernel<K, V>, hipFuncAttributeMaxDynamicSharedMemorySize,
+                          Tiles<K>::BYTES) != hipSuccess)
     return false;
   if (known) had[dev].store(true, std::memory_order_relaxed);
   return true;
@@ -946,7 +948,8 @@ int prefill(const lq_delta* d, const lq_seqs* s, Coef* work, hipStream_t st) {
 }  // namespace
 
 __attribute__((visibility("hidden"))) bool lq_prefill_fits(const lq_delta* d, const lq_seqs* s) {
-  return (seq_runs<C>(s) + 8) * d->HV <= 0x7fffffffll && ((long long)s->N * d->HV + 8) * 8 <= 0x7fffffffll && d->mixed_ld <= (1 << 24);
+  return (seq_runs<C>(s) + 8) * d->HV <= 0x7fffffffll && ((long long)s->N * d->HV + 8) * 8 <= 0x7fffffffll &&
+         d->mixed_ld <= (1 << 24);
 }
 
 extern "C" long long lq_delta_workspace(const lq_delta* d, const lq_seqs* s) {
