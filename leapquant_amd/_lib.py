@@ -1,4 +1,4 @@
-"""ctypes binding of liblq.so (include/lq.h) and liblq_seq.so (include/lq_seq.h).  The product path has no fallback: if a
+"""ctypes binding of liblq.so (include/lq.h), liblq_seq.so (include/lq_seq.h) and liblq_attn.so (include/lq_attn.h).  The product path has no fallback: if a
 library is missing or a call fails, this raises."""
 import ctypes
 import importlib.machinery
@@ -10,8 +10,11 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_build", "liblq.so")
 SEQ_LIB_PATH = os.path.join(_HERE, "_build", "liblq_seq.so")
 SEQ_CALL_PATH = os.path.join(_HERE, "_build", "lq_seq_call.so")
+ATTN_LIB_PATH = os.path.join(_HERE, "_build", "liblq_attn.so")
+ATTN_CALL_PATH = os.path.join(_HERE, "_build", "lq_attn_call.so")
 ABI_VERSION = 6
 SEQ_ABI_VERSION = 1
+ATTN_ABI_VERSION = 1
 SCHED_INTS = 512           # include/lq.h: LQ_SCHED_INTS
 
 c_void_p, c_int, c_float, c_ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
@@ -52,6 +55,30 @@ class LqNorm(ctypes.Structure):
                [("act", c_int), ("weight_bf16", c_int)]
 
 
+class LqPages(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, c_ll) for n in ("page_ld", "row_ld", "head_ld", "s_page_ld", "s_row_ld", "s_head_ld")] + \
+               [(n, c_int) for n in ("NP", "page", "HK", "D", "int8")]
+
+
+class LqBatch(ctypes.Structure):
+    _fields_ = [("loc", c_void_p), ("lens", c_void_p), ("table", c_void_p), ("table_ld", c_ll), ("width", c_int), ("N", c_int),
+                ("T", c_int)]
+
+
+class LqRows(ctypes.Structure):
+    _fields_ = [("p", c_void_p), ("ld", c_ll), ("hd", c_ll)]
+
+
+class LqRope(ctypes.Structure):
+    _fields_ = [(n, LqRows) for n in ("q", "k", "v", "out")] + [(n, c_void_p) for n in ("q_weight", "k_weight", "inv_freq")] + \
+               [(n, c_int) for n in ("HQ", "rot", "weight_bf16", "freq64", "interleaved")] + [("eps", c_float), ("offset", c_float)]
+
+
+class LqAttention(ctypes.Structure):
+    _fields_ = [(n, LqRows) for n in ("q", "gate", "out")] + [("HQ", c_int), ("window", c_int), ("scale", c_float)]
+
+
 # exported symbol -> (restype, argtypes); must match include/lq.h
 SIGNATURES = {
     "lq_abi_version": (c_int, []),
@@ -87,6 +114,14 @@ SEQ_SIGNATURES = {
     "lq_conv_seq": (c_int, [c_void_p, c_void_p, c_void_p, c_ll, c_void_p, c_int, c_void_p]),
     "lq_gated_norm": (c_int, [c_void_p, c_void_p]),
     "lq_add_norm": (c_int, [c_void_p, c_void_p]),
+}
+# the same of include/lq_attn.h
+ATTN_SIGNATURES = {
+    "lq_attn_abi_version": (c_int, []),
+    "lq_rope_norm": (c_int, [ctypes.POINTER(LqRope), ctypes.POINTER(LqPages), ctypes.POINTER(LqBatch), c_void_p]),
+    "lq_attend": (c_int, [ctypes.POINTER(LqAttention), ctypes.POINTER(LqPages), ctypes.POINTER(LqBatch), c_int, c_void_p, c_ll,
+                          c_void_p]),
+    "lq_attend_workspace": (c_ll, [ctypes.POINTER(LqAttention), ctypes.POINTER(LqPages), ctypes.POINTER(LqBatch), c_int]),
 }
 _SEQS, _DELTA, _NORM = struct.Struct("@3P2i0P"), struct.Struct("@Pq5i6P3qf2if0P"), struct.Struct("@5P6q3i3f2i0P")
 for _layout, _type in ((_SEQS, LqSeqs), (_DELTA, LqDelta), (_NORM, LqNorm)):
@@ -127,25 +162,46 @@ def seq_lib():
 
 
 _SEQ_CALL = [None]
+_ATTN_LIB = [None]
+_ATTN_CALL = [None]
+
+
+def _extension(name, path, version):
+    """A Python extension in front of one of the libraries (raises if it has not been built, or for other structures than
+    those of this binding, or against another torch)."""
+    import torch
+    if not os.path.exists(path):
+        raise RuntimeError("%s is missing: build it with python -m leapquant_amd.build" % path)
+    loader = importlib.machinery.ExtensionFileLoader(name, path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_file_location(name, path, loader=loader))
+    loader.exec_module(module)
+    built = getattr(module, "ABI", None), getattr(module, "TORCH", None)
+    if built != (version, torch.__version__):
+        raise RuntimeError("%s.so: ABI %s with torch %s, expected %d with %s: rebuild it" % ((name,) + built + (version, torch.__version__)))
+    return module
 
 
 def seq_call():
-    """The loaded lq_seq_call.so, a Python extension (raises if it has not been built, or for other structures than those of
-    this binding, or against another torch)."""
+    """The loaded lq_seq_call.so."""
     if _SEQ_CALL[0] is None:
-        import torch
         seq_lib()                        # the library behind it, of the same version
-        if not os.path.exists(SEQ_CALL_PATH):
-            raise RuntimeError("%s is missing: build it with python -m leapquant_amd.build" % SEQ_CALL_PATH)
-        loader = importlib.machinery.ExtensionFileLoader("lq_seq_call", SEQ_CALL_PATH)
-        module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("lq_seq_call", SEQ_CALL_PATH, loader=loader))
-        loader.exec_module(module)
-        built = getattr(module, "ABI", None), getattr(module, "TORCH", None)
-        if built != (SEQ_ABI_VERSION, torch.__version__):
-            raise RuntimeError("lq_seq_call.so: ABI %s with torch %s, expected %d with %s: rebuild it"
-                               % (built + (SEQ_ABI_VERSION, torch.__version__)))
-        _SEQ_CALL[0] = module
+        _SEQ_CALL[0] = _extension("lq_seq_call", SEQ_CALL_PATH, SEQ_ABI_VERSION)
     return _SEQ_CALL[0]
+
+
+def attn_lib():
+    """The loaded liblq_attn.so (raises if it has not been built)."""
+    if _ATTN_LIB[0] is None:
+        _ATTN_LIB[0] = _load(ATTN_LIB_PATH, ATTN_SIGNATURES, "lq_attn_abi_version", ATTN_ABI_VERSION)
+    return _ATTN_LIB[0]
+
+
+def attn_call():
+    """The loaded lq_attn_call.so."""
+    if _ATTN_CALL[0] is None:
+        attn_lib()                       # the library behind it, of the same version
+        _ATTN_CALL[0] = _extension("lq_attn_call", ATTN_CALL_PATH, ATTN_ABI_VERSION)
+    return _ATTN_CALL[0]
 
 
 _ERR = {-1: "bad argument (unsupported shape / size / pointer)", -2: "HIP launch error",
