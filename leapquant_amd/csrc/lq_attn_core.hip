@@ -21,16 +21,14 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) char lds_t;
 typedef const __attribute__((address_space(4))) int const_int;     // what no kernel of the call writes: scalar loads
 
-// The launches of a call: the few rows of a decode or draft (kernel A: a sequence's rows in one wave, waves share out the
-// keys) and the many of a prompt (kernel B: waves share out the rows of a tile, tiles numbered over the batch).
 struct Plan {
-  int few, splits;         // rows up to which a sequence is the other kernel's (A: none); pieces of the keys at most
+  int few, splits;         // rows up to which a sequence is the other kernel's (0: none); pieces of the keys at most
   int G;
-  uint32_t g_mul;          // x / G = x * g_mul >> 32 for x < 2^16.., see rows_div
   PageDiv div;
   float* work;
 };
@@ -38,24 +36,34 @@ struct Plan {
 constexpr float GROWN = 8.f;
 constexpr float LOG2E = 1.44269504f;
 
-__device__ __forceinline__ f32x16 mfma(const u32x4& a, const u32x4& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 __device__ __forceinline__ u32x4 lds_read16(const char* p) { return *(const u32x4*)p; }
 __device__ __forceinline__ u32x2 lds_read_tr(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_t*)p));
 }
+__device__ __forceinline__ u32x2 lds_read_tr8(const char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(lds_t*)p));
+}
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// 16 bytes a lane from base + off into LDS at lds + 16 lane; the caller waits before it reads them
-__device__ __forceinline__ void tile_load16(const char* base, uint32_t off, const char* lds) {
+// 16 (4) bytes a lane from base + off into LDS at lds + 16 lane (4 lane); the caller waits before it reads them
+__device__ __forceinline__ void load16(const char* base, uint32_t off, const char* lds) {
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(to) : "memory", "m0");
 }
+__device__ __forceinline__ void load4(const float* from, const char* lds) {
+  const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(from), "s"(to) : "memory", "m0");
+}
 #pragma clang diagnostic pop
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LEFT) : "memory"); }
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// a sequence's rows and keys, as a workgroup finds them
+// four codes of 8 bits as bf16
+__device__ __forceinline__ u32x2 codes(uint32_t w) {
+  return u32x2{pk_bf16((float)(int8_t)w, (float)(int8_t)(w >> 8)), pk_bf16((float)(int8_t)(w >> 16), (float)(int8_t)(w >> 24))};
+}
+
+// ---- sequences, keys, pieces --------------------------------------------------------------------------------------------
 struct Seq {
   int lo, rows, pos0, len;  // first packed token, rows (tokens x G), position of the first new token, cached tokens
 };
@@ -81,10 +89,10 @@ __device__ __forceinline__ Keys keys_of(const Seq& s, int G, int r0, int r1, int
 }
 // tiles of KT keys [t0, t1) that piece `split` of a row tile's keys holds, and how many pieces there are
 struct Piece { int t0, t1, pieces; };
-template <int KT, int LEAST> __device__ __forceinline__ Piece piece_of(const Keys& k, int splits, int split) {
-  const int a = k.lo / KT, b = (k.hi + KT - 1) / KT, tiles = max(b - a, 0);
+template <class S> __device__ __forceinline__ Piece piece_of(const Keys& k, int splits, int split) {
+  const int a = k.lo / S::KT, b = (k.hi + S::KT - 1) / S::KT, tiles = max(b - a, 0);
   Piece p;
-  p.pieces = max(min(splits, tiles / LEAST), 1);
+  p.pieces = max(min(splits, tiles / S::LEAST), 1);
   const int per = (tiles + p.pieces - 1) / p.pieces;
   p.pieces = max((tiles + per - 1) / max(per, 1), 1);          // none is empty
   p.t0 = a + split * per;
@@ -92,385 +100,373 @@ template <int KT, int LEAST> __device__ __forceinline__ Piece piece_of(const Key
   return p;
 }
 
-// Rows of a row tile: D is the head's size; RW waves of 32 rows share a tile of keys, KW of them (or groups of RW) each take
-// tiles of their own.
-template <int D_, int RW_, int KW_, int KT_, int LEAST_, bool I8_> struct Shape {
-  static constexpr int D = D_, RW = RW_, KW = KW_, KT = KT_, LEAST = LEAST_;
-  static constexpr bool I8 = I8_;
-  static constexpr int WAVES = RW * KW, THREADS = 64 * WAVES, ROWS = 32 * RW;
-  static constexpr int TILE = KT * D * 2;                      // bytes of a tile of K or V in LDS
-  static constexpr int STAGE = 2 * KW * TILE;
-  static constexpr int SCALES = I8 ? 2 * KW * 2 * KT * 4 : 0;
-  static constexpr int JOIN = KW > 1 ? KW * ROWS * (D + 4) * 4 + KW * ROWS * 8 : 0;
-  static constexpr int LDS0 = 2 * STAGE + SCALES;
-  static constexpr int LDS = LDS0 > JOIN ? LDS0 : JOIN;
-  static constexpr int PART = ROWS * (D + 2);                  // floats of a workgroup's part of split keys
+// ---- 32 keys and the rows of a wave -----------------------------------------------------------------------------------
+// R = 32: 32 x 32 x 16 products, R = 16: 16 x 16 x 32.  A lane (group g = lane / R) holds E of 32 scores of the row lane % R: the
+// i-th is of key STEP (i / 4) + 4 g + i % 4.  Eight in a row are a right operand of the second product (F of them).
+template <int R> struct Rows;
+template <> struct Rows<32> {
+  typedef f32x16 acc;
+  static constexpr int E = 16, F = 2, STEP = 8, A = 1, AN = 16, DM = 32;    // A accumulators of AN; channels of an output
+  static __device__ __forceinline__ acc mfma(const u32x4& a, const u32x4& b, const acc& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float max_over(float x) { return xor32_max(x); }
+  static __device__ __forceinline__ float sum_over(float x) { return xor32_sum(x); }
+};
+template <> struct Rows<16> {
+  typedef f32x4 acc;
+  static constexpr int E = 8, F = 1, STEP = 16, A = 2, AN = 4, DM = 16;
+  static __device__ __forceinline__ acc mfma(const u32x4& a, const u32x4& b, const acc& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float max_over(float x) { return xor32_max(xor16_max(x)); }
+  static __device__ __forceinline__ float sum_over(float x) { return xor32_sum(xor16_sum(x)); }
 };
 
-template <class S> __device__ __forceinline__ int swizzle_k(int key) { return key & 7; }
-template <class S> __device__ __forceinline__ int swizzle_v(int key) { return S::D == 64 ? (key & 3) << 1 : (key & 7) << 1; }
-
-// The work of a workgroup: rows [r0, r0 + ROWS) of a sequence and head hk of the cache, piece `split` of the keys.
-template <class S>
-__device__ __forceinline__ void attend(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds,
-                                       int n, int hk, int split, int splits, int r0, const Seq& sq, float* part) {
-  constexpr int D = S::D, RW = S::RW, KW = S::KW, KT = S::KT, TILE = S::TILE, KB = KT / 32, MB = D / 32, KS = D / 16;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW, kw = wave / RW;
-  const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-  const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
-  const Keys keys = keys_of(sq, G, r0, r0 + rows, a.window);
-  const Piece piece = piece_of<KT, S::LEAST>(keys, splits, split);
-  if (split >= piece.pieces) return;
-
-  // this lane's row
-  const int row = r0 + 32 * rw + col, rc = min(row, r0 + rows - 1);
-  const int tok = rc / G, g = rc - tok * G, pos = sq.pos0 + tok, head = hk * G + g;
-  const bool busy = 32 * rw < rows;                            // the wave has rows
-  const int first = sq.pos0 + min(r0 + 32 * rw, r0 + rows - 1) / G, last = sq.pos0 + (min(r0 + 32 * rw + 32, r0 + rows) - 1) / G;
-  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;               // keys from .. pos are seen
-  const int wave_from = a.window > 0 ? max(first - a.window + 1, 0) : 0;        // the wave's first and last key
-  const int wave_full = a.window > 0 ? max(last - a.window + 1, 0) : 0;         // all rows see wave_full .. first
-  u32x4 q[KS];
-  {
-    const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)head * a.q.hd + 8 * half;
+// What a wave carries along its keys: outputs O^T, a row's running maximum (of q . k, not scaled) and sum.
+template <int R, int D> struct Run {
+  typedef Rows<R> W;
+  static constexpr int MB = D / W::DM;
+  typename W::acc o[MB];
+  float m, l;
+  __device__ __forceinline__ void start() {
+    m = -INFINITY;
+    l = 0.f;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 16 * s);
+    for (int i = 0; i < MB; ++i) o[i] = typename W::acc(0.f);
   }
+};
 
-  // ---- tiles: this wave loads KT / RW keys of its group's tile -----------------------------------------------------------
-  constexpr int OWN = KT / RW, GROUPS = OWN > 16 ? OWN / 16 : 1, GK = OWN / GROUPS;    // keys a wave loads, in groups of one page
-  const int* tab = b.table + (long long)n * b.table_ld;
-  const char* kbase = (const char*)pg.k + (long long)hk * pg.head_ld * (S::I8 ? 1 : 2);
-  const char* vbase = (const char*)pg.v + (long long)hk * pg.head_ld * (S::I8 ? 1 : 2);
-  constexpr int PER = S::I8 ? 16 : 8;                          // elements of a 16-byte load
-  constexpr int CPR = D / PER, LOADS = GK * CPR / 64 > 0 ? GK * CPR / 64 : 1;
-  static_assert(GK * CPR >= 64 || S::I8, "a load of a whole wave");
-  u32x4 kreg[S::I8 ? GROUPS * LOADS : 1], vreg[S::I8 ? GROUPS * LOADS : 1];
-  float ksc = 0.f, vsc = 0.f;
-  const int tend = max(sq.len - 1, 0);
-  auto stage = [&](int t, int buf) {                           // t: the tile
-    const int k0 = t * KT + rw * OWN;
+// Softmax and second product of 32 keys' scores s.  Keys of lo .. hi (places in the 32, less 4 g) are seen where `masked`.
+// vscale: scales of the values, by places as s, or nothing.  value(f, i): the f-th operand of values for the channels of o[i].
+template <int R, int D, bool I8, class V>
+__device__ __forceinline__ void soft_step(Run<R, D>& run, typename Rows<R>::acc (&s)[Rows<R>::A], float c, bool masked, int lo, int hi,
+                                          const float* vscale, const V& value) {
+  typedef Rows<R> W;
+  constexpr int E = W::E, AN = W::AN, MB = Run<R, D>::MB;
+  if (masked) {
 #pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-      const int kg = min(k0 + 16 * i, OWN >= 16 ? tend & ~15 : (tend & ~(OWN - 1)));
-      const int pi = __builtin_amdgcn_readfirstlane(page_of(pl.div, kg));
-      int page = __builtin_amdgcn_readfirstlane(((const_int*)tab)[pi]);
-      page = page >= 0 && page < pg.NP ? page : 0;
-      const int in = kg - pi * pg.page;
-      const long long base = (long long)page * pg.page_ld + (long long)in * pg.row_ld;
-      const int most = tend - kg;                              // places of the group's last cached token
-      const char *kp = kbase + base * (S::I8 ? 1 : 2), *vp = vbase + base * (S::I8 ? 1 : 2);
-      if constexpr (!S::I8) {
+    for (int i = 0; i < E; ++i) {
+      const int j = W::STEP * (i >> 2) + (i & 3);
+      s[i / AN][i % AN] = j >= lo && j <= hi ? s[i / AN][i % AN] : -INFINITY;
+    }
+  }
+  float mx = s[0][0];
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          const int c = 64 * j + lane, key = c / CPR, tk = rw * OWN + 16 * i + key;
-          const uint32_t off = (uint32_t)min(key, most) * (uint32_t)(2 * pg.row_ld);
-          char* to = lds + buf * S::STAGE + (2 * kw) * TILE + (rw * OWN + 16 * i) * D * 2 + 1024 * j;
-          tile_load16(kp, off + 16 * ((c % CPR) ^ swizzle_k<S>(tk)), to);
-          tile_load16(vp, off + 16 * ((c % CPR) ^ swizzle_v<S>(tk)), to + TILE);
-        }
-      } else {
+  for (int i = 1; i < E; ++i) mx = fmaxf(mx, s[i / AN][i % AN]);
+  mx = W::max_over(mx);
+  if (__any((mx - run.m) * c > GROWN)) {
+    const float to = fmaxf(run.m, mx), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((run.m - to) * c);
+    run.m = to;
+    run.l *= alpha;
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          const int c = 64 * j + lane, key = min(c / CPR, GK - 1);
-          const uint32_t off = (uint32_t)min(key, most) * (uint32_t)pg.row_ld + 16 * (c % CPR);
-          kreg[i * LOADS + j] = *(const u32x4*)(kp + off);
-          vreg[i * LOADS + j] = *(const u32x4*)(vp + off);
-        }
+    for (int i = 0; i < MB; ++i) run.o[i] *= alpha;
+  }
+  const float raw = run.m == -INFINITY ? 0.f : run.m, ref = raw * c;
+  // s c - ref is rounded once, but ref itself is off by half its last place, which 2^ref would be too much for beyond 2^24
+  if (__any(fabsf(ref) > 0x1p24f)) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[i / AN][i % AN] = (s[i / AN][i % AN] - raw) * c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) s[i / AN][i % AN] = fmaf(s[i / AN][i % AN], c, -ref);
+  }
+  float part[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    s[i / AN][i % AN] = __builtin_amdgcn_exp2f(s[i / AN][i % AN]);
+    part[i & 1] += s[i / AN][i % AN];
+  }
+  run.l += part[0] + part[1];
+  if constexpr (I8) {
+#pragma unroll
+    for (int i = 0; i < E; i += 4) {
+      const f32x4 x = *(const f32x4*)(vscale + W::STEP * (i >> 2));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = W::STEP * (i >> 2) + e;
+        const float y = s[i / AN][i % AN + e] * x[e];
+        s[i / AN][i % AN + e] = !masked || (j >= lo && j <= hi) ? y : 0.f;     // a scale that is not finite, not seen
       }
     }
-    if constexpr (S::I8) {                                     // lane's scale: key `lane` of the wave's (at most 64)
-      const int kk = min(k0 + min(lane, OWN - 1), tend);
-      const int pi = page_of(pl.div, kk);
-      int page = tab[pi];
+  }
+  u32x4 p[W::F];
+#pragma unroll
+  for (int i = 0; i < E / 2; ++i) p[i >> 2][i & 3] = pk_bf16(s[2 * i / AN][2 * i % AN], s[2 * i / AN][2 * i % AN + 1]);
+#pragma unroll
+  for (int f = 0; f < W::F; ++f)
+#pragma unroll
+    for (int i = 0; i < MB; ++i) run.o[i] = W::mfma(value(f, i), p[f], run.o[i]);
+}
+// whether 32 rows of D bf16 in LDS hold an infinity or NaN
+template <int D> __device__ __forceinline__ bool tile_not_finite(const char* tile) {
+  const int lane = threadIdx.x & 63;
+  uint32_t hit = 0;
+#pragma unroll 4
+  for (int i = 0; i < D / 16; ++i) {
+    const u32x4 w = lds_read16(tile + (lane & 31) * 2 * D + 16 * ((lane >> 5) + 2 * i));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = (w[e] & 0x7f807f80u) ^ 0x7f807f80u;   // a half of zero: an exponent of ones
+      hit |= (x - 0x00010001u) & ~x & 0x80008000u;
+    }
+  }
+  return __any(hit != 0);
+}
+
+// Rows [ra, rb) of a sequence again, key by key: for a wave that met values which are not finite in a tile that not all of its rows
+// see.  The products give a key that a row does not see a probability of zero, and zero times an infinity or NaN is not zero.  Keys
+// are those of the wave, 32 u .. 32 u + 31 for u = u0, u0 + step .. < u1.  sink(row, m, l, y): channels D / 64 lane .. of a row.
+template <int D, class F>
+__device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, int n, int hk,
+                                           const Seq& sq, int ra, int rb, int u0, int u1, int step, const F& sink) {
+  constexpr int C = D / 64;
+  const int lane = threadIdx.x & 63, tend = max(sq.len - 1, 0);
+  const float c = a.scale * LOG2E;
+  for (int r = ra; r < rb; ++r) {
+    const int tok = r / pl.G, pos = sq.pos0 + tok, from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    const bf16_t* q = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * pl.G + r - tok * pl.G) * a.q.hd;
+    float m = -INFINITY, l = 0.f, y[C] = {};
+    for (int u = u0; u < u1; u += step) {
+      if (32 * u > pos || 32 * u + 31 < from) continue;
+      const int key = 32 * u + (lane & 31), kk = min(key, tend), pi = page_of(pl.div, kk);
+      const bool sees = lane < 32 && key >= from && key <= pos;
+      int page = b.table[(long long)n * b.table_ld + pi];
       page = page >= 0 && page < pg.NP ? page : 0;
-      const long long at = (long long)page * pg.s_page_ld + (kk - pi * pg.page) * pg.s_row_ld + hk * pg.s_head_ld;
-      ksc = pg.k_scale[at];
-      vsc = pg.v_scale[at];
+      const long long at = (long long)page * pg.page_ld + (long long)(kk - pi * pg.page) * pg.row_ld + (long long)hk * pg.head_ld;
+      float s = 0.f;
+      for (int i = 0; i < D; i += 8) {
+        const u32x4 x = *(const u32x4*)(q + i), k = *(const u32x4*)((const bf16_t*)pg.k + at + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s = fmaf(bf_hi(x[e]), bf_hi(k[e]), fmaf(bf_lo(x[e]), bf_lo(k[e]), s));
+      }
+      if (!sees) s = -INFINITY;
+      const float to = fmaxf(m, max64(s)), raw = to == -INFINITY ? 0.f : to;
+      const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - raw) * c);
+      const float p = sees ? __builtin_amdgcn_exp2f((s - raw) * c) : 0.f;
+      m = to;
+      l = fmaf(l, alpha, sum64(p));
+#pragma unroll
+      for (int e = 0; e < C; ++e) y[e] *= alpha;
+      for (int j = 0; j < 32; ++j) {
+        if (32 * u + j < from || 32 * u + j > pos) continue;
+        const float pj = __shfl(p, j);
+        const long long vj = __shfl(at, j);
+#pragma unroll
+        for (int e = 0; e < C; ++e) y[e] = fmaf(pj, bf2f(((const bf16_t*)pg.v)[vj + C * lane + e]), y[e]);
+      }
+    }
+    sink(r, m, l, y);
+  }
+}
+
+// ---- outputs ----------------------------------------------------------------------------------------------------------------
+// sigmoid(gate) of 4 neighbours
+__device__ __forceinline__ f32x4 gate4(const lq_rows& gate, long long token, int head, int d) {
+  const u32x2 w = *(const u32x2*)((const bf16_t*)gate.p + token * gate.ld + (long long)head * gate.hd + d);
+  const f32x4 z = {bf_lo(w[0]), bf_hi(w[0]), bf_lo(w[1]), bf_hi(w[1])};
+  f32x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_rcpf(1.0f + __expf(-z[e]));
+  return y;
+}
+__device__ __forceinline__ void store4(const lq_attention& a, long long token, int head, int d, f32x4 y) {
+  if (a.gate.p) y *= gate4(a.gate, token, head, d);
+  *(u32x2*)((bf16_t*)a.out.p + token * a.out.ld + (long long)head * a.out.hd + d) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+}
+
+__device__ __forceinline__ void store1(const lq_attention& a, long long token, int head, int d, float y) {
+  if (a.gate.p) y *= __builtin_amdgcn_rcpf(1.0f + __expf(-bf2f(((const bf16_t*)a.gate.p)[token * a.gate.ld + (long long)head * a.gate.hd + d])));
+  ((bf16_t*)a.out.p)[token * a.out.ld + (long long)head * a.out.hd + d] = f2bf(y);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------------
+// Up to 16 rows of a sequence (a token's heads): a wave takes all of them, the KW waves of a workgroup every KW-th tile of 32 keys,
+// each by itself: K and V of a tile have a place in LDS each, and the next tile's are asked for as soon as this one's are used, so
+// that 32 D .. 64 D elements a wave are on their way at any time.  Codes stay codes in LDS.
+template <int D_, int KW_, bool I8_> struct Few {
+  static constexpr int D = D_, KW = KW_, R = 16, ROWS = 16, KT = 32, LEAST = KW, THREADS = 64 * KW;
+  static constexpr bool I8 = I8_;
+  static constexpr int ES = I8 ? 1 : 2, RB = D * ES, CPR = RB / 16, RPL = 64 / CPR;  // bytes and chunks of a row, rows of a load
+  static constexpr int UNIT = KT * RB, LOADS = UNIT / 1024, SC = I8 ? 1 : 0;
+  static constexpr int WAVE = 2 * UNIT + SC * 512;             // K, V, the scales of two tiles
+  static constexpr int JOIN = KW * ROWS * ((D + 4) * 4 + 8);
+  static constexpr int LDS = KW * WAVE > JOIN ? KW * WAVE : JOIN;
+  static constexpr int PART = ROWS * (D + 2);                  // floats of a workgroup's part of split keys
+  // a chunk's place in its row: spread so that the reads below go over all banks
+  static __device__ __forceinline__ int place_k(int key) { return CPR >= 8 ? key & 7 : (key >> 1) & 3; }
+  static __device__ __forceinline__ int place_v(int key) {
+    if (I8) return (key & 3) | (CPR >= 8 ? (key >> 2) & 4 : 0);
+    return CPR >= 16 ? (key & 7) << 1 : (key & 3) << 1;
+  }
+};
+
+template <class S>
+__device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
+                                         int hk, int split, int splits, int r0, const Seq& sq, float* part) {
+  constexpr int D = S::D, KW = S::KW, MB = D / 16, KS = D / 32;
+  const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
+  const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), splits, split);
+  if (split >= piece.pieces) return;
+  const int rc = r0 + min(col, rows - 1), tok = rc / G, pos = sq.pos0 + tok;
+  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;              // keys from .. pos are seen
+  const int first = sq.pos0 + r0 / G, last = sq.pos0 + (r0 + rows - 1) / G;    // all rows see full .. first
+  const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+
+  char* const mine = lds + kw * S::WAVE;
+  const int* tab = b.table + (long long)n * b.table_ld;
+  const int tend = max(sq.len - 1, 0);
+  const char *at[2], *vat = (const char*)((const char*)pg.v - (const char*)pg.k);
+  int most[2], pages[2], in[2];
+  auto places = [&](int t) {                                   // where the two halves of tile t lie
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int kg = min(t * 32 + 16 * i, tend & ~15), pi = __builtin_amdgcn_readfirstlane(page_of(pl.div, kg));
+      int page = ((const_int*)tab)[pi];
+      page = page >= 0 && page < pg.NP ? page : 0;
+      pages[i] = page;
+      in[i] = kg - pi * pg.page;
+      at[i] = (const char*)pg.k + ((long long)page * pg.page_ld + (long long)in[i] * pg.row_ld + (long long)hk * pg.head_ld) * S::ES;
+      most[i] = tend - kg;
     }
   };
-  auto settle = [&](int buf) {                                 // codes in registers -> bf16 in LDS
+  const uint32_t row_bytes = (uint32_t)pg.row_ld * S::ES;
+  auto ask = [&](bool values) {                                // for K or V of the tile that places() found
+#pragma unroll
+    for (int j = 0; j < S::LOADS; ++j) {
+      const int key = S::RPL * j + lane / S::CPR, i = 2 * j / S::LOADS;
+      const uint32_t off = (uint32_t)min(key - 16 * i, most[i]) * row_bytes + 16 * ((lane % S::CPR) ^ (values ? S::place_v(key) : S::place_k(key)));
+      load16(at[i] + (values ? (size_t)vat : 0), off, mine + (values ? S::UNIT : 0) + 1024 * j);
+    }
+  };
+  auto ask_scales = [&](int odd) {                             // lanes 0 .. 31: of the keys, 32 .. 63: of the values
     if constexpr (S::I8) {
-#pragma unroll
-      for (int i = 0; i < GROUPS; ++i)
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j) {
-          const int c = 64 * j + lane, key = c / CPR, tk = rw * OWN + 16 * i + key, ch = 2 * (c % CPR);
-          if (key < GK) {
-            char* to = lds + buf * S::STAGE + (2 * kw) * TILE + tk * D * 2;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const u32x4 w = x ? vreg[i * LOADS + j] : kreg[i * LOADS + j];
-              const int sw = x ? swizzle_v<S>(tk) : swizzle_k<S>(tk);
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                u32x4 o;
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  const int two = (int)w[2 * y + (z >> 1)] >> (16 * (z & 1));
-                  o[z] = pk_bf16((float)(int8_t)two, (float)(int8_t)(two >> 8));
-                }
-                *(u32x4*)(to + x * TILE + 16 * ((ch + y) ^ sw)) = o;
-              }
-            }
-          }
-        }
-      float* sc = (float*)(lds + 2 * S::STAGE) + (buf * KW + kw) * 2 * KT + rw * OWN;
-      if (lane < OWN) { sc[lane] = ksc; sc[KT + lane] = vsc; }
+      const int p0 = pages[0], p1 = pages[1], i0 = in[0], i1 = in[1], m0 = most[0], m1 = most[1];
+      const bool far = lane & 16;
+      const int row = (far ? i1 : i0) + min(lane & 15, far ? m1 : m0);
+      const long long x = (long long)(far ? p1 : p0) * pg.s_page_ld + (long long)row * pg.s_row_ld + (long long)hk * pg.s_head_ld;
+      load4((lane < 32 ? pg.k_scale : pg.v_scale) + x, mine + 2 * S::UNIT + 256 * odd);
     }
   };
 
   const float c = a.scale * LOG2E;
-  float m = -INFINITY, l = 0.f;
-  f32x16 o[MB];
-#pragma unroll
-  for (int i = 0; i < MB; ++i) o[i] = f32x16(0.f);
-  // this lane's reads: a row of K; V by 4 keys x 16 channels a group of 16 lanes
-  const int kread = col * D * 2 + 16 * (half ^ swizzle_k<S>(col));
-  const int vkey = 4 * half + ((lane & 15) >> 2);
-  const int vread = vkey * D * 2 + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ swizzle_v<S>(vkey)) + 8 * (lane & 1);
-
-  auto tile = [&](int t, int buf) {
-    const char* K = lds + buf * S::STAGE + (2 * kw) * TILE;
-    const char* V = K + TILE;
-    const int k0 = t * KT;
-    if (!busy || k0 > last || k0 + KT <= wave_from) return;
-    f32x16 s[KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      s[kb] = f32x16(0.f);
-#pragma unroll
-      for (int i = 0; i < KS; ++i) s[kb] = mfma(lds_read16(K + kb * 32 * D * 2 + (kread ^ (32 * i))), q[i], s[kb]);
-    }
-    if constexpr (S::I8) {
-      const float* sc = (const float*)(lds + 2 * S::STAGE) + (buf * KW + kw) * 2 * KT + 4 * half;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *(const f32x4*)(sc + 32 * kb + 8 * i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[kb][4 * i + e] *= x[e];
-        }
-    }
-    const bool masked = k0 + KT - 1 > first || k0 < wave_full;
-    if (masked) {
-      const int lo = from - k0 - 4 * half, hi = pos - k0 - 4 * half;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = 32 * kb + 8 * (i >> 2) + (i & 3);
-          s[kb][i] = j >= lo && j <= hi ? s[kb][i] : -INFINITY;
-        }
-    }
-    float mx = s[0][0];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
-    mx = xor32_max(mx);
-    if (__any((mx - m) * c > GROWN)) {
-      const float to = fmaxf(m, mx), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
-      m = to;
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < MB; ++i) o[i] *= alpha;
-    }
-    const float ref = m == -INFINITY ? 0.f : m * c;
-    // s c - ref is rounded once, but ref itself is off by half its last place, which 2^ref would be too much for beyond 2^24
-    if (__any(fabsf(ref) > 0x1p24f)) {
-      const float raw = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f((s[kb][i] - raw) * c);
-    } else {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = __builtin_amdgcn_exp2f(fmaf(s[kb][i], c, -ref));
-    }
-    u32x4 pr[2 * KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) l += s[kb][i];
-      if constexpr (S::I8) {
-        const float* sc = (const float*)(lds + 2 * S::STAGE) + (buf * KW + kw) * 2 * KT + KT + 4 * half;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 x = *(const f32x4*)(sc + 32 * kb + 8 * i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = 32 * kb + 8 * i + e + 4 * half + k0;
-            const float y = s[kb][4 * i + e] * x[e];
-            s[kb][4 * i + e] = !masked || (j >= from && j <= pos) ? y : 0.f;
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) pr[2 * kb + (i >> 2)][i & 3] = pk_bf16(s[kb][2 * i], s[kb][2 * i + 1]);
-    }
-    uint32_t bad[KB] = {};                                     // keys of a masked tile whose values are not finite
-    bool some = false;
-    if (!S::I8 && masked) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        uint32_t hit = 0;
-        for (int i = 0; i < D / 16; ++i) {
-          const u32x4 w = lds_read16(V + (kb * 32 + col) * D * 2 + 16 * (half + 2 * i));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t x = (w[e] & 0x7f807f80u) ^ 0x7f807f80u;
-            hit |= (x - 0x00010001u) & ~x & 0x80008000u;
-          }
-        }
-        const unsigned long long any = __ballot(hit != 0);
-        bad[kb] = (uint32_t)any | (uint32_t)(any >> 32);
-        some |= bad[kb] != 0;
-      }
-    }
-    if (!some) {
-#pragma unroll
-      for (int t2 = 0; t2 < 2 * KB; ++t2)
-#pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          const char* at = V + t2 * 16 * D * 2 + (vread ^ (64 * i));
-          const u32x2 x = lds_read_tr(at), y = lds_read_tr(at + 8 * D * 2);
-          o[i] = mfma(u32x4{x[0], x[1], y[0], y[1]}, pr[t2], o[i]);
-        }
-    } else {
-      // The finite keys at once, then each of the others by itself, into the rows that see it alone: a zero probability times
-      // an infinity or NaN is not zero.
-#pragma unroll
-      for (int t2 = 0; t2 < 2 * KB; ++t2) {
-        const uint32_t b16 = bad[t2 >> 1] >> (16 * (t2 & 1)) & 0xffffu;
-        for (int pass = -1; pass < 16; ++pass) {
-          if (pass >= 0 && !(b16 >> pass & 1)) continue;
-          const uint32_t take = pass < 0 ? ~b16 : 1u << pass;  // keys of the 16
-          const uint32_t mine = take >> (4 * half);            // this half's: 0 .. 3 and 8 .. 11
-          u32x4 keep;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t two = mine >> (8 * (e >> 1) + 2 * (e & 1));
-            keep[e] = (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
-          }
-          const int j = k0 + 16 * t2 + pass;
-          const bool sees = pass < 0 || (j >= from && j <= pos);
-#pragma unroll
-          for (int i = 0; i < MB; ++i) {
-            const char* at = V + t2 * 16 * D * 2 + (vread ^ (64 * i));
-            const u32x2 x = lds_read_tr(at), y = lds_read_tr(at + 8 * D * 2);
-            const f32x16 d = mfma(u32x4{x[0], x[1], y[0], y[1]} & keep, pr[t2], f32x16(0.f));
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[i][e] += sees ? d[e] : 0.f;
-            __builtin_amdgcn_sched_barrier(0);                 // one product's registers at a time
-          }
-        }
-      }
-    }
-  };
-
-  // ---- the walk over the piece's tiles -----------------------------------------------------------------------------------
-  const int stages = (piece.t1 - piece.t0 + KW - 1) / KW;
-  if (stages > 0) {
-    stage(min(piece.t0 + kw, piece.t1 - 1), 0);
-    if constexpr (S::I8) settle(0);
-    for (int i = 0; i < stages; ++i) {
-      if constexpr (!S::I8) wait_loads();
-      if constexpr (S::WAVES > 1 || S::I8) __syncthreads();
-      const int t = piece.t0 + i * KW + kw, buf = i & 1;
-      if (i + 1 < stages) stage(min(t + KW, piece.t1 - 1), buf ^ 1);
-      if (t < piece.t1) tile(t, buf);
-      if constexpr (S::I8) {
-        if (i + 1 < stages) settle(buf ^ 1);
-      }
-    }
-  }
-  l = xor32_sum(l);
-
-  // ---- outputs ---------------------------------------------------------------------------------------------------------------
-  const bool whole = piece.pieces == 1;
-  if constexpr (KW == 1) {
-    if (row >= r0 + rows) return;
-    if (!whole) {
-      float* to = part + (32 * rw + col) * D;
-#pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) *(f32x4*)(to + 32 * i + 8 * e + 4 * half) = f32x4{o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
-      if (half == 0) { part[S::ROWS * D + 32 * rw + col] = m; part[S::ROWS * (D + 1) + 32 * rw + col] = l; }
-      return;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    bf16_t* to = (bf16_t*)a.out.p + (long long)(sq.lo + tok) * a.out.ld + (long long)head * a.out.hd + 4 * half;
-    const bf16_t* gate = a.gate.p ? (const bf16_t*)a.gate.p + (long long)(sq.lo + tok) * a.gate.ld + (long long)head * a.gate.hd + 4 * half : nullptr;
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float y[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) y[x] = o[i][4 * e + x] * inv;
-        if (gate) {
-          const u32x2 w = *(const u32x2*)(gate + 32 * i + 8 * e);
-          const float z[4] = {bf_lo(w[0]), bf_hi(w[0]), bf_lo(w[1]), bf_hi(w[1])};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) y[x] *= __builtin_amdgcn_rcpf(1.0f + __expf(-z[x]));
-        }
-        *(u32x2*)(to + 32 * i + 8 * e) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
-      }
-  } else {
-    // the groups' parts of a row, joined through LDS
-    float* jo = (float*)lds;                                   // [KW][ROWS][D + 4]
-    float* jm = jo + KW * S::ROWS * (D + 4);                   // [KW][ROWS] maxima, then sums
-    __syncthreads();
+  Run<16, D> run;
+  run.start();
+  bool poisoned = false;
+  int t = piece.t0 + kw;
+  if (t < piece.t1) {
+    u32x4 q[KS];
     {
-      float* to = jo + (kw * S::ROWS + 32 * rw + col) * (D + 4);
+      const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + rc - tok * G) * a.q.hd + 8 * g;
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) *(f32x4*)(to + 32 * i + 8 * e + 4 * half) = f32x4{o[i][4 * e], o[i][4 * e + 1], o[i][4 * e + 2], o[i][4 * e + 3]};
-      if (half == 0) { jm[kw * S::ROWS + 32 * rw + col] = m; jm[(KW + kw) * S::ROWS + 32 * rw + col] = l; }
+      for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 32 * s);
     }
-    __syncthreads();
-    for (int x = threadIdx.x; x < rows * (D / 8); x += S::THREADS) {
-      const int rr = x / (D / 8), d = 8 * (x % (D / 8));
-      float M = -INFINITY, L = 0.f, y[8] = {};
+    places(t);
+    ask_scales(0);
+    ask(false);
+    ask(true);
+    // this lane's reads: 8 channels of two keys; 4 (8) keys by 16 channels a group of 16 lanes
+    const int kread = col * S::RB + (S::I8 ? ((g >> 1) ^ S::place_k(col)) * 16 + 8 * (g & 1) : (g ^ S::place_k(col)) * 16);
+    const int vkey = S::I8 ? 4 * g + ((lane & 15) >> 1 & 3) + 16 * ((lane & 15) >> 3) : 4 * g + ((lane & 15) >> 2);
+    const int vread = vkey * S::RB + (S::I8 ? S::place_v(vkey) * 16 + 8 * (lane & 1) : (((lane & 3) >> 1) ^ S::place_v(vkey)) * 16 + 8 * (lane & 1));
+    for (int odd = 0; t < piece.t1; t += KW, odd ^= 1) {
+      const bool more = t + KW < piece.t1;
+      const float* sc = (const float*)(mine + 2 * S::UNIT + 256 * odd) + 4 * g;
+      if (more) places(t + KW);
+      wait_loads<S::LOADS>();                                  // K is here, V may be on its way
+      f32x4 s[2];
 #pragma unroll
-      for (int k = 0; k < KW; ++k) M = fmaxf(M, jm[k * S::ROWS + rr]);
+      for (int x = 0; x < 2; ++x) {
+        s[x] = f32x4(0.f);
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const float mk = jm[k * S::ROWS + rr], w = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mk - M) * c);
-        const float* z = jo + (k * S::ROWS + rr) * (D + 4) + d;
-        const float lk = jm[(KW + k) * S::ROWS + rr];
-        L += mk == -INFINITY ? lk : w * lk;                    // NaN scores: no maximum, a sum of NaN
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = mk == -INFINITY ? y[e] + z[e] : fmaf(w, z[e], y[e]);
+        for (int i = 0; i < KS; ++i) {
+          u32x4 k;
+          if constexpr (S::I8) {
+            const u32x2 w = *(const u32x2*)(mine + 16 * x * S::RB + (kread ^ (32 * i)));
+            const u32x2 y = codes(w[0]), z = codes(w[1]);
+            k = u32x4{y[0], y[1], z[0], z[1]};
+          } else {
+            k = lds_read16(mine + 16 * x * S::RB + (kread ^ (64 * i)));
+          }
+          s[x] = Rows<16>::mfma(k, q[i], s[x]);
+        }
       }
-      if (!whole) {
-        *(f32x4*)(part + rr * D + d) = f32x4{y[0], y[1], y[2], y[3]};
-        *(f32x4*)(part + rr * D + d + 4) = f32x4{y[4], y[5], y[6], y[7]};
-        if (d == 0) { part[S::ROWS * D + rr] = M; part[S::ROWS * (D + 1) + rr] = L; }
-        continue;
-      }
-      const float inv = L == 0.f ? 0.f : 1.f / L;
-      const int tk = (r0 + rr) / G, hd = hk * G + (r0 + rr - tk * G);
+      if constexpr (S::I8) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] *= inv;
-      if (a.gate.p) {
-        const u32x4 w = *(const u32x4*)((const bf16_t*)a.gate.p + (long long)(sq.lo + tk) * a.gate.ld + (long long)hd * a.gate.hd + d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] *= __builtin_amdgcn_rcpf(1.0f + __expf(-(e & 1 ? bf_hi(w[e >> 1]) : bf_lo(w[e >> 1]))));
+        for (int x = 0; x < 2; ++x) s[x] *= *(const f32x4*)(sc + 16 * x);
       }
-      *(u32x4*)((bf16_t*)a.out.p + (long long)(sq.lo + tk) * a.out.ld + (long long)hd * a.out.hd + d) =
-          u32x4{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3]), pk_bf16(y[4], y[5]), pk_bf16(y[6], y[7])};
+      if (more) {
+        wait_lds();
+        ask_scales(odd ^ 1);
+        ask(false);
+        wait_loads<S::LOADS + S::SC>();
+      } else {
+        wait_loads<0>();
+      }
+      const int k0 = 32 * t;
+      const bool masked = k0 + 31 > first || k0 < full;
+      const char* V = mine + S::UNIT;
+      soft_step<16, D, S::I8>(run, s, c, masked, from - k0 - 4 * g, pos - k0 - 4 * g, sc + 32,
+        [&](int, int i) {
+          if constexpr (S::I8) {
+            const u32x2 w = lds_read_tr8(V + (vread ^ (16 * i)));
+            const u32x2 y = codes(w[0]), z = codes(w[1]);
+            return u32x4{y[0], y[1], z[0], z[1]};
+          } else {
+            const u32x2 x = lds_read_tr(V + (vread ^ (32 * i))), y = lds_read_tr(V + 16 * S::RB + (vread ^ (32 * i)));
+            return u32x4{x[0], x[1], y[0], y[1]};
+          }
+        });
+      if (!S::I8 && masked) poisoned |= tile_not_finite<D>(V);
+      if (more) {
+        wait_lds();
+        ask(true);
+      }
     }
+    run.l = Rows<16>::sum_over(run.l);
+  }
+
+  // the waves' parts of a row, joined through LDS
+  float* jo = (float*)lds;                                     // [KW][ROWS][D + 4]
+  float* jm = jo + KW * S::ROWS * (D + 4);                     // [KW][ROWS] maxima, then sums
+  __syncthreads();
+  if (!poisoned) {
+    float* to = jo + (kw * S::ROWS + col) * (D + 4) + 4 * g;
+#pragma unroll
+    for (int i = 0; i < MB; ++i) *(f32x4*)(to + 16 * i) = run.o[i];
+    if (g == 0) { jm[kw * S::ROWS + col] = run.m; jm[(KW + kw) * S::ROWS + col] = run.l; }
+  } else {
+    rows_again<D>(a, pg, b, pl, n, hk, sq, r0, r0 + rows, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
+      constexpr int C = D / 64;
+#pragma unroll
+      for (int e = 0; e < C; ++e) jo[(kw * S::ROWS + r - r0) * (D + 4) + C * lane + e] = y[e];
+      if (lane == 0) { jm[kw * S::ROWS + r - r0] = m; jm[(KW + kw) * S::ROWS + r - r0] = l; }
+    });
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < rows * (D / 4); x += S::THREADS) {
+    const int rr = x / (D / 4), d = 4 * (x % (D / 4));
+    float M = -INFINITY, L = 0.f;
+    f32x4 y = f32x4(0.f);
+#pragma unroll
+    for (int k = 0; k < KW; ++k) M = fmaxf(M, jm[k * S::ROWS + rr]);
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const float mk = jm[k * S::ROWS + rr], w = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * c);
+      L = fmaf(w, jm[(KW + k) * S::ROWS + rr], L);             // a wave without a maximum: zeros, or NaN
+      y += w * *(const f32x4*)(jo + (k * S::ROWS + rr) * (D + 4) + d);
+    }
+    if (piece.pieces > 1) {
+      *(f32x4*)(part + rr * D + d) = y;
+      if (d == 0) { part[S::ROWS * D + rr] = M; part[S::ROWS * (D + 1) + rr] = L; }
+      continue;
+    }
+    const int tk = (r0 + rr) / G;
+    store4(a, sq.lo + tk, hk * G + (r0 + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
   }
 }
 
-// ---- A: sequences of few rows -------------------------------------------------------------------------------------------
 // workgroup (split, sequence, head)
 template <class S>
 __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
@@ -481,12 +477,201 @@ __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_page
   // more rows than a tile has, where no other launch takes them: one workgroup all of them, a tile after the other
   const int splits = sq.rows > S::ROWS ? 1 : pl.splits;
   for (int r0 = 0; r0 < sq.rows; r0 += S::ROWS) {
-    attend<S>(a, pg, b, pl, lds, n, hk, split, splits, r0, sq, pl.work + (long long)blockIdx.x * S::PART);
+    few_rows<S>(a, pg, b, pl, lds, n, hk, split, splits, r0, sq, pl.work + (long long)blockIdx.x * S::PART);
     __syncthreads();
   }
 }
 
-// ---- B: sequences of many rows -----------------------------------------------------------------------------------------
+// ---- many rows ------------------------------------------------------------------------------------------------------------
+// RW waves of 32 rows each share a tile of KT keys, K and V twice in LDS.  Codes go through registers and into LDS as bf16.
+template <int D_, int RW_, int KT_, int LEAST_, int EU_, bool I8_> struct Many {
+  static constexpr int D = D_, RW = RW_, EU = EU_, KT = KT_, LEAST = LEAST_, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
+  static constexpr bool I8 = I8_;
+  static constexpr int RB = 2 * D, TILE = KT * RB, STAGE = 2 * TILE;                 // bytes in LDS
+  static constexpr int SCALES = I8 ? 2 * 2 * KT * 4 : 0;
+  static constexpr int LDS = 2 * STAGE + SCALES;
+  static constexpr int PART = ROWS * (D + 2);
+  static constexpr int OWN = KT / RW;                          // keys of a tile that a wave loads, all of one page
+  static_assert(OWN == 8 || OWN == 16, "keys of one page");
+  static __device__ __forceinline__ int place_k(int key) { return key & 7; }
+  static __device__ __forceinline__ int place_v(int key) { return D == 64 ? (key & 3) << 1 : (key & 7) << 1; }
+};
+
+template <class S>
+__device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
+                                          int hk, int split, int r0, const Seq& sq, float* part) {
+  constexpr int D = S::D, KT = S::KT, KS = D / 16, MB = D / 32, OWN = S::OWN;
+  const int rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
+  const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
+  const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), pl.splits, split);
+  if (split >= piece.pieces) return;
+  const int row = r0 + 32 * rw + col, rc = min(row, r0 + rows - 1), tok = rc / G, pos = sq.pos0 + tok, head = hk * G + rc - tok * G;
+  const bool busy = 32 * rw < rows;                            // the wave has rows
+  const int first = sq.pos0 + min(r0 + 32 * rw, r0 + rows - 1) / G, last = sq.pos0 + (min(r0 + 32 * rw + 32, r0 + rows) - 1) / G;
+  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;               // keys from .. pos are seen
+  const int wave_from = a.window > 0 ? max(first - a.window + 1, 0) : 0;        // the wave sees keys wave_from .. last,
+  const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;              // all its rows full .. first
+  u32x4 q[KS];
+  {
+    const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)head * a.q.hd + 8 * g;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 16 * s);
+  }
+
+  // ---- tiles
+  const int* tab = b.table + (long long)n * b.table_ld;
+  const int tend = max(sq.len - 1, 0);
+  constexpr int ES = S::I8 ? 1 : 2, CPR = D * ES / 16, RPL = 64 / CPR, LOADS = OWN / RPL > 0 ? OWN / RPL : 1;
+  static_assert(S::I8 || OWN % RPL == 0, "a load of a whole wave");
+  const char* kbase = (const char*)pg.k + (long long)hk * pg.head_ld * ES;
+  const char* vbase = (const char*)pg.v + (long long)hk * pg.head_ld * ES;
+  const uint32_t row_bytes = (uint32_t)pg.row_ld * ES;
+  // places of this lane's chunks: their row, and where they come from so that they lie swizzled
+  const int lrow = lane / CPR;
+  u32x4 kreg[S::I8 ? LOADS : 1], vreg[S::I8 ? LOADS : 1];
+  float ksc = 0.f, vsc = 0.f;
+  auto page_at = [&](int t) {                                  // of this wave's keys of tile t
+    const int kg = min(t * KT + rw * OWN, tend & ~(OWN - 1)), pi = __builtin_amdgcn_readfirstlane(page_of(pl.div, kg));
+    return ((const_int*)tab)[pi];
+  };
+  auto ask = [&](int t, int page, int buf) {
+    const int kg = min(t * KT + rw * OWN, tend & ~(OWN - 1)), in = kg - __builtin_amdgcn_readfirstlane(page_of(pl.div, kg)) * pg.page;
+    page = page >= 0 && page < pg.NP ? page : 0;
+    const long long base = ((long long)page * pg.page_ld + (long long)in * pg.row_ld) * ES;
+    const int most = tend - kg;                                // the group's last cached token
+    const char *kp = kbase + base, *vp = vbase + base;
+    char* to = lds + buf * S::STAGE + rw * OWN * S::RB;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      if constexpr (!S::I8) {
+        const int key = RPL * j + lrow;
+        const uint32_t off = (uint32_t)min(key, most) * row_bytes;
+        load16(kp, off + 16 * ((lane % CPR) ^ S::place_k(key)), to + 1024 * j);
+        load16(vp, off + 16 * ((lane % CPR) ^ S::place_v(key)), to + S::TILE + 1024 * j);
+      } else {
+        const uint32_t off = (uint32_t)min(min(RPL * j + lrow, OWN - 1), most) * row_bytes + 16 * (lane % CPR);
+        kreg[j] = *(const u32x4*)(kp + off);
+        vreg[j] = *(const u32x4*)(vp + off);
+      }
+    }
+    if constexpr (S::I8) {
+      const long long x = (long long)page * pg.s_page_ld + (long long)(in + min(min(lane, OWN - 1), most)) * pg.s_row_ld + (long long)hk * pg.s_head_ld;
+      ksc = pg.k_scale[x];
+      vsc = pg.v_scale[x];
+    }
+  };
+  auto settle = [&](int buf) {                                 // codes in registers -> bf16 in LDS
+    if constexpr (S::I8) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int key = RPL * j + lrow, tk = rw * OWN + key, ch = 2 * (lane % CPR);
+        if (key < OWN) {
+          char* to = lds + buf * S::STAGE + tk * S::RB;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const u32x2 k0 = codes(kreg[j][2 * y]), k1 = codes(kreg[j][2 * y + 1]), v0 = codes(vreg[j][2 * y]), v1 = codes(vreg[j][2 * y + 1]);
+            *(u32x4*)(to + 16 * ((ch + y) ^ S::place_k(tk))) = u32x4{k0[0], k0[1], k1[0], k1[1]};
+            *(u32x4*)(to + S::TILE + 16 * ((ch + y) ^ S::place_v(tk))) = u32x4{v0[0], v0[1], v1[0], v1[1]};
+          }
+        }
+      }
+      float* sc = (float*)(lds + 2 * S::STAGE) + buf * 2 * KT + rw * OWN;
+      if (lane < OWN) { sc[lane] = ksc; sc[KT + lane] = vsc; }
+    }
+  };
+
+  const float c = a.scale * LOG2E;
+  Run<32, D> run;
+  run.start();
+  bool poisoned = false;
+  // this lane's reads: a row of K; 4 keys by 16 channels a group of 16 lanes of V
+  const int kread = col * S::RB + 16 * (g ^ S::place_k(col));
+  const int vkey = 4 * g + ((lane & 15) >> 2);
+  const int vread = vkey * S::RB + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ S::place_v(vkey)) + 8 * (lane & 1);
+  auto tile = [&](int t, int buf) {
+    if (!busy) return;
+#pragma unroll
+    for (int x = 0; x < KT / 32; ++x) {
+      const char* K = lds + buf * S::STAGE + 32 * x * S::RB;
+      const char* V = K + S::TILE;
+      const int k0 = t * KT + 32 * x;
+      if (k0 > last || k0 + 32 <= wave_from) continue;
+      f32x16 s[1] = {f32x16(0.f)};
+#pragma unroll
+      for (int i = 0; i < KS; ++i) s[0] = Rows<32>::mfma(lds_read16(K + (kread ^ (32 * i))), q[i], s[0]);
+      const float* sc = (const float*)(lds + 2 * S::STAGE) + buf * 2 * KT + 32 * x + 4 * g;
+      if constexpr (S::I8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 w = *(const f32x4*)(sc + 8 * i);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[0][4 * i + e] *= w[e];
+        }
+      }
+      const bool masked = k0 + 31 > first || k0 < full;
+      soft_step<32, D, S::I8>(run, s, c, masked, from - k0 - 4 * g, pos - k0 - 4 * g, sc + KT,
+        [&](int f, int i) {
+          const char* at = V + f * 16 * S::RB + (vread ^ (64 * i));
+          const u32x2 y = lds_read_tr(at), z = lds_read_tr(at + 8 * S::RB);
+          return u32x4{y[0], y[1], z[0], z[1]};
+        });
+      if (!S::I8 && masked) poisoned |= tile_not_finite<D>(V);
+    }
+  };
+  const int tiles = piece.t1 - piece.t0;
+  if (tiles > 0) {
+    ask(piece.t0, page_at(piece.t0), 0);
+    int page = page_at(piece.t0 + 1);
+    settle(0);
+    for (int i = 0; i < tiles; ++i) {
+      if constexpr (!S::I8) wait_loads<0>();
+      __syncthreads();
+      const int t = piece.t0 + i, buf = i & 1;
+      if (i + 1 < tiles) {
+        ask(t + 1, page, buf ^ 1);
+        page = page_at(t + 2);
+      }
+      tile(t, buf);
+      if (i + 1 < tiles) settle(buf ^ 1);
+    }
+  }
+  if (poisoned) {
+    rows_again<D>(a, pg, b, pl, n, hk, sq, r0 + 32 * rw, min(r0 + 32 * rw + 32, r0 + rows), piece.t0 * (KT / 32), piece.t1 * (KT / 32), 1,
+                  [&](int r, float m, float l, const float* y) {
+      constexpr int C = D / 64;
+      const int tk = r / G;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        const int d = C * lane + e;
+        if (piece.pieces > 1) part[(r - r0) * D + d] = y[e];
+        else store1(a, sq.lo + tk, hk * G + r - tk * G, d, y[e] * inv);
+      }
+      if (piece.pieces > 1 && lane == 0) { part[S::ROWS * D + r - r0] = m; part[S::ROWS * (D + 1) + r - r0] = l; }
+    });
+    return;
+  }
+  run.l = xor32_sum(run.l);
+  if (row >= r0 + rows) return;
+  if (piece.pieces > 1) {
+    float* to = part + (32 * rw + col) * D + 4 * g;
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *(f32x4*)(to + 32 * i + 8 * e) = f32x4{run.o[i][4 * e], run.o[i][4 * e + 1], run.o[i][4 * e + 2], run.o[i][4 * e + 3]};
+    if (g == 0) { part[S::ROWS * D + 32 * rw + col] = run.m; part[S::ROWS * (D + 1) + 32 * rw + col] = run.l; }
+    return;
+  }
+  const float inv = run.l == 0.f ? 0.f : 1.f / run.l;
+#pragma unroll
+  for (int i = 0; i < MB; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      store4(a, sq.lo + tok, head, 32 * i + 8 * e + 4 * g, f32x4{run.o[i][4 * e], run.o[i][4 * e + 1], run.o[i][4 * e + 2], run.o[i][4 * e + 3]} * inv);
+      __builtin_amdgcn_sched_barrier(0);                       // not all gates at once: their registers
+    }
+}
+
 // Row tiles are numbered without a scan over the batch: tile j of sequence n has the number loc[n] G / ROWS + n + j; numbers
 // left over find a tile past the end.
 struct RowTile { int n, r0; };
@@ -510,7 +695,7 @@ template <int ROWS> __device__ __forceinline__ RowTile row_tile(const lq_batch& 
 // Workgroups go to the XCDs in turn: a head of the cache stays on one of them (or on 8 / HK), whose L2 then holds its tiles.
 // The last row tiles, which see the most keys, come first.
 template <class S>
-__global__ __launch_bounds__(S::THREADS) void many_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl, int tiles) {
+__global__ __launch_bounds__(S::THREADS) __attribute__((amdgpu_waves_per_eu(S::EU, S::EU))) void many_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl, int tiles) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int per = tiles * pg.HK, split = blockIdx.x / per, x = blockIdx.x % per;
   int hk, number;
@@ -522,64 +707,89 @@ __global__ __launch_bounds__(S::THREADS) void many_kernel(lq_attention a, lq_pag
     hk = x % pg.HK;
     number = x / pg.HK;
   }
-  const RowTile rt = row_tile<S::ROWS>(b, pl.G, tiles - 1 - number);
+  number = tiles - 1 - number;
+  const RowTile rt = row_tile<S::ROWS>(b, pl.G, number);
   const Seq sq = sequence(b, pg, pl.G, rt.n);
   if (rt.r0 >= sq.rows || sq.rows <= pl.few) return;
-  attend<S>(a, pg, b, pl, lds, rt.n, hk, split, pl.splits, rt.r0, sq,
-            pl.work + ((long long)split * per + (long long)(tiles - 1 - number) * pg.HK + hk) * S::PART);
+  many_rows<S>(a, pg, b, pl, lds, rt.n, hk, split, rt.r0, sq, pl.work + ((long long)split * per + (long long)number * pg.HK + hk) * S::PART);
 }
 
 // ---- the pieces of split keys, joined -----------------------------------------------------------------------------------
-// A workgroup for each row tile and head; a thread for 4 channels of a row.
-template <class S, bool FEW>
+// A row's D / 4 threads take 4 channels each; P of them share out the pieces of a row.
+template <class S, bool FEW, int P>
 __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl, int tiles) {
-  constexpr int D = S::D, ROWS = S::ROWS;
-  const int item = blockIdx.x, hk = item % pg.HK, number = item / pg.HK;
+  constexpr int D = S::D, ROWS = S::ROWS, C = D / 4, PER = 256 / (C * P);      // rows of a workgroup
+  static_assert(PER >= 1 && ROWS % PER == 0, "rows of a workgroup");
+  __shared__ float lds[P > 1 ? 256 * 4 + 2 * P * PER : 1];
+  const int item = blockIdx.x / (ROWS / PER), rr = (blockIdx.x % (ROWS / PER)) * PER + threadIdx.x / (C * P);
+  const int hk = item % pg.HK, number = item / pg.HK;
   RowTile rt = {number, 0};
   if (!FEW) rt = row_tile<ROWS>(b, pl.G, number);
   const Seq sq = sequence(b, pg, pl.G, rt.n);
   if (FEW ? sq.rows <= 0 || sq.rows > ROWS : rt.r0 >= sq.rows || sq.rows <= pl.few) return;
   const int rows = min(ROWS, sq.rows - rt.r0);
-  const Piece piece = piece_of<S::KT, S::LEAST>(keys_of(sq, pl.G, rt.r0, rt.r0 + rows, a.window), pl.splits, 0);
+  if ((blockIdx.x % (ROWS / PER)) * PER >= rows) return;
+  const Piece piece = piece_of<S>(keys_of(sq, pl.G, rt.r0, rt.r0 + rows, a.window), pl.splits, 0);
   if (piece.pieces == 1) return;
+  const int which = (threadIdx.x / C) % P, d = 4 * (threadIdx.x % C);
   const long long step = (long long)tiles * pg.HK * S::PART;
   const float* part = pl.work + (long long)item * S::PART;
   const float c = a.scale * LOG2E;
-  for (int x = blockIdx.y * 256 + threadIdx.x; x < rows * (D / 4); x += 256 * gridDim.y) {
-    const int rr = x / (D / 4), d = 4 * (x % (D / 4));
-    float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < piece.pieces; ++k) M = fmaxf(M, part[k * step + ROWS * D + rr]);
-    f32x4 y = f32x4(0.f);
-    for (int k = 0; k < piece.pieces; ++k) {
-      const float* p = part + k * step;
-      const float mk = p[ROWS * D + rr], w = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * c);
-      L = fmaf(w, p[ROWS * (D + 1) + rr], L);                  // a piece without a maximum: zeros, or NaN
-      y += w * *(const f32x4*)(p + rr * D + d);
-    }
-    y *= L == 0.f ? 0.f : 1.f / L;
-    const int tk = (rt.r0 + rr) / pl.G, hd = hk * pl.G + (rt.r0 + rr - tk * pl.G);
-    if (a.gate.p) {
-      const u32x2 w = *(const u32x2*)((const bf16_t*)a.gate.p + (long long)(sq.lo + tk) * a.gate.ld + (long long)hd * a.gate.hd + d);
+  float M = -INFINITY, L = 0.f;
+  f32x4 y = f32x4(0.f);
+  constexpr int U = 8;                                         // pieces on their way at once
+  for (int k0 = which; k0 < piece.pieces; k0 += U * P) {
+    float mk[U], lk[U];
+    f32x4 yk[U];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] *= __builtin_amdgcn_rcpf(1.0f + __expf(-(e & 1 ? bf_hi(w[e >> 1]) : bf_lo(w[e >> 1]))));
+    for (int u = 0; u < U; ++u) {
+      const float* p = part + min(k0 + u * P, piece.pieces - 1) * step;
+      mk[u] = p[ROWS * D + rr];
+      lk[u] = p[ROWS * (D + 1) + rr];
+      yk[u] = *(const f32x4*)(p + rr * D + d);
     }
-    *(u32x2*)((bf16_t*)a.out.p + (long long)(sq.lo + tk) * a.out.ld + (long long)hd * a.out.hd + d) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+    float to = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u * P < piece.pieces) to = fmaxf(to, mk[u]);
+    const float w = M == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((M - to) * c);
+    L *= w;
+    y *= w;
+    M = to;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u * P < piece.pieces) {
+        const float w = mk[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk[u] - M) * c);    // none: zeros, or NaN
+        L = fmaf(w, lk[u], L);
+        y += w * yk[u];
+      }
   }
+  if constexpr (P > 1) {
+    float* jm = lds + 256 * 4;                                 // [PER][P] maxima, then sums
+    *(f32x4*)(lds + 4 * threadIdx.x) = y;
+    if (d == 0) { jm[threadIdx.x / C] = M; jm[PER * P + threadIdx.x / C] = L; }
+    __syncthreads();
+    if (which > 0) return;
+    const int at = threadIdx.x / C;
+    M = -INFINITY; L = 0.f; y = f32x4(0.f);
+#pragma unroll
+    for (int k = 0; k < P; ++k) M = fmaxf(M, jm[at + k]);
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      const float w = jm[at + k] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((jm[at + k] - M) * c);
+      L = fmaf(w, jm[PER * P + at + k], L);
+      y += w * *(const f32x4*)(lds + 4 * (threadIdx.x + C * k));
+    }
+  }
+  if (rr >= rows) return;
+  const int tk = (rt.r0 + rr) / pl.G;
+  store4(a, sq.lo + tk, hk * pl.G + (rt.r0 + rr - tk * pl.G), d, y * (L == 0.f ? 0.f : 1.f / L));
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
-template <int D, bool I8> struct Shapes;
-template <bool I8> struct Shapes<64, I8> {
-  typedef Shape<64, 1, 4, 32, 8, I8> Few;
-  typedef Shape<64, 4, 1, 64, 8, I8> Many;
-};
-template <bool I8> struct Shapes<128, I8> {
-  typedef Shape<128, 1, 4, 32, 8, I8> Few;
-  typedef Shape<128, 4, 1, 64, 8, I8> Many;
-};
-template <bool I8> struct Shapes<256, I8> {
-  typedef Shape<256, 1, 2, 32, 8, I8> Few;
-  typedef Shape<256, 4, 1, 32, 16, I8> Many;
+template <int D, bool I8> struct Shapes {
+  typedef Few<D, 4, I8> F;
+  typedef Many<D, 4, D == 256 ? 32 : 64, 8, D == 256 ? 1 : 2, I8> M;
 };
 
 // LDS beyond what a kernel has unasked: asked for once on each device, and again where that failed.
@@ -604,8 +814,8 @@ struct Calls {
   long long few_work, many_work;     // floats
 };
 template <int D, bool I8> Calls calls(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest) {
-  typedef typename Shapes<D, I8>::Few F;
-  typedef typename Shapes<D, I8>::Many M;
+  typedef typename Shapes<D, I8>::F F;
+  typedef typename Shapes<D, I8>::M M;
   const long long G = a->HQ / p->HK, cus = lq_attn_cus();
   const long long most = longest > 0 && longest < b->T ? longest : b->T;
   Calls c = {};
@@ -625,10 +835,18 @@ template <int D, bool I8> Calls calls(const lq_attention* a, const lq_pages* p, 
   return c;
 }
 
+// four groups of threads a row where there are pieces enough for them
+template <class S, bool FEW> void join(const lq_attention* a, const lq_pages* p, const lq_batch* b, const Plan& pl, int tiles, hipStream_t s) {
+  const unsigned items = (unsigned)(tiles * p->HK);
+  constexpr int per = 256 / (S::D / 4);
+  if (pl.splits > 8) join_kernel<S, FEW, 4><<<items * (S::ROWS / (per / 4)), 256, 0, s>>>(*a, *p, *b, pl, tiles);
+  else join_kernel<S, FEW, 1><<<items * (S::ROWS / per), 256, 0, s>>>(*a, *p, *b, pl, tiles);
+}
+
 template <int D, bool I8>
 int go(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest, float* work, hipStream_t s) {
-  typedef typename Shapes<D, I8>::Few F;
-  typedef typename Shapes<D, I8>::Many M;
+  typedef typename Shapes<D, I8>::F F;
+  typedef typename Shapes<D, I8>::M M;
   const Calls c = calls<D, I8>(a, p, b, longest);
   Plan pl = {};
   pl.G = a->HQ / p->HK;
@@ -642,7 +860,7 @@ int go(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest,
     few_kernel<F><<<(unsigned)(fi * c.few_splits), F::THREADS, F::LDS, s>>>(*a, *p, *b, pl);
     if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
     if (c.few_splits > 1) {
-      join_kernel<F, true><<<(unsigned)fi, 256, 0, s>>>(*a, *p, *b, pl, b->N);
+      join<F, true>(a, p, b, pl, b->N, s);
       if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
     }
   }
@@ -654,7 +872,7 @@ int go(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest,
     many_kernel<M><<<(unsigned)(mi * c.many_splits), M::THREADS, M::LDS, s>>>(*a, *p, *b, pl, c.tiles);
     if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
     if (c.many_splits > 1) {
-      join_kernel<M, false><<<dim3((unsigned)mi, 4), 256, 0, s>>>(*a, *p, *b, pl, c.tiles);
+      join<M, false>(a, p, b, pl, c.tiles, s);
       if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
     }
   }
