@@ -293,11 +293,12 @@ template <int D_, int KW_, bool I8_> struct Few {
   static constexpr int JOIN = KW * ROWS * ((D + 4) * 4 + 8);
   static constexpr int LDS = KW * WAVE > JOIN ? KW * WAVE : JOIN;
   static constexpr int PART = ROWS * (D + 2);                  // floats of a workgroup's part of split keys
-  // a chunk's place in its row: spread so that the reads below go over all banks
-  static __device__ __forceinline__ int place_k(int key) { return CPR >= 8 ? key & 7 : (key >> 1) & 3; }
+  // A chunk's place in its row, so that 256 bytes of the reads below go over all banks: 16 keys by a chunk of K; 8 keys by two chunks
+  // of V, or, codes, 16 keys (of which 8 neighbours and those 16 on) by one.
+  static constexpr int SPAN = CPR >= 16 ? 1 : 16 / CPR;        // rows of 256 bytes
+  static __device__ __forceinline__ int place_k(int key) { return key / SPAN & (16 / SPAN - 1); }
   static __device__ __forceinline__ int place_v(int key) {
-    if (I8) return (key & 3) | (CPR >= 8 ? (key >> 2) & 4 : 0);
-    return CPR >= 16 ? (key & 7) << 1 : (key & 3) << 1;
+    return I8 ? ((key & 7) | (key >> 4 & 1) << 3) / SPAN : ((key & 7) / SPAN) << 1;
   }
 };
 
@@ -493,8 +494,10 @@ template <int D_, int RW_, int KT_, int LEAST_, int EU_, bool I8_> struct Many {
   static constexpr int PART = ROWS * (D + 2);
   static constexpr int OWN = KT / RW;                          // keys of a tile that a wave loads, all of one page
   static_assert(OWN == 8 || OWN == 16, "keys of one page");
-  static __device__ __forceinline__ int place_k(int key) { return key & 7; }
-  static __device__ __forceinline__ int place_v(int key) { return D == 64 ? (key & 3) << 1 : (key & 7) << 1; }
+  // as Few's: 16 keys by a chunk of K, 4 keys by four chunks of V
+  static constexpr int SPAN = D == 64 ? 2 : 1;
+  static __device__ __forceinline__ int place_k(int key) { return key / SPAN & (16 / SPAN - 1); }
+  static __device__ __forceinline__ int place_v(int key) { return (key & 3) / SPAN << 2; }
 };
 
 template <class S>
@@ -546,8 +549,8 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       if constexpr (!S::I8) {
         const int key = RPL * j + lrow;
         const uint32_t off = (uint32_t)min(key, most) * row_bytes;
-        load16(kp, off + 16 * ((lane % CPR) ^ S::place_k(key)), to + 1024 * j);
-        load16(vp, off + 16 * ((lane % CPR) ^ S::place_v(key)), to + S::TILE + 1024 * j);
+        load16(kp, off + 16 * ((lane % CPR) ^ S::place_k(rw * OWN + key)), to + 1024 * j);
+        load16(vp, off + 16 * ((lane % CPR) ^ S::place_v(rw * OWN + key)), to + S::TILE + 1024 * j);
       } else {
         const uint32_t off = (uint32_t)min(min(RPL * j + lrow, OWN - 1), most) * row_bytes + 16 * (lane % CPR);
         kreg[j] = *(const u32x4*)(kp + off);
