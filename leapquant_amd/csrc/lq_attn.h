@@ -29,7 +29,7 @@ static inline bool pages_ok(const lq_pages* p) {
   if (p->page_ld < 0 || p->row_ld < 0 || p->head_ld < 0) return false;
   if (p->page_ld % unit || p->row_ld % unit || p->head_ld % unit) return false;
   const long long far = 1ll << 29;                 // 32-bit byte offsets within a page
-  if (p->row_ld >= far || p->head_ld >= far) return false;
+  if (p->row_ld >= far || p->head_ld >= far || p->page_ld >= 1ll << 31) return false;
   if ((p->page - 1) * p->row_ld + (p->HK - 1) * p->head_ld + p->D > far) return false;
   if (p->int8) {
     if (!p->k_scale || !p->v_scale || p->s_page_ld < 0 || p->s_row_ld < 0 || p->s_head_ld < 0) return false;

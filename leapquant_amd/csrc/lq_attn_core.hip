@@ -36,6 +36,8 @@ struct Plan {
 constexpr float GROWN = 8.f;
 constexpr float LOG2E = 1.44269504f;
 
+// a value where it is computed: not moved to its use
+template <typename T> __device__ __forceinline__ void stay(T& x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ u32x4 lds_read16(const char* p) { return *(const u32x4*)p; }
 __device__ __forceinline__ u32x2 lds_read_tr(const char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_t*)p));
@@ -49,6 +51,20 @@ __device__ __forceinline__ u32x2 lds_read_tr8(const char* p) {
 __device__ __forceinline__ void load16(const char* base, uint32_t off, const char* lds) {
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(to) : "memory", "m0");
+}
+// N of them, the j-th with an immediate of 1024 j bytes on both its address and its place
+template <int N> __device__ __forceinline__ void load16s(const char* base, const uint32_t (&off)[N], const char* lds) {
+  static_assert(N == 1 || N == 2 || N == 4, "loads of a wave");
+  const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
+  if constexpr (N == 1)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0" :: "s"(base), "s"(to), "v"(off[0]) : "memory", "m0");
+  else if constexpr (N == 2)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024"
+                 :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
+                 "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:3072"
+                 :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "m0");
 }
 __device__ __forceinline__ void load4(const float* from, const char* lds) {
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
@@ -123,86 +139,89 @@ template <> struct Rows<16> {
   static __device__ __forceinline__ float sum_over(float x) { return xor32_sum(xor16_sum(x)); }
 };
 
-// What a wave carries along its keys: outputs O^T, a row's running maximum (of q . k, not scaled) and sum.
+// What a wave carries along its keys: outputs O^T, a row's running maximum m (of q . k, not scaled) and sum l.
 template <int R, int D> struct Run {
   typedef Rows<R> W;
-  static constexpr int MB = D / W::DM;
+  static constexpr int MB = D / W::DM, E = W::E, AN = W::AN;
   typename W::acc o[MB];
-  float m, l;
+  float m, l, ref;
+  bool huge;
   __device__ __forceinline__ void start() {
     m = -INFINITY;
-    l = 0.f;
+    l = ref = 0.f;
+    huge = false;
 #pragma unroll
     for (int i = 0; i < MB; ++i) o[i] = typename W::acc(0.f);
   }
-};
-
-// Softmax and second product of 32 keys' scores s.  Keys of lo .. hi (places in the 32, less 4 g) are seen where `masked`.
-// vscale: scales of the values, by places as s, or nothing.  value(f, i): the f-th operand of values for the channels of o[i].
-template <int R, int D, bool I8, class V>
-__device__ __forceinline__ void soft_step(Run<R, D>& run, typename Rows<R>::acc (&s)[Rows<R>::A], float c, bool masked, int lo, int hi,
-                                          const float* vscale, const V& value) {
-  typedef Rows<R> W;
-  constexpr int E = W::E, AN = W::AN, MB = Run<R, D>::MB;
-  if (masked) {
+  // the largest of 32 keys' scores
+  static __device__ __forceinline__ float largest(const typename W::acc (&s)[W::A]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) mx = fmaxf(mx, s[i / AN][i % AN]);
+    return mx;
+  }
+  // m follows scores whose largest is mx, by steps of 2^GROWN or more
+  __device__ __forceinline__ void follow(typename W::acc (&s)[W::A], float mx, float c) {
+    mx = W::max_over(mx);
+    if (__any((mx - m) * c > GROWN)) {
+      const float to = fmaxf(m, mx), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
+      m = to;
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        o[i] *= alpha;
+        __builtin_amdgcn_sched_barrier(0);                     // few at a time outside the accumulators' registers
+      }
+      // s c - ref is rounded once, but ref = m c itself is off by half its last place, which 2^ref would be too much for beyond 2^24
+      huge = __any(fabsf(m * c) > 0x1p24f && m != -INFINITY);
+      ref = huge || m == -INFINITY ? 0.f : m * c;
+    }
+    if (huge) {
+      const float raw = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int i = 0; i < E; ++i) s[i / AN][i % AN] -= raw;
+    }
+  }
+  // scores into weights, their sum into l
+  __device__ __forceinline__ void weigh(typename W::acc (&s)[W::A], float c) {
+    float part[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      s[i / AN][i % AN] = __builtin_amdgcn_exp2f(fmaf(s[i / AN][i % AN], c, -ref));
+      part[i & 1] += s[i / AN][i % AN];
+    }
+    l += part[0] + part[1];
+  }
+  // weights as operands of the second product
+  static __device__ __forceinline__ void pack(const typename W::acc (&s)[W::A], u32x4 (&p)[W::F]) {
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) p[i >> 2][i & 3] = pk_bf16(s[2 * i / AN][2 * i % AN], s[2 * i / AN][2 * i % AN + 1]);
+  }
+  // Keys at places lo .. hi of the 32 (less 4 g) are seen, the others' scores or weights become `none`.
+  static __device__ __forceinline__ void mask(typename W::acc (&s)[W::A], int lo, int hi, float none) {
+    asm volatile("" : "+v"(lo), "+v"(hi));                     // a branch of its own, not selects for every tile
 #pragma unroll
     for (int i = 0; i < E; ++i) {
       const int j = W::STEP * (i >> 2) + (i & 3);
-      s[i / AN][i % AN] = j >= lo && j <= hi ? s[i / AN][i % AN] : -INFINITY;
+      s[i / AN][i % AN] = j >= lo && j <= hi ? s[i / AN][i % AN] : none;
     }
   }
-  float mx = s[0][0];
-#pragma unroll
-  for (int i = 1; i < E; ++i) mx = fmaxf(mx, s[i / AN][i % AN]);
-  mx = W::max_over(mx);
-  if (__any((mx - run.m) * c > GROWN)) {
-    const float to = fmaxf(run.m, mx), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((run.m - to) * c);
-    run.m = to;
-    run.l *= alpha;
-#pragma unroll
-    for (int i = 0; i < MB; ++i) run.o[i] *= alpha;
-  }
-  const float raw = run.m == -INFINITY ? 0.f : run.m, ref = raw * c;
-  // s c - ref is rounded once, but ref itself is off by half its last place, which 2^ref would be too much for beyond 2^24
-  if (__any(fabsf(ref) > 0x1p24f)) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) s[i / AN][i % AN] = (s[i / AN][i % AN] - raw) * c;
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) s[i / AN][i % AN] = fmaf(s[i / AN][i % AN], c, -ref);
-  }
-  float part[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    s[i / AN][i % AN] = __builtin_amdgcn_exp2f(s[i / AN][i % AN]);
-    part[i & 1] += s[i / AN][i % AN];
-  }
-  run.l += part[0] + part[1];
-  if constexpr (I8) {
+  // times the scales of the keys or values, by places less 4 g
+  static __device__ __forceinline__ void times(typename W::acc (&s)[W::A], const float* scale) {
 #pragma unroll
     for (int i = 0; i < E; i += 4) {
-      const f32x4 x = *(const f32x4*)(vscale + W::STEP * (i >> 2));
+      const f32x4 x = *(const f32x4*)(scale + W::STEP * (i >> 2));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int j = W::STEP * (i >> 2) + e;
-        const float y = s[i / AN][i % AN + e] * x[e];
-        s[i / AN][i % AN + e] = !masked || (j >= lo && j <= hi) ? y : 0.f;     // a scale that is not finite, not seen
-      }
+      for (int e = 0; e < 4; ++e) s[i / AN][i % AN + e] *= x[e];
     }
   }
-  u32x4 p[W::F];
-#pragma unroll
-  for (int i = 0; i < E / 2; ++i) p[i >> 2][i & 3] = pk_bf16(s[2 * i / AN][2 * i % AN], s[2 * i / AN][2 * i % AN + 1]);
-#pragma unroll
-  for (int f = 0; f < W::F; ++f)
-#pragma unroll
-    for (int i = 0; i < MB; ++i) run.o[i] = W::mfma(value(f, i), p[f], run.o[i]);
-}
+};
+
 // whether 32 rows of D bf16 in LDS hold an infinity or NaN
 template <int D> __device__ __forceinline__ bool tile_not_finite(const char* tile) {
   const int lane = threadIdx.x & 63;
   uint32_t hit = 0;
-#pragma unroll 4
+#pragma unroll 2
   for (int i = 0; i < D / 16; ++i) {
     const u32x4 w = lds_read16(tile + (lane & 31) * 2 * D + 16 * ((lane >> 5) + 2 * i));
 #pragma unroll
@@ -227,6 +246,7 @@ __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages
     const int tok = r / pl.G, pos = sq.pos0 + tok, from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
     const bf16_t* q = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * pl.G + r - tok * pl.G) * a.q.hd;
     float m = -INFINITY, l = 0.f, y[C] = {};
+#pragma unroll 1
     for (int u = u0; u < u1; u += step) {
       if (32 * u > pos || 32 * u + 31 < from) continue;
       const int key = 32 * u + (lane & 31), kk = min(key, tend), pi = page_of(pl.div, kk);
@@ -235,6 +255,7 @@ __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages
       page = page >= 0 && page < pg.NP ? page : 0;
       const long long at = (long long)page * pg.page_ld + (long long)(kk - pi * pg.page) * pg.row_ld + (long long)hk * pg.head_ld;
       float s = 0.f;
+#pragma unroll 1
       for (int i = 0; i < D; i += 8) {
         const u32x4 x = *(const u32x4*)(q + i), k = *(const u32x4*)((const bf16_t*)pg.k + at + i);
 #pragma unroll
@@ -248,6 +269,7 @@ __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages
       l = fmaf(l, alpha, sum64(p));
 #pragma unroll
       for (int e = 0; e < C; ++e) y[e] *= alpha;
+#pragma unroll 1
       for (int j = 0; j < 32; ++j) {
         if (32 * u + j < from || 32 * u + j > pos) continue;
         const float pj = __shfl(p, j);
@@ -393,32 +415,39 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           s[x] = Rows<16>::mfma(k, q[i], s[x]);
         }
       }
-      if constexpr (S::I8) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) s[x] *= *(const f32x4*)(sc + 16 * x);
-      }
+      if constexpr (S::I8) run.times(s, sc);
       if (more) {
         wait_lds();
         ask_scales(odd ^ 1);
         ask(false);
-        wait_loads<S::LOADS + S::SC>();
-      } else {
-        wait_loads<0>();
       }
-      const int k0 = 32 * t;
+      const int k0 = 32 * t, lo = from - k0 - 4 * g, hi = pos - k0 - 4 * g;
       const bool masked = k0 + 31 > first || k0 < full;
+      if (masked) run.mask(s, lo, hi, -INFINITY);
+      run.follow(s, run.largest(s), c);
+      run.weigh(s, c);
+      if constexpr (S::I8) {
+        run.times(s, sc + 32);
+        if (masked) run.mask(s, lo, hi, 0.f);                  // a scale that is not finite, not seen
+      }
+      u32x4 p[1];
+      run.pack(s, p);
+      if (more) wait_loads<S::LOADS + S::SC>();                // V is here
+      else wait_loads<0>();
       const char* V = mine + S::UNIT;
-      soft_step<16, D, S::I8>(run, s, c, masked, from - k0 - 4 * g, pos - k0 - 4 * g, sc + 32,
-        [&](int, int i) {
-          if constexpr (S::I8) {
-            const u32x2 w = lds_read_tr8(V + (vread ^ (16 * i)));
-            const u32x2 y = codes(w[0]), z = codes(w[1]);
-            return u32x4{y[0], y[1], z[0], z[1]};
-          } else {
-            const u32x2 x = lds_read_tr(V + (vread ^ (32 * i))), y = lds_read_tr(V + 16 * S::RB + (vread ^ (32 * i)));
-            return u32x4{x[0], x[1], y[0], y[1]};
-          }
-        });
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        u32x4 v;
+        if constexpr (S::I8) {
+          const u32x2 w = lds_read_tr8(V + (vread ^ (16 * i)));
+          const u32x2 y = codes(w[0]), z = codes(w[1]);
+          v = u32x4{y[0], y[1], z[0], z[1]};
+        } else {
+          const u32x2 x = lds_read_tr(V + (vread ^ (32 * i))), y = lds_read_tr(V + 16 * S::RB + (vread ^ (32 * i)));
+          v = u32x4{x[0], x[1], y[0], y[1]};
+        }
+        run.o[i] = Rows<16>::mfma(v, p[0], run.o[i]);
+      }
       if (!S::I8 && masked) poisoned |= tile_not_finite<D>(V);
       if (more) {
         wait_lds();
@@ -484,16 +513,16 @@ __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_page
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------
-// RW waves of 32 rows each share a tile of KT keys, K and V twice in LDS.  Codes go through registers and into LDS as bf16.
-template <int D_, int RW_, int KT_, int LEAST_, int EU_, bool I8_> struct Many {
-  static constexpr int D = D_, RW = RW_, EU = EU_, KT = KT_, LEAST = LEAST_, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
+// RW waves of 32 rows each share tiles of 32 keys.  A wave forms the scores of a tile while it takes the exponentials of the one before,
+// and looks for their maximum while that one meets its values: matrix and vector instructions of a wave overlap.  K is so a tile
+// ahead of V, and two tiles of each lie in LDS.  Codes go through registers and into LDS as bf16.
+template <int D_, int RW_, int LEAST_, int EU_, bool I8_> struct Many {
+  static constexpr int D = D_, RW = RW_, EU = EU_, KT = 32, LEAST = LEAST_, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
   static constexpr bool I8 = I8_;
-  static constexpr int RB = 2 * D, TILE = KT * RB, STAGE = 2 * TILE;                 // bytes in LDS
-  static constexpr int SCALES = I8 ? 2 * 2 * KT * 4 : 0;
-  static constexpr int LDS = 2 * STAGE + SCALES;
+  static constexpr int RB = 2 * D, TILE = KT * RB;             // bytes in LDS
+  static constexpr int K0 = 0, V0 = 2 * TILE, SCALES = 4 * TILE, LDS = SCALES + (I8 ? 4 * KT * 4 : 0);
   static constexpr int PART = ROWS * (D + 2);
   static constexpr int OWN = KT / RW;                          // keys of a tile that a wave loads, all of one page
-  static_assert(OWN == 8 || OWN == 16, "keys of one page");
   // as Few's: 16 keys by a chunk of K, 4 keys by four chunks of V
   static constexpr int SPAN = D == 64 ? 2 : 1;
   static __device__ __forceinline__ int place_k(int key) { return key / SPAN & (16 / SPAN - 1); }
@@ -503,7 +532,7 @@ template <int D_, int RW_, int KT_, int LEAST_, int EU_, bool I8_> struct Many {
 template <class S>
 __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
                                           int hk, int split, int r0, const Seq& sq, float* part) {
-  constexpr int D = S::D, KT = S::KT, KS = D / 16, MB = D / 32, OWN = S::OWN;
+  constexpr int D = S::D, KS = D / 16, MB = D / 32, OWN = S::OWN;
   const int rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
   const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), pl.splits, split);
@@ -512,8 +541,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   const bool busy = 32 * rw < rows;                            // the wave has rows
   const int first = sq.pos0 + min(r0 + 32 * rw, r0 + rows - 1) / G, last = sq.pos0 + (min(r0 + 32 * rw + 32, r0 + rows) - 1) / G;
   const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;               // keys from .. pos are seen
-  const int wave_from = a.window > 0 ? max(first - a.window + 1, 0) : 0;        // the wave sees keys wave_from .. last,
-  const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;              // all its rows full .. first
+  const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;              // all rows of the wave see full .. first
   u32x4 q[KS];
   {
     const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)head * a.q.hd + 8 * g;
@@ -521,65 +549,97 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
     for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 16 * s);
   }
 
-  // ---- tiles
-  const int* tab = b.table + (long long)n * b.table_ld;
+  // ---- tiles: this wave's keys of each
+  const_int* tab = (const_int*)(b.table + (long long)n * b.table_ld);
   const int tend = max(sq.len - 1, 0);
   constexpr int ES = S::I8 ? 1 : 2, CPR = D * ES / 16, RPL = 64 / CPR, LOADS = OWN / RPL > 0 ? OWN / RPL : 1;
   static_assert(S::I8 || OWN % RPL == 0, "a load of a whole wave");
-  const char* kbase = (const char*)pg.k + (long long)hk * pg.head_ld * ES;
-  const char* vbase = (const char*)pg.v + (long long)hk * pg.head_ld * ES;
-  const uint32_t row_bytes = (uint32_t)pg.row_ld * ES;
-  // places of this lane's chunks: their row, and where they come from so that they lie swizzled
+  // The j-th load's immediate, 1024 j, moves its place in LDS and its address: the offsets below are that much less, and the
+  // bases 4096 less.
+  constexpr int AHEAD_OF = S::I8 ? 0 : 4096;
+  const char* kbase = (const char*)pg.k + (long long)hk * pg.head_ld * ES - AHEAD_OF;
+  const long long vfar = (const char*)pg.v - (const char*)pg.k;
+  const uint32_t row_bytes = (uint32_t)pg.row_ld * ES, page_bytes = (uint32_t)pg.page_ld * ES;
   const int lrow = lane / CPR;
+  uint32_t koff[LOADS], voff[LOADS];                           // where this lane's chunks come from, so that they lie swizzled
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int key = min(RPL * j + lrow, OWN - 1), tk = rw * OWN + key;
+    const uint32_t off = (uint32_t)key * row_bytes + AHEAD_OF - (S::I8 ? 0 : 1024 * j);
+    koff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_k(tk));
+    voff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_v(tk));
+  }
   u32x4 kreg[S::I8 ? LOADS : 1], vreg[S::I8 ? LOADS : 1];
   float ksc = 0.f, vsc = 0.f;
-  auto page_at = [&](int t) {                                  // of this wave's keys of tile t
-    const int kg = min(t * KT + rw * OWN, tend & ~(OWN - 1)), pi = __builtin_amdgcn_readfirstlane(page_of(pl.div, kg));
-    return ((const_int*)tab)[pi];
+  // the keys to ask for next: of tile at / 32, in `page` of the table's row at place `in`; a tile on by steps
+  const int key0 = piece.t0 * 32 + rw * OWN, end = tend & ~(OWN - 1), whole = 32 / pg.page, rest = 32 - whole * pg.page;
+  struct Place { int key, entry, in; };
+  auto place_of = [&](int key) {
+    Place p;
+    p.key = min(key, end);
+    p.entry = __builtin_amdgcn_readfirstlane(page_of(pl.div, p.key));
+    p.in = p.key - p.entry * pg.page;
+    return p;
   };
-  auto ask = [&](int t, int page, int buf) {
-    const int kg = min(t * KT + rw * OWN, tend & ~(OWN - 1)), in = kg - __builtin_amdgcn_readfirstlane(page_of(pl.div, kg)) * pg.page;
-    page = page >= 0 && page < pg.NP ? page : 0;
-    const long long base = ((long long)page * pg.page_ld + (long long)in * pg.row_ld) * ES;
-    const int most = tend - kg;                                // the group's last cached token
-    const char *kp = kbase + base, *vp = vbase + base;
-    char* to = lds + buf * S::STAGE + rw * OWN * S::RB;
+  Place place = place_of(key0);
+  auto step = [&]() {
+    if (place.key + 32 > end) {                                // the last cached tokens, once and again
+      place = place_of(end);
+    } else {
+      place.key += 32;
+      place.entry += whole;
+      place.in += rest;
+      if (place.in >= pg.page) { place.in -= pg.page; ++place.entry; }
+    }
+  };
+  struct From { const char* k; int most, page, in; };          // addresses, and the last cached token, of the tiles asked for
+  auto where = [&](int page) {
+    page = (unsigned)page < (unsigned)pg.NP ? page : 0;
+    From f;
+    f.k = kbase + (unsigned long long)(uint32_t)page * page_bytes + (uint32_t)place.in * row_bytes;
+    f.most = tend - place.key;
+    f.page = page;
+    f.in = place.in;
+    return f;
+  };
+  auto ask = [&](const From& f, bool values, int buf) {
+    uint32_t off[LOADS];
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      if constexpr (!S::I8) {
-        const int key = RPL * j + lrow;
-        const uint32_t off = (uint32_t)min(key, most) * row_bytes;
-        load16(kp, off + 16 * ((lane % CPR) ^ S::place_k(rw * OWN + key)), to + 1024 * j);
-        load16(vp, off + 16 * ((lane % CPR) ^ S::place_v(rw * OWN + key)), to + S::TILE + 1024 * j);
-      } else {
-        const uint32_t off = (uint32_t)min(min(RPL * j + lrow, OWN - 1), most) * row_bytes + 16 * (lane % CPR);
-        kreg[j] = *(const u32x4*)(kp + off);
-        vreg[j] = *(const u32x4*)(vp + off);
-      }
-    }
-    if constexpr (S::I8) {
-      const long long x = (long long)page * pg.s_page_ld + (long long)(in + min(min(lane, OWN - 1), most)) * pg.s_row_ld + (long long)hk * pg.s_head_ld;
-      ksc = pg.k_scale[x];
-      vsc = pg.v_scale[x];
-    }
-  };
-  auto settle = [&](int buf) {                                 // codes in registers -> bf16 in LDS
-    if constexpr (S::I8) {
+    for (int j = 0; j < LOADS; ++j) off[j] = values ? voff[j] : koff[j];
+    if (f.most < OWN - 1) {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
-        const int key = RPL * j + lrow, tk = rw * OWN + key, ch = 2 * (lane % CPR);
+        const int key = min(RPL * j + lrow, OWN - 1);
+        off[j] -= (uint32_t)(key - min(key, f.most)) * row_bytes;
+      }
+    }
+    const char* from = values ? f.k + vfar : f.k;
+    if constexpr (S::I8) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) (values ? vreg : kreg)[j] = *(const u32x4*)(from + off[j]);
+      const long long x = (long long)f.page * pg.s_page_ld + (long long)(f.in + min(min(lane, OWN - 1), f.most)) * pg.s_row_ld + (long long)hk * pg.s_head_ld;
+      if (values) vsc = pg.v_scale[x];
+      else ksc = pg.k_scale[x];
+    } else {
+      load16s<LOADS>(from, off, lds + (values ? S::V0 : S::K0) + buf * S::TILE + rw * OWN * S::RB);
+    }
+  };
+  auto settle = [&](bool values, int buf) {                    // codes in registers -> bf16 in LDS
+    if constexpr (S::I8) {
+      char* at = lds + (values ? S::V0 : S::K0) + buf * S::TILE;
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int key = RPL * j + lrow, tk = rw * OWN + key, ch = 2 * (lane % CPR), pl = values ? S::place_v(tk) : S::place_k(tk);
         if (key < OWN) {
-          char* to = lds + buf * S::STAGE + tk * S::RB;
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const u32x2 k0 = codes(kreg[j][2 * y]), k1 = codes(kreg[j][2 * y + 1]), v0 = codes(vreg[j][2 * y]), v1 = codes(vreg[j][2 * y + 1]);
-            *(u32x4*)(to + 16 * ((ch + y) ^ S::place_k(tk))) = u32x4{k0[0], k0[1], k1[0], k1[1]};
-            *(u32x4*)(to + S::TILE + 16 * ((ch + y) ^ S::place_v(tk))) = u32x4{v0[0], v0[1], v1[0], v1[1]};
+            const u32x4& w = (values ? vreg : kreg)[j];
+            const u32x2 c0 = codes(w[2 * y]), c1 = codes(w[2 * y + 1]);
+            *(u32x4*)(at + tk * S::RB + 16 * ((ch + y) ^ pl)) = u32x4{c0[0], c0[1], c1[0], c1[1]};
           }
         }
       }
-      float* sc = (float*)(lds + 2 * S::STAGE) + buf * 2 * KT + rw * OWN;
-      if (lane < OWN) { sc[lane] = ksc; sc[KT + lane] = vsc; }
+      if (lane < OWN) ((float*)(lds + S::SCALES))[32 * (2 * values + buf) + rw * OWN + lane] = values ? vsc : ksc;
     }
   };
 
@@ -591,55 +651,147 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   const int kread = col * S::RB + 16 * (g ^ S::place_k(col));
   const int vkey = 4 * g + ((lane & 15) >> 2);
   const int vread = vkey * S::RB + 16 * ((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ S::place_v(vkey)) + 8 * (lane & 1);
-  auto tile = [&](int t, int buf) {
-    if (!busy) return;
+  const char *kat[KS], *vat[MB];
 #pragma unroll
-    for (int x = 0; x < KT / 32; ++x) {
-      const char* K = lds + buf * S::STAGE + 32 * x * S::RB;
-      const char* V = K + S::TILE;
-      const int k0 = t * KT + 32 * x;
-      if (k0 > last || k0 + 32 <= wave_from) continue;
-      f32x16 s[1] = {f32x16(0.f)};
+  for (int j = 0; j < KS; ++j) kat[j] = lds + S::K0 + (kread ^ (32 * j));
 #pragma unroll
-      for (int i = 0; i < KS; ++i) s[0] = Rows<32>::mfma(lds_read16(K + (kread ^ (32 * i))), q[i], s[0]);
-      const float* sc = (const float*)(lds + 2 * S::STAGE) + buf * 2 * KT + 32 * x + 4 * g;
-      if constexpr (S::I8) {
+  for (int j = 0; j < MB; ++j) vat[j] = lds + S::V0 + (vread ^ (64 * j));
+  auto keys = [&](int buf, int j) { return lds_read16(kat[j] + buf * S::TILE); };
+  auto values = [&](int buf, int j) {                          // the j-th operand: channels 32 (j % MB) .., keys 16 (j / MB) ..
+    const char* at = vat[j % MB] + buf * S::TILE + j / MB * 16 * S::RB;
+    const u32x2 y = lds_read_tr(at), z = lds_read_tr(at + 8 * S::RB);
+    return u32x4{y[0], y[1], z[0], z[1]};
+  };
+  auto masked = [&](int t) { return t * 32 + 31 > first || t * 32 < full; };
+  auto adjust = [&](int t, int buf, f32x16 (&s)[1]) {
+    if constexpr (S::I8) run.times(s, (const float*)(lds + S::SCALES) + 32 * buf + 4 * g);
+    if (masked(t)) run.mask(s, from - t * 32 - 4 * g, pos - t * 32 - 4 * g, -INFINITY);
+  };
+
+  // The order of the next two is kept as written (nothing moves over a sched_barrier): a matrix instruction, its share of vector
+  // instructions, the operands of the matrix instruction AHEAD of it.
+  constexpr int AHEAD = 4, N = 2 * MB;
+  u32x4 v[N];
+  auto scores_and_weigh = [&](int kbuf, int vbuf, f32x16 (&next)[1], f32x16 (&s)[1], u32x4 (&p)[2]) {
+    u32x4 k[KS];
+    float part[2] = {0.f, 0.f};
+    uint32_t w[8];
+    auto weigh = [&](int lo, int hi) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 w = *(const f32x4*)(sc + 8 * i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[0][4 * i + e] *= w[e];
-        }
+      for (int e = lo; e < hi; ++e) {
+        float y = __builtin_amdgcn_exp2f(fmaf(s[0][e], c, -run.ref));
+        stay(y);
+        s[0][e] = y;
+        part[e & 1] += y;
+        if (!S::I8 && (e & 1)) { w[e >> 1] = pk_bf16(s[0][e - 1], s[0][e]); stay(w[e >> 1]); }
       }
-      const bool masked = k0 + 31 > first || k0 < full;
-      soft_step<32, D, S::I8>(run, s, c, masked, from - k0 - 4 * g, pos - k0 - 4 * g, sc + KT,
-        [&](int f, int i) {
-          const char* at = V + f * 16 * S::RB + (vread ^ (64 * i));
-          const u32x2 y = lds_read_tr(at), z = lds_read_tr(at + 8 * S::RB);
-          return u32x4{y[0], y[1], z[0], z[1]};
-        });
-      if (!S::I8 && masked) poisoned |= tile_not_finite<D>(V);
+      stay(part[0]);
+      stay(part[1]);
+    };
+#pragma unroll
+    for (int j = 0; j < (AHEAD < KS ? AHEAD : KS); ++j) k[j] = keys(kbuf, j);
+    __builtin_amdgcn_sched_barrier(0);
+    weigh(0, 4);                                               // while they are on their way
+    __builtin_amdgcn_sched_barrier(0);
+    next[0] = f32x16(0.f);
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      if (j + AHEAD < KS) k[j + AHEAD] = keys(kbuf, j + AHEAD);
+      next[0] = Rows<32>::mfma(k[j], q[j], next[0]);
+      weigh(4 + 12 * j / KS, 4 + 12 * (j + 1) / KS);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    run.l += part[0] + part[1];
+    if (!S::I8) {
+      p[0] = u32x4{w[0], w[1], w[2], w[3]};
+      p[1] = u32x4{w[4], w[5], w[6], w[7]};
+    }
+#pragma unroll
+    for (int j = 0; j < (AHEAD < N ? AHEAD : N); ++j) v[j] = values(vbuf, j);
+  };
+  auto meet_and_largest = [&](int vbuf, const u32x4 (&p)[2], const f32x16 (&next)[1], float& mx) {
+    constexpr int SHARE = 16 / N > 0 ? 16 / N : 1;
+    mx = next[0][0];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j + AHEAD < N) v[j + AHEAD] = values(vbuf, j + AHEAD);
+      run.o[j % MB] = Rows<32>::mfma(v[j], p[j / MB], run.o[j % MB]);
+#pragma unroll
+      for (int e = j * SHARE; e < (j + 1) * SHARE; ++e) mx = fmaxf(mx, next[0][e]);
+      stay(mx);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
+
   const int tiles = piece.t1 - piece.t0;
   if (tiles > 0) {
-    ask(piece.t0, page_at(piece.t0), 0);
-    int page = page_at(piece.t0 + 1);
-    settle(0);
-    for (int i = 0; i < tiles; ++i) {
-      if constexpr (!S::I8) wait_loads<0>();
-      __syncthreads();
-      const int t = piece.t0 + i, buf = i & 1;
-      if (i + 1 < tiles) {
-        ask(t + 1, page, buf ^ 1);
-        page = page_at(t + 2);
+    From kfrom = where(tab[place.entry]), vfrom = kfrom;
+    ask(kfrom, false, 0);
+    ask(kfrom, true, 0);
+    settle(false, 0);
+    settle(true, 0);
+    step();
+    if (tiles > 1) {
+      vfrom = where(tab[place.entry]);
+      ask(vfrom, false, 1);
+      settle(false, 1);
+    }
+    step();
+    int entry = tab[place.entry];
+    if constexpr (!S::I8) wait_loads<0>();
+    __syncthreads();
+    f32x16 one[1], two[1];                                     // scores of a tile and of the next, in turn
+    if (busy) {
+      one[0] = f32x16(0.f);
+#pragma unroll
+      for (int j = 0; j < KS; ++j) one[0] = Rows<32>::mfma(keys(0, j), q[j], one[0]);
+      adjust(piece.t0, 0, one);
+      run.follow(one, run.largest(one), c);
+    }
+    auto tile = [&](int i, int buf, f32x16 (&s)[1], f32x16 (&next)[1]) {     // buf: i & 1
+      const bool more = i + 1 < tiles;
+      const int t = piece.t0 + i;
+      if (i > 0) {
+        // this tile's V and the next one's K are here; the K of this one and the V before it are used up
+        if constexpr (S::I8) {
+          if (more) settle(false, buf ^ 1);
+          settle(true, buf);
+        } else {
+          wait_loads<0>();
+        }
+        __syncthreads();
       }
-      tile(t, buf);
-      if (i + 1 < tiles) settle(buf ^ 1);
+      if (more) ask(vfrom, true, buf ^ 1);
+      if (i + 2 < tiles) {
+        vfrom = where(entry);
+        ask(vfrom, false, buf);
+        step();
+        entry = tab[place.entry];
+      }
+      if (!busy) return;
+      u32x4 p[2];
+      float mx;
+      scores_and_weigh(buf ^ 1, buf, next, s, p);              // after the last tile: of what lies there, for nothing
+      if constexpr (S::I8) {
+        run.times(s, (const float*)(lds + S::SCALES) + 32 * (2 + buf) + 4 * g);
+        if (masked(t)) run.mask(s, from - t * 32 - 4 * g, pos - t * 32 - 4 * g, 0.f);      // a scale that is not finite, not seen
+        run.pack(s, p);
+      }
+      if (more) adjust(t + 1, buf ^ 1, next);
+      meet_and_largest(buf, p, next, mx);
+      if (!S::I8 && masked(t)) poisoned |= tile_not_finite<D>(lds + S::V0 + buf * S::TILE);
+      if (more) run.follow(next, mx, c);
+    };
+    for (int i = 0;;) {
+      tile(i, 0, one, two);
+      if (++i >= tiles) break;
+      tile(i, 1, two, one);
+      if (++i >= tiles) break;
     }
   }
-  if (poisoned) {
-    rows_again<D>(a, pg, b, pl, n, hk, sq, r0 + 32 * rw, min(r0 + 32 * rw + 32, r0 + rows), piece.t0 * (KT / 32), piece.t1 * (KT / 32), 1,
+  if (__builtin_amdgcn_readfirstlane(poisoned)) {
+    rows_again<D>(a, pg, b, pl, n, hk, sq, r0 + 32 * rw, min(r0 + 32 * rw + 32, r0 + rows), piece.t0, piece.t1, 1,
                   [&](int r, float m, float l, const float* y) {
       constexpr int C = D / 64;
       const int tk = r / G;
@@ -792,7 +944,7 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
   typedef Few<D, 4, I8> F;
-  typedef Many<D, 4, D == 256 ? 32 : 64, 8, D == 256 ? 1 : 2, I8> M;
+  typedef Many<D, 4, 16, D == 256 ? 1 : 2, I8> M;
 };
 
 // LDS beyond what a kernel has unasked: asked for once on each device, and again where that failed.
