@@ -389,6 +389,8 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
     ask_scales(0);
     ask(false);
     ask(true);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) stay(q[s]);                   // here now: the loop must not wait for them, nor for what it asks for
     // this lane's reads: 8 channels of two keys; 4 (8) keys by 16 channels a group of 16 lanes
     const int kread = col * S::RB + (S::I8 ? ((g >> 1) ^ S::place_k(col)) * 16 + 8 * (g & 1) : (g ^ S::place_k(col)) * 16);
     const int vkey = S::I8 ? 4 * g + ((lane & 15) >> 1 & 3) + 16 * ((lane & 15) >> 3) : 4 * g + ((lane & 15) >> 2);
@@ -739,6 +741,8 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
     }
     step();
     int entry = tab[place.entry];
+#pragma unroll
+    for (int j = 0; j < KS; ++j) stay(q[j]);                   // here now: the loop must not wait for them, nor for what it asks for
     if constexpr (!S::I8) wait_loads<0>();
     __syncthreads();
     f32x16 one[1], two[1];                                     // scores of a tile and of the next, in turn
