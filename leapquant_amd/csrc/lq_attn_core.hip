@@ -20,6 +20,8 @@
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -47,22 +49,26 @@ __device__ __forceinline__ u32x2 lds_read_tr8(const char* p) {
 }
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-// 16 (4) bytes a lane from base + off into LDS at lds + 16 lane (4 lane); the caller waits before it reads them
+// 16 (4) bytes a lane from base + off into LDS at lds + 16 lane (4 lane); the caller waits before it reads them.  The compiler does not see
+// what these wait for: M0, written by the scalar unit, one instruction on, and a base that v_readlane wrote, five on.
 __device__ __forceinline__ void load16(const char* base, uint32_t off, const char* lds) {
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(to) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(off), "s"(base), "s"(to) : "memory", "m0");
 }
 // N of them, the j-th with an immediate of 1024 j bytes on both its address and its place
 template <int N> __device__ __forceinline__ void load16s(const char* base, const uint32_t (&off)[N], const char* lds) {
-  static_assert(N == 1 || N == 2 || N == 4, "loads of a wave");
+  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "loads of a wave");
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
   if constexpr (N == 1)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0" :: "s"(base), "s"(to), "v"(off[0]) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0" :: "s"(base), "s"(to), "v"(off[0]) : "memory", "m0");
   else if constexpr (N == 2)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024"
                  :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
+  else if constexpr (N == 8) {                                 // an immediate has 12 bits: the j-th of 1024 (j & 3)
+    load16s<4>(base, {off[0], off[1], off[2], off[3]}, lds);
+    load16s<4>(base, {off[4], off[5], off[6], off[7]}, lds + 4096);
+  } else
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
                  "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:3072"
                  :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "m0");
 }
@@ -122,7 +128,7 @@ template <class S> __device__ __forceinline__ Piece piece_of(const Keys& k, int 
 template <int R> struct Rows;
 template <> struct Rows<32> {
   typedef f32x16 acc;
-  static constexpr int E = 16, F = 2, STEP = 8, A = 1, AN = 16, DM = 32;    // A accumulators of AN; channels of an output
+  static constexpr int STEP = 8, AN = 16, DM = 32;             // scores of an accumulator, channels of an output
   static __device__ __forceinline__ acc mfma(const u32x4& a, const u32x4& b, const acc& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -131,7 +137,7 @@ template <> struct Rows<32> {
 };
 template <> struct Rows<16> {
   typedef f32x4 acc;
-  static constexpr int E = 8, F = 1, STEP = 16, A = 2, AN = 4, DM = 16;
+  static constexpr int STEP = 16, AN = 4, DM = 16;
   static __device__ __forceinline__ acc mfma(const u32x4& a, const u32x4& b, const acc& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
@@ -142,7 +148,7 @@ template <> struct Rows<16> {
 // What a wave carries along its keys: outputs O^T, a row's running maximum m (of q . k, not scaled) and sum l.
 template <int R, int D> struct Run {
   typedef Rows<R> W;
-  static constexpr int MB = D / W::DM, E = W::E, AN = W::AN;
+  static constexpr int MB = D / W::DM, AN = W::AN;
   typename W::acc o[MB];
   float m, l, ref;
   bool huge;
@@ -153,15 +159,15 @@ template <int R, int D> struct Run {
 #pragma unroll
     for (int i = 0; i < MB; ++i) o[i] = typename W::acc(0.f);
   }
-  // the largest of 32 keys' scores
-  static __device__ __forceinline__ float largest(const typename W::acc (&s)[W::A]) {
+  // the largest of some keys' scores
+  template <int A> static __device__ __forceinline__ float largest(const typename W::acc (&s)[A]) {
     float mx = s[0][0];
 #pragma unroll
-    for (int i = 1; i < E; ++i) mx = fmaxf(mx, s[i / AN][i % AN]);
+    for (int i = 1; i < A * AN; ++i) mx = fmaxf(mx, s[i / AN][i % AN]);
     return mx;
   }
   // m follows scores whose largest is mx, by steps of 2^GROWN or more
-  __device__ __forceinline__ void follow(typename W::acc (&s)[W::A], float mx, float c) {
+  template <int A> __device__ __forceinline__ void follow(typename W::acc (&s)[A], float mx, float c) {
     mx = W::max_over(mx);
     if (__any((mx - m) * c > GROWN)) {
       const float to = fmaxf(m, mx), alpha = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - to) * c);
@@ -179,40 +185,26 @@ template <int R, int D> struct Run {
     if (huge) {
       const float raw = m == -INFINITY ? 0.f : m;
 #pragma unroll
-      for (int i = 0; i < E; ++i) s[i / AN][i % AN] -= raw;
+      for (int i = 0; i < A * AN; ++i) s[i / AN][i % AN] -= raw;
     }
   }
-  // scores into weights, their sum into l
-  __device__ __forceinline__ void weigh(typename W::acc (&s)[W::A], float c) {
-    float part[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      s[i / AN][i % AN] = __builtin_amdgcn_exp2f(fmaf(s[i / AN][i % AN], c, -ref));
-      part[i & 1] += s[i / AN][i % AN];
-    }
-    l += part[0] + part[1];
-  }
-  // weights as operands of the second product
-  static __device__ __forceinline__ void pack(const typename W::acc (&s)[W::A], u32x4 (&p)[W::F]) {
-#pragma unroll
-    for (int i = 0; i < E / 2; ++i) p[i >> 2][i & 3] = pk_bf16(s[2 * i / AN][2 * i % AN], s[2 * i / AN][2 * i % AN + 1]);
-  }
-  // Keys at places lo .. hi of the 32 (less 4 g) are seen, the others' scores or weights become `none`.
-  static __device__ __forceinline__ void mask(typename W::acc (&s)[W::A], int lo, int hi, float none) {
+  // Of one accumulator, whose i-th score is of key STEP (i / 4) + i % 4: keys lo .. hi are seen, the others' become `none`.
+  static __device__ __forceinline__ void mask(typename W::acc& s, int lo, int hi, float none) {
     asm volatile("" : "+v"(lo), "+v"(hi));                     // a branch of its own, not selects for every tile
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
+    for (int i = 0; i < AN; ++i) {
       const int j = W::STEP * (i >> 2) + (i & 3);
-      s[i / AN][i % AN] = j >= lo && j <= hi ? s[i / AN][i % AN] : none;
+      s[i] = j >= lo && j <= hi ? s[i] : none;
     }
   }
-  // times the scales of the keys or values, by places less 4 g
-  static __device__ __forceinline__ void times(typename W::acc (&s)[W::A], const float* scale) {
+  // times the scales of its keys
+  static __device__ __forceinline__ void times(typename W::acc& s, const float* scale) {
 #pragma unroll
-    for (int i = 0; i < E; i += 4) {
+    for (int i = 0; i < AN; i += 4) {
       const f32x4 x = *(const f32x4*)(scale + W::STEP * (i >> 2));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i / AN][i % AN + e] *= x[e];
+      for (int e = 0; e < 4; ++e) s[i + e] *= x[e];
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -233,10 +225,15 @@ template <int D> __device__ __forceinline__ bool tile_not_finite(const char* til
   return __any(hit != 0);
 }
 
-// Rows [ra, rb) of a sequence again, key by key: for a wave that met values which are not finite in a tile that not all of its rows
-// see.  The products give a key that a row does not see a probability of zero, and zero times an infinity or NaN is not zero.  Keys
-// are those of the wave, 32 u .. 32 u + 31 for u = u0, u0 + step .. < u1.  sink(row, m, l, y): channels D / 64 lane .. of a row.
-template <int D, class F>
+__device__ __forceinline__ bool scales_not_finite(const float* scale) {
+  return __any(!(fabsf(scale[threadIdx.x & 31]) < INFINITY));
+}
+
+// Rows [ra, rb) of a sequence again, key by key: for a wave that met values (or scales of them) which are not finite in a tile that not
+// all of its rows see.  The products give a key that a row does not see a probability of zero, and zero times an infinity or NaN is
+// not zero.  Keys are those of the wave, 32 u .. 32 u + 31 for u = u0, u0 + step .. < u1.  sink(row, m, l, y): channels D / 64
+// lane .. of a row.
+template <int D, bool I8, class F>
 __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, int n, int hk,
                                            const Seq& sq, int ra, int rb, int u0, int u1, int step, const F& sink) {
   constexpr int C = D / 64;
@@ -257,9 +254,22 @@ __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages
       float s = 0.f;
 #pragma unroll 1
       for (int i = 0; i < D; i += 8) {
-        const u32x4 x = *(const u32x4*)(q + i), k = *(const u32x4*)((const bf16_t*)pg.k + at + i);
+        const u32x4 x = *(const u32x4*)(q + i);
+        u32x4 k;
+        if constexpr (I8) {
+          const u32x2 w = *(const u32x2*)((const int8_t*)pg.k + at + i), k0 = codes(w[0]), k1 = codes(w[1]);
+          k = u32x4{k0[0], k0[1], k1[0], k1[1]};
+        } else {
+          k = *(const u32x4*)((const bf16_t*)pg.k + at + i);
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) s = fmaf(bf_hi(x[e]), bf_hi(k[e]), fmaf(bf_lo(x[e]), bf_lo(k[e]), s));
+      }
+      float vs = 1.f;
+      if constexpr (I8) {
+        const long long x = (long long)page * pg.s_page_ld + (long long)(kk - pi * pg.page) * pg.s_row_ld + (long long)hk * pg.s_head_ld;
+        s *= pg.k_scale[x];
+        vs = pg.v_scale[x];
       }
       if (!sees) s = -INFINITY;
       const float to = fmaxf(m, max64(s)), raw = to == -INFINITY ? 0.f : to;
@@ -272,10 +282,13 @@ __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages
 #pragma unroll 1
       for (int j = 0; j < 32; ++j) {
         if (32 * u + j < from || 32 * u + j > pos) continue;
-        const float pj = __shfl(p, j);
+        const float pj = __shfl(p, j) * __shfl(vs, j);
         const long long vj = __shfl(at, j);
 #pragma unroll
-        for (int e = 0; e < C; ++e) y[e] = fmaf(pj, bf2f(((const bf16_t*)pg.v)[vj + C * lane + e]), y[e]);
+        for (int e = 0; e < C; ++e) {
+          const long long x = vj + C * lane + e;
+          y[e] = fmaf(pj, I8 ? (float)((const int8_t*)pg.v)[x] : bf2f(((const bf16_t*)pg.v)[x]), y[e]);
+        }
       }
     }
     sink(r, m, l, y);
@@ -417,23 +430,34 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           s[x] = Rows<16>::mfma(k, q[i], s[x]);
         }
       }
-      if constexpr (S::I8) run.times(s, sc);
+      if constexpr (S::I8) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) run.times(s[x], sc + 16 * x);
+      }
       if (more) {
         wait_lds();
         ask_scales(odd ^ 1);
         ask(false);
       }
-      const int k0 = 32 * t, lo = from - k0 - 4 * g, hi = pos - k0 - 4 * g;
+      const int k0 = 32 * t;
       const bool masked = k0 + 31 > first || k0 < full;
-      if (masked) run.mask(s, lo, hi, -INFINITY);
-      run.follow(s, run.largest(s), c);
-      run.weigh(s, c);
-      if constexpr (S::I8) {
-        run.times(s, sc + 32);
-        if (masked) run.mask(s, lo, hi, 0.f);                  // a scale that is not finite, not seen
+      if (masked) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) run.mask(s[x], from - k0 - 16 * x - 4 * g, pos - k0 - 16 * x - 4 * g, -INFINITY);
       }
-      u32x4 p[1];
-      run.pack(s, p);
+      run.follow(s, run.largest(s), c);
+      u32x4 p;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[x][e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], c, -run.ref));
+          run.l += s[x][e];
+        }
+        if constexpr (S::I8) run.times(s[x], sc + 32 + 16 * x);
+        p[2 * x] = pk_bf16(s[x][0], s[x][1]);
+        p[2 * x + 1] = pk_bf16(s[x][2], s[x][3]);
+      }
       if (more) wait_loads<S::LOADS + S::SC>();                // V is here
       else wait_loads<0>();
       const char* V = mine + S::UNIT;
@@ -448,9 +472,9 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           const u32x2 x = lds_read_tr(V + (vread ^ (32 * i))), y = lds_read_tr(V + 16 * S::RB + (vread ^ (32 * i)));
           v = u32x4{x[0], x[1], y[0], y[1]};
         }
-        run.o[i] = Rows<16>::mfma(v, p[0], run.o[i]);
+        run.o[i] = Rows<16>::mfma(v, p, run.o[i]);
       }
-      if (!S::I8 && masked) poisoned |= tile_not_finite<D>(V);
+      if (masked) poisoned |= S::I8 ? scales_not_finite(sc - 4 * g + 32) : tile_not_finite<D>(V);
       if (more) {
         wait_lds();
         ask(true);
@@ -469,7 +493,7 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
     for (int i = 0; i < MB; ++i) *(f32x4*)(to + 16 * i) = run.o[i];
     if (g == 0) { jm[kw * S::ROWS + col] = run.m; jm[(KW + kw) * S::ROWS + col] = run.l; }
   } else {
-    rows_again<D>(a, pg, b, pl, n, hk, sq, r0, r0 + rows, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
+    rows_again<D, S::I8>(a, pg, b, pl, n, hk, sq, r0, r0 + rows, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
       constexpr int C = D / 64;
 #pragma unroll
       for (int e = 0; e < C; ++e) jo[(kw * S::ROWS + r - r0) * (D + 4) + C * lane + e] = y[e];
@@ -515,26 +539,133 @@ __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_page
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------
-// RW waves of 32 rows each share tiles of 32 keys.  A wave forms the scores of a tile while it takes the exponentials of the one before,
-// and looks for their maximum while that one meets its values: matrix and vector instructions of a wave overlap.  K is so a tile
-// ahead of V, and two tiles of each lie in LDS.  Codes go through registers and into LDS as bf16.
+// RW waves of 32 rows each share tiles of 64 keys, K and V twice in LDS, K a tile ahead of V.  A wave forms the scores of a tile while it
+// takes the exponentials of the one before, and looks for their maximum while that one meets its values, so that its vector
+// instructions go in the shadow of its matrix instructions.  What bounds it then is the number of a wave's instructions.
+// Codes go through registers and into LDS as bf16.
 template <int D_, int RW_, int LEAST_, int EU_, bool I8_> struct Many {
-  static constexpr int D = D_, RW = RW_, EU = EU_, KT = 32, LEAST = LEAST_, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
+  static constexpr int D = D_, RW = RW_, EU = EU_, KT = 64, LEAST = LEAST_, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
   static constexpr bool I8 = I8_;
   static constexpr int RB = 2 * D, TILE = KT * RB;             // bytes in LDS
   static constexpr int K0 = 0, V0 = 2 * TILE, SCALES = 4 * TILE, LDS = SCALES + (I8 ? 4 * KT * 4 : 0);
   static constexpr int PART = ROWS * (D + 2);
+  static constexpr int AHEAD = D == 256 ? 6 : 4;               // operands on their way: registers
   static constexpr int OWN = KT / RW;                          // keys of a tile that a wave loads, all of one page
+  static_assert(OWN <= 16, "keys of one page");
   // as Few's: 16 keys by a chunk of K, 4 keys by four chunks of V
   static constexpr int SPAN = D == 64 ? 2 : 1;
   static __device__ __forceinline__ int place_k(int key) { return key / SPAN & (16 / SPAN - 1); }
   static __device__ __forceinline__ int place_v(int key) { return (key & 3) / SPAN << 2; }
 };
 
+// A wave's keys of the tiles, one tile after the other: where they lie, and on their way into LDS.
+template <class S> struct Tiles {
+  static constexpr int D = S::D, KT = S::KT, OWN = S::OWN, ES = S::I8 ? 1 : 2, CPR = D * ES / 16, RPL = 64 / CPR;
+  static constexpr int LOADS = OWN / RPL > 0 ? OWN / RPL : 1;
+  static_assert(S::I8 || OWN % RPL == 0, "a load of a whole wave");
+  // The j-th load's immediate, 1024 (j & 3), moves its place in LDS and its address: the offsets are that much less, and the bases
+  // 4096 less.
+  static constexpr int LESS = S::I8 ? 0 : 4096;
+  const_int* tab;
+  const char* kbase;
+  long long vfar;
+  uint32_t row_bytes, page_bytes;
+  int rw, lane, hk, tend, end, whole, rest;
+  uint32_t koff[LOADS], voff[LOADS];                           // where this lane's chunks come from, so that they lie swizzled
+  int key, entry, in;                                          // the next tile's: in `entry` of the table's row, at place `in` of its page
+  struct From { const char* k; int most, page, in; };          // addresses, and the last cached token, of a tile
+  u32x4 kreg[S::I8 ? LOADS : 1], vreg[S::I8 ? LOADS : 1];
+  float ksc, vsc;
+
+  __device__ __forceinline__ void at(const lq_pages& pg, const PageDiv& div, int k) {
+    key = min(k, end);
+    entry = __builtin_amdgcn_readfirstlane(page_of(div, key));
+    in = key - entry * pg.page;
+  }
+  __device__ __forceinline__ void start(const lq_pages& pg, const lq_batch& b, const PageDiv& div, int n, int hk_, int rw_, int last, int t0) {
+    rw = rw_;
+    hk = hk_;
+    lane = threadIdx.x & 63;
+    tab = (const_int*)(b.table + (long long)n * b.table_ld);
+    tend = last;
+    end = last & ~(OWN - 1);
+    whole = KT / pg.page;
+    rest = KT - whole * pg.page;
+    kbase = (const char*)pg.k + (long long)hk * pg.head_ld * ES - LESS;
+    vfar = (const char*)pg.v - (const char*)pg.k;
+    row_bytes = (uint32_t)pg.row_ld * ES;
+    page_bytes = (uint32_t)pg.page_ld * ES;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int k = min(RPL * j + lane / CPR, OWN - 1), tk = rw * OWN + k;
+      const uint32_t off = (uint32_t)k * row_bytes + LESS - (S::I8 ? 0 : 1024 * (j & 3));
+      koff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_k(tk));
+      voff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_v(tk));
+    }
+    at(pg, div, t0 * KT + rw * OWN);
+  }
+  __device__ __forceinline__ void step(const lq_pages& pg, const PageDiv& div) {
+    if (key + KT > end) {                                      // the last cached tokens, once and again
+      at(pg, div, end);
+    } else {
+      key += KT;
+      entry += whole;
+      in += rest;
+      if (in >= pg.page) { in -= pg.page; ++entry; }
+    }
+  }
+  __device__ __forceinline__ int page() const { return tab[entry]; }
+  __device__ __forceinline__ From where(const lq_pages& pg, int page) const {
+    page = (unsigned)page < (unsigned)pg.NP ? page : 0;
+    return {kbase + (unsigned long long)(uint32_t)page * page_bytes + (uint32_t)in * row_bytes, tend - key, page, in};
+  }
+  __device__ __forceinline__ void ask(const lq_pages& pg, const From& f, bool values, char* to) {
+    uint32_t off[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) off[j] = values ? voff[j] : koff[j];
+    if (f.most < OWN - 1) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int k = min(RPL * j + lane / CPR, OWN - 1);
+        off[j] -= (uint32_t)(k - min(k, f.most)) * row_bytes;
+      }
+    }
+    const char* from = values ? f.k + vfar : f.k;
+    if constexpr (S::I8) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) (values ? vreg : kreg)[j] = *(const u32x4*)(from + off[j]);
+      const long long x = (long long)f.page * pg.s_page_ld + (long long)(f.in + min(min(lane, OWN - 1), f.most)) * pg.s_row_ld + (long long)hk * pg.s_head_ld;
+      if (values) vsc = pg.v_scale[x];
+      else ksc = pg.k_scale[x];
+    } else {
+      load16s<LOADS>(from, off, to + rw * OWN * S::RB);
+    }
+  }
+  // codes in registers -> bf16 in LDS
+  __device__ __forceinline__ void settle(bool values, char* to, float* scale) const {
+    if constexpr (S::I8) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int k = RPL * j + lane / CPR, tk = rw * OWN + k, ch = 2 * (lane % CPR), place = values ? S::place_v(tk) : S::place_k(tk);
+        if (k < OWN) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const u32x4& w = (values ? vreg : kreg)[j];
+            const u32x2 c0 = codes(w[2 * y]), c1 = codes(w[2 * y + 1]);
+            *(u32x4*)(to + tk * S::RB + 16 * ((ch + y) ^ place)) = u32x4{c0[0], c0[1], c1[0], c1[1]};
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      if (lane < OWN) scale[rw * OWN + lane] = values ? vsc : ksc;
+    }
+  }
+};
+
 template <class S>
 __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
                                           int hk, int split, int r0, const Seq& sq, float* part) {
-  constexpr int D = S::D, KS = D / 16, MB = D / 32, OWN = S::OWN;
+  constexpr int D = S::D, KT = S::KT, KS = D / 16, MB = D / 32;
   const int rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
   const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), pl.splits, split);
@@ -550,105 +681,12 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
 #pragma unroll
     for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 16 * s);
   }
-
-  // ---- tiles: this wave's keys of each
-  const_int* tab = (const_int*)(b.table + (long long)n * b.table_ld);
-  const int tend = max(sq.len - 1, 0);
-  constexpr int ES = S::I8 ? 1 : 2, CPR = D * ES / 16, RPL = 64 / CPR, LOADS = OWN / RPL > 0 ? OWN / RPL : 1;
-  static_assert(S::I8 || OWN % RPL == 0, "a load of a whole wave");
-  // The j-th load's immediate, 1024 j, moves its place in LDS and its address: the offsets below are that much less, and the
-  // bases 4096 less.
-  constexpr int AHEAD_OF = S::I8 ? 0 : 4096;
-  const char* kbase = (const char*)pg.k + (long long)hk * pg.head_ld * ES - AHEAD_OF;
-  const long long vfar = (const char*)pg.v - (const char*)pg.k;
-  const uint32_t row_bytes = (uint32_t)pg.row_ld * ES, page_bytes = (uint32_t)pg.page_ld * ES;
-  const int lrow = lane / CPR;
-  uint32_t koff[LOADS], voff[LOADS];                           // where this lane's chunks come from, so that they lie swizzled
-#pragma unroll
-  for (int j = 0; j < LOADS; ++j) {
-    const int key = min(RPL * j + lrow, OWN - 1), tk = rw * OWN + key;
-    const uint32_t off = (uint32_t)key * row_bytes + AHEAD_OF - (S::I8 ? 0 : 1024 * j);
-    koff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_k(tk));
-    voff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_v(tk));
-  }
-  u32x4 kreg[S::I8 ? LOADS : 1], vreg[S::I8 ? LOADS : 1];
-  float ksc = 0.f, vsc = 0.f;
-  // the keys to ask for next: of tile at / 32, in `page` of the table's row at place `in`; a tile on by steps
-  const int key0 = piece.t0 * 32 + rw * OWN, end = tend & ~(OWN - 1), whole = 32 / pg.page, rest = 32 - whole * pg.page;
-  struct Place { int key, entry, in; };
-  auto place_of = [&](int key) {
-    Place p;
-    p.key = min(key, end);
-    p.entry = __builtin_amdgcn_readfirstlane(page_of(pl.div, p.key));
-    p.in = p.key - p.entry * pg.page;
-    return p;
-  };
-  Place place = place_of(key0);
-  auto step = [&]() {
-    if (place.key + 32 > end) {                                // the last cached tokens, once and again
-      place = place_of(end);
-    } else {
-      place.key += 32;
-      place.entry += whole;
-      place.in += rest;
-      if (place.in >= pg.page) { place.in -= pg.page; ++place.entry; }
-    }
-  };
-  struct From { const char* k; int most, page, in; };          // addresses, and the last cached token, of the tiles asked for
-  auto where = [&](int page) {
-    page = (unsigned)page < (unsigned)pg.NP ? page : 0;
-    From f;
-    f.k = kbase + (unsigned long long)(uint32_t)page * page_bytes + (uint32_t)place.in * row_bytes;
-    f.most = tend - place.key;
-    f.page = page;
-    f.in = place.in;
-    return f;
-  };
-  auto ask = [&](const From& f, bool values, int buf) {
-    uint32_t off[LOADS];
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) off[j] = values ? voff[j] : koff[j];
-    if (f.most < OWN - 1) {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        const int key = min(RPL * j + lrow, OWN - 1);
-        off[j] -= (uint32_t)(key - min(key, f.most)) * row_bytes;
-      }
-    }
-    const char* from = values ? f.k + vfar : f.k;
-    if constexpr (S::I8) {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) (values ? vreg : kreg)[j] = *(const u32x4*)(from + off[j]);
-      const long long x = (long long)f.page * pg.s_page_ld + (long long)(f.in + min(min(lane, OWN - 1), f.most)) * pg.s_row_ld + (long long)hk * pg.s_head_ld;
-      if (values) vsc = pg.v_scale[x];
-      else ksc = pg.k_scale[x];
-    } else {
-      load16s<LOADS>(from, off, lds + (values ? S::V0 : S::K0) + buf * S::TILE + rw * OWN * S::RB);
-    }
-  };
-  auto settle = [&](bool values, int buf) {                    // codes in registers -> bf16 in LDS
-    if constexpr (S::I8) {
-      char* at = lds + (values ? S::V0 : S::K0) + buf * S::TILE;
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        const int key = RPL * j + lrow, tk = rw * OWN + key, ch = 2 * (lane % CPR), pl = values ? S::place_v(tk) : S::place_k(tk);
-        if (key < OWN) {
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const u32x4& w = (values ? vreg : kreg)[j];
-            const u32x2 c0 = codes(w[2 * y]), c1 = codes(w[2 * y + 1]);
-            *(u32x4*)(at + tk * S::RB + 16 * ((ch + y) ^ pl)) = u32x4{c0[0], c0[1], c1[0], c1[1]};
-          }
-        }
-      }
-      if (lane < OWN) ((float*)(lds + S::SCALES))[32 * (2 * values + buf) + rw * OWN + lane] = values ? vsc : ksc;
-    }
-  };
-
   const float c = a.scale * LOG2E;
-  Run<32, D> run;
+  typedef Run<32, D> Carry;
+  Carry run;
   run.start();
   bool poisoned = false;
+
   // this lane's reads: a row of K; 4 keys by 16 channels a group of 16 lanes of V
   const int kread = col * S::RB + 16 * (g ^ S::place_k(col));
   const int vkey = 4 * g + ((lane & 15) >> 2);
@@ -658,133 +696,161 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   for (int j = 0; j < KS; ++j) kat[j] = lds + S::K0 + (kread ^ (32 * j));
 #pragma unroll
   for (int j = 0; j < MB; ++j) vat[j] = lds + S::V0 + (vread ^ (64 * j));
-  auto keys = [&](int buf, int j) { return lds_read16(kat[j] + buf * S::TILE); };
-  auto values = [&](int buf, int j) {                          // the j-th operand: channels 32 (j % MB) .., keys 16 (j / MB) ..
+  constexpr int NK = 2 * KS, NV = 4 * MB;                      // operands of a tile: the j-th of
+  auto keys = [&](int buf, int j) { return lds_read16(kat[j % KS] + buf * S::TILE + j / KS * 32 * S::RB); };   // 32 keys by 16 channels
+  auto values = [&](int buf, int j) {                                                                       // 32 channels by 16 keys
     const char* at = vat[j % MB] + buf * S::TILE + j / MB * 16 * S::RB;
     const u32x2 y = lds_read_tr(at), z = lds_read_tr(at + 8 * S::RB);
     return u32x4{y[0], y[1], z[0], z[1]};
   };
-  auto masked = [&](int t) { return t * 32 + 31 > first || t * 32 < full; };
-  auto adjust = [&](int t, int buf, f32x16 (&s)[1]) {
-    if constexpr (S::I8) run.times(s, (const float*)(lds + S::SCALES) + 32 * buf + 4 * g);
-    if (masked(t)) run.mask(s, from - t * 32 - 4 * g, pos - t * 32 - 4 * g, -INFINITY);
+  auto scale_at = [&](bool values, int buf) { return (const float*)(lds + S::SCALES) + KT * (2 * values + buf) + 4 * g; };
+  auto masked = [&](int t) { return t * KT + KT - 1 > first || t * KT < full; };
+  auto adjust = [&](int t, int buf, f32x16 (&s)[2]) {          // scores of tile t
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if constexpr (S::I8) Carry::times(s[x], scale_at(false, buf) + 32 * x);
+      if (masked(t)) Carry::mask(s[x], from - t * KT - 32 * x - 4 * g, pos - t * KT - 32 * x - 4 * g, -INFINITY);
+    }
   };
 
-  // The order of the next two is kept as written (nothing moves over a sched_barrier): a matrix instruction, its share of vector
-  // instructions, the operands of the matrix instruction AHEAD of it.
-  constexpr int AHEAD = 4, N = 2 * MB;
-  u32x4 v[N];
-  auto scores_and_weigh = [&](int kbuf, int vbuf, f32x16 (&next)[1], f32x16 (&s)[1], u32x4 (&p)[2]) {
-    u32x4 k[KS];
-    float part[2] = {0.f, 0.f};
-    uint32_t w[8];
-    auto weigh = [&](int lo, int hi) {
+  // The order of what follows is kept as written (nothing moves over a sched_barrier): a matrix instruction with its share of vector
+  // instructions, and the operand of the one AHEAD of it.  Weights go in pairs: the product in the exponent of one beside
+  // the exponentials of the one before, and the rounding and the sum (of what was rounded) of the one before that.
+  constexpr int PAIRS = 16, EARLY = 8;                         // of a tile; those beside the next tile's scores
+  float ex[2], old[2], vs[2];
+  uint32_t w[PAIRS];
+  auto exponent = [&](const f32x16 (&s)[2], int i) {
 #pragma unroll
-      for (int e = lo; e < hi; ++e) {
-        float y = __builtin_amdgcn_exp2f(fmaf(s[0][e], c, -run.ref));
-        stay(y);
-        s[0][e] = y;
-        part[e & 1] += y;
-        if (!S::I8 && (e & 1)) { w[e >> 1] = pk_bf16(s[0][e - 1], s[0][e]); stay(w[e >> 1]); }
-      }
-      stay(part[0]);
-      stay(part[1]);
-    };
-#pragma unroll
-    for (int j = 0; j < (AHEAD < KS ? AHEAD : KS); ++j) k[j] = keys(kbuf, j);
-    __builtin_amdgcn_sched_barrier(0);
-    weigh(0, 4);                                               // while they are on their way
-    __builtin_amdgcn_sched_barrier(0);
-    next[0] = f32x16(0.f);
-#pragma unroll
-    for (int j = 0; j < KS; ++j) {
-      if (j + AHEAD < KS) k[j + AHEAD] = keys(kbuf, j + AHEAD);
-      next[0] = Rows<32>::mfma(k[j], q[j], next[0]);
-      weigh(4 + 12 * j / KS, 4 + 12 * (j + 1) / KS);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    run.l += part[0] + part[1];
-    if (!S::I8) {
-      p[0] = u32x4{w[0], w[1], w[2], w[3]};
-      p[1] = u32x4{w[4], w[5], w[6], w[7]};
-    }
-#pragma unroll
-    for (int j = 0; j < (AHEAD < N ? AHEAD : N); ++j) v[j] = values(vbuf, j);
+    for (int e = 0; e < 2; ++e) { ex[e] = fmaf(s[i >> 3][2 * (i & 7) + e], c, -run.ref); stay(ex[e]); }
   };
-  auto meet_and_largest = [&](int vbuf, const u32x4 (&p)[2], const f32x16 (&next)[1], float& mx) {
-    constexpr int SHARE = 16 / N > 0 ? 16 / N : 1;
-    mx = next[0][0];
+  auto finish = [&](int i) {
+    if constexpr (S::I8) {
+      w[i] = pk_bf16(old[0] * vs[0], old[1] * vs[1]);
+      run.l += old[0] + old[1];
+    } else {
+      w[i] = pk_bf16(old[0], old[1]);
+      run.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, w[i]), s16x2{0x3f80, 0x3f80}, run.l, false);
+    }
+    stay(w[i]);
+  };
+  auto weigh = [&](const f32x16 (&s)[2], int buf, int lo, int hi) {            // pairs lo .. hi - 1; exponents of lo are there
+#pragma unroll
+    for (int i = lo; i < hi; ++i) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { f[e] = __builtin_amdgcn_exp2f(ex[e]); stay(f[e]); }
+      if (i + 1 < PAIRS) exponent(s, i + 1);
+      if (i > 0) finish(i - 1);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) old[e] = f[e];
+      if constexpr (S::I8) {
+        const f32x2 x = *(const f32x2*)(scale_at(true, buf) + 32 * (i >> 3) + 8 * ((i & 7) >> 1) + 2 * (i & 1));
+        vs[0] = x[0];
+        vs[1] = x[1];
+      }
+    }
+  };
+  auto scores_and_weigh = [&](int kbuf, int vbuf, f32x16 (&next)[2], const f32x16 (&s)[2]) {
+    u32x4 k[NK];
+#pragma unroll
+    for (int j = 0; j < S::AHEAD; ++j) k[j] = keys(kbuf, j);
+    exponent(s, 0);
+    next[0] = next[1] = f32x16(0.f);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j + AHEAD < N) v[j + AHEAD] = values(vbuf, j + AHEAD);
-      run.o[j % MB] = Rows<32>::mfma(v[j], p[j / MB], run.o[j % MB]);
-#pragma unroll
-      for (int e = j * SHARE; e < (j + 1) * SHARE; ++e) mx = fmaxf(mx, next[0][e]);
-      stay(mx);
+    for (int j = 0; j < NK; ++j) {
+      if (j + S::AHEAD < NK) k[j + S::AHEAD] = keys(kbuf, j + S::AHEAD);
+      next[j / KS] = Rows<32>::mfma(k[j], q[j % KS], next[j / KS]);
+      weigh(s, vbuf, EARLY * j / NK, EARLY * (j + 1) / NK);
       __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  auto meet_and_largest = [&](int vbuf, const f32x16 (&s)[2], const f32x16 (&next)[2]) {
+    u32x4 v[NV];
+    float mx = next[0][0];
+#pragma unroll
+    for (int j = 0; j < S::AHEAD; ++j) v[j] = values(vbuf, j);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (j + S::AHEAD < NV) v[j + S::AHEAD] = values(vbuf, j + S::AHEAD);
+      // the weights of the 16 keys j / MB are there: the last 8 pairs by the middle of the values, and a pair behind
+      const u32x4 p = {w[4 * (j / MB)], w[4 * (j / MB) + 1], w[4 * (j / MB) + 2], w[4 * (j / MB) + 3]};
+      run.o[j % MB] = Rows<32>::mfma(v[j], p, run.o[j % MB]);
+      if (j < 2 * MB) {
+        weigh(s, vbuf, EARLY + (PAIRS - EARLY) * j / (2 * MB), EARLY + (PAIRS - EARLY) * (j + 1) / (2 * MB));
+        if (j == 2 * MB - 1) finish(PAIRS - 1);
+      } else {
+#pragma unroll
+        for (int e = 32 * (j - 2 * MB) / (2 * MB); e < 32 * (j + 1 - 2 * MB) / (2 * MB); ++e) mx = fmaxf(mx, next[e >> 4][e & 15]);
+        stay(mx);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return mx;
   };
 
   const int tiles = piece.t1 - piece.t0;
   if (tiles > 0) {
-    From kfrom = where(tab[place.entry]), vfrom = kfrom;
-    ask(kfrom, false, 0);
-    ask(kfrom, true, 0);
-    settle(false, 0);
-    settle(true, 0);
-    step();
+    Tiles<S> tl;
+    tl.start(pg, b, pl.div, n, hk, rw, max(sq.len - 1, 0), piece.t0);
+    auto kplace = [&](int buf) { return lds + S::K0 + buf * S::TILE; };
+    auto vplace = [&](int buf) { return lds + S::V0 + buf * S::TILE; };
+    auto scale_to = [&](bool values, int buf) { return (float*)(lds + S::SCALES) + KT * (2 * values + buf); };
+    typename Tiles<S>::From vfrom = tl.where(pg, tl.page());
+    tl.ask(pg, vfrom, false, kplace(0));
+    tl.ask(pg, vfrom, true, vplace(0));
+    tl.settle(false, kplace(0), scale_to(false, 0));
+    tl.settle(true, vplace(0), scale_to(true, 0));
+    tl.step(pg, pl.div);
     if (tiles > 1) {
-      vfrom = where(tab[place.entry]);
-      ask(vfrom, false, 1);
-      settle(false, 1);
+      vfrom = tl.where(pg, tl.page());
+      tl.ask(pg, vfrom, false, kplace(1));
+      tl.settle(false, kplace(1), scale_to(false, 1));
     }
-    step();
-    int entry = tab[place.entry];
+    tl.step(pg, pl.div);
+    int page = tl.page();
 #pragma unroll
     for (int j = 0; j < KS; ++j) stay(q[j]);                   // here now: the loop must not wait for them, nor for what it asks for
     if constexpr (!S::I8) wait_loads<0>();
     __syncthreads();
-    f32x16 one[1], two[1];                                     // scores of a tile and of the next, in turn
+    f32x16 one[2], two[2];                                     // scores of a tile and of the next, in turn
     if (busy) {
-      one[0] = f32x16(0.f);
+      one[0] = one[1] = f32x16(0.f);
 #pragma unroll
-      for (int j = 0; j < KS; ++j) one[0] = Rows<32>::mfma(keys(0, j), q[j], one[0]);
+      for (int j = 0; j < NK; ++j) one[j / KS] = Rows<32>::mfma(keys(0, j), q[j % KS], one[j / KS]);
       adjust(piece.t0, 0, one);
-      run.follow(one, run.largest(one), c);
+      run.follow(one, Carry::largest(one), c);
     }
-    auto tile = [&](int i, int buf, f32x16 (&s)[1], f32x16 (&next)[1]) {     // buf: i & 1
+    auto tile = [&](int i, int buf, f32x16 (&s)[2], f32x16 (&next)[2]) {       // buf: i & 1
       const bool more = i + 1 < tiles;
       const int t = piece.t0 + i;
       if (i > 0) {
         // this tile's V and the next one's K are here; the K of this one and the V before it are used up
         if constexpr (S::I8) {
-          if (more) settle(false, buf ^ 1);
-          settle(true, buf);
+          if (more) tl.settle(false, kplace(buf ^ 1), scale_to(false, buf ^ 1));
+          tl.settle(true, vplace(buf), scale_to(true, buf));
         } else {
           wait_loads<0>();
         }
         __syncthreads();
       }
-      if (more) ask(vfrom, true, buf ^ 1);
+      if (more) tl.ask(pg, vfrom, true, vplace(buf ^ 1));
       if (i + 2 < tiles) {
-        vfrom = where(entry);
-        ask(vfrom, false, buf);
-        step();
-        entry = tab[place.entry];
+        vfrom = tl.where(pg, page);
+        tl.ask(pg, vfrom, false, kplace(buf));
+        tl.step(pg, pl.div);
+        page = tl.page();
       }
       if (!busy) return;
-      u32x4 p[2];
-      float mx;
-      scores_and_weigh(buf ^ 1, buf, next, s, p);              // after the last tile: of what lies there, for nothing
-      if constexpr (S::I8) {
-        run.times(s, (const float*)(lds + S::SCALES) + 32 * (2 + buf) + 4 * g);
-        if (masked(t)) run.mask(s, from - t * 32 - 4 * g, pos - t * 32 - 4 * g, 0.f);      // a scale that is not finite, not seen
-        run.pack(s, p);
-      }
+      scores_and_weigh(buf ^ 1, buf, next, s);                 // after the last tile: of what lies there, for nothing
       if (more) adjust(t + 1, buf ^ 1, next);
-      meet_and_largest(buf, p, next, mx);
-      if (!S::I8 && masked(t)) poisoned |= tile_not_finite<D>(lds + S::V0 + buf * S::TILE);
+      const float mx = meet_and_largest(buf, s, next);
+      if (masked(t)) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          poisoned |= S::I8 ? scales_not_finite(scale_to(true, buf) + 32 * x) : tile_not_finite<D>(vplace(buf) + 32 * x * S::RB);
+      }
       if (more) run.follow(next, mx, c);
     };
     for (int i = 0;;) {
@@ -795,7 +861,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
     }
   }
   if (__builtin_amdgcn_readfirstlane(poisoned)) {
-    rows_again<D>(a, pg, b, pl, n, hk, sq, r0 + 32 * rw, min(r0 + 32 * rw + 32, r0 + rows), piece.t0, piece.t1, 1,
+    rows_again<D, S::I8>(a, pg, b, pl, n, hk, sq, r0 + 32 * rw, min(r0 + 32 * rw + 32, r0 + rows), piece.t0 * (KT / 32), piece.t1 * (KT / 32), 1,
                   [&](int r, float m, float l, const float* y) {
       constexpr int C = D / 64;
       const int tk = r / G;
@@ -948,7 +1014,7 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
   typedef Few<D, 4, I8> F;
-  typedef Many<D, 4, 16, D == 256 ? 1 : 2, I8> M;
+  typedef Many<D, 4, 8, D == 256 ? 1 : 2, I8> M;
 };
 
 // LDS beyond what a kernel has unasked: asked for once on each device, and again where that failed.
