@@ -539,12 +539,12 @@ __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_page
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------
-// RW waves of 32 rows each share tiles of 64 keys, K and V twice in LDS, K a tile ahead of V.  A wave forms the scores of a tile while it
+// RW waves of 32 rows each share tiles of KT keys, K and V twice in LDS, K a tile ahead of V.  A wave forms the scores of a tile while it
 // takes the exponentials of the one before, and looks for their maximum while that one meets its values, so that its vector
 // instructions go in the shadow of its matrix instructions.  What bounds it then is the number of a wave's instructions.
 // Codes go through registers and into LDS as bf16.
-template <int D_, int RW_, int LEAST_, int EU_, bool I8_> struct Many {
-  static constexpr int D = D_, RW = RW_, EU = EU_, KT = 64, LEAST = LEAST_, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
+template <int D_, int RW_, int KT_, int EU_, bool I8_> struct Many {
+  static constexpr int D = D_, RW = RW_, EU = EU_, KT = KT_, X = KT / 32, LEAST = 512 / KT, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
   static constexpr bool I8 = I8_;
   static constexpr int RB = 2 * D, TILE = KT * RB;             // bytes in LDS
   static constexpr int K0 = 0, V0 = 2 * TILE, SCALES = 4 * TILE, LDS = SCALES + (I8 ? 4 * KT * 4 : 0);
@@ -665,7 +665,7 @@ template <class S> struct Tiles {
 template <class S>
 __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
                                           int hk, int split, int r0, const Seq& sq, float* part) {
-  constexpr int D = S::D, KT = S::KT, KS = D / 16, MB = D / 32;
+  constexpr int D = S::D, KT = S::KT, X = S::X, KS = D / 16, MB = D / 32;
   const int rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
   const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), pl.splits, split);
@@ -696,7 +696,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   for (int j = 0; j < KS; ++j) kat[j] = lds + S::K0 + (kread ^ (32 * j));
 #pragma unroll
   for (int j = 0; j < MB; ++j) vat[j] = lds + S::V0 + (vread ^ (64 * j));
-  constexpr int NK = 2 * KS, NV = 4 * MB;                      // operands of a tile: the j-th of
+  constexpr int NK = X * KS, NV = 2 * X * MB;                      // operands of a tile: the j-th of
   auto keys = [&](int buf, int j) { return lds_read16(kat[j % KS] + buf * S::TILE + j / KS * 32 * S::RB); };   // 32 keys by 16 channels
   auto values = [&](int buf, int j) {                                                                       // 32 channels by 16 keys
     const char* at = vat[j % MB] + buf * S::TILE + j / MB * 16 * S::RB;
@@ -705,9 +705,9 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   };
   auto scale_at = [&](bool values, int buf) { return (const float*)(lds + S::SCALES) + KT * (2 * values + buf) + 4 * g; };
   auto masked = [&](int t) { return t * KT + KT - 1 > first || t * KT < full; };
-  auto adjust = [&](int t, int buf, f32x16 (&s)[2]) {          // scores of tile t
+  auto adjust = [&](int t, int buf, f32x16 (&s)[X]) {          // scores of tile t
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < X; ++x) {
       if constexpr (S::I8) Carry::times(s[x], scale_at(false, buf) + 32 * x);
       if (masked(t)) Carry::mask(s[x], from - t * KT - 32 * x - 4 * g, pos - t * KT - 32 * x - 4 * g, -INFINITY);
     }
@@ -716,10 +716,10 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   // The order of what follows is kept as written (nothing moves over a sched_barrier): a matrix instruction with its share of vector
   // instructions, and the operand of the one AHEAD of it.  Weights go in pairs: the product in the exponent of one beside
   // the exponentials of the one before, and the rounding and the sum (of what was rounded) of the one before that.
-  constexpr int PAIRS = 16, EARLY = 8;                         // of a tile; those beside the next tile's scores
+  constexpr int PAIRS = 8 * X, EARLY = X == 1 ? 5 : 4 * X;      // of a tile; those beside the next scores, with all four of the first operand
   float ex[2], old[2], vs[2];
   uint32_t w[PAIRS];
-  auto exponent = [&](const f32x16 (&s)[2], int i) {
+  auto exponent = [&](const f32x16 (&s)[X], int i) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) { ex[e] = fmaf(s[i >> 3][2 * (i & 7) + e], c, -run.ref); stay(ex[e]); }
   };
@@ -733,7 +733,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
     }
     stay(w[i]);
   };
-  auto weigh = [&](const f32x16 (&s)[2], int buf, int lo, int hi) {            // pairs lo .. hi - 1; exponents of lo are there
+  auto weigh = [&](const f32x16 (&s)[X], int buf, int lo, int hi) {            // pairs lo .. hi - 1; exponents of lo are there
 #pragma unroll
     for (int i = lo; i < hi; ++i) {
       float f[2];
@@ -750,12 +750,13 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       }
     }
   };
-  auto scores_and_weigh = [&](int kbuf, int vbuf, f32x16 (&next)[2], const f32x16 (&s)[2]) {
+  auto scores_and_weigh = [&](int kbuf, int vbuf, f32x16 (&next)[X], const f32x16 (&s)[X]) {
     u32x4 k[NK];
 #pragma unroll
     for (int j = 0; j < S::AHEAD; ++j) k[j] = keys(kbuf, j);
     exponent(s, 0);
-    next[0] = next[1] = f32x16(0.f);
+#pragma unroll
+    for (int x = 0; x < X; ++x) next[x] = f32x16(0.f);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
@@ -765,7 +766,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto meet_and_largest = [&](int vbuf, const f32x16 (&s)[2], const f32x16 (&next)[2]) {
+  auto meet_and_largest = [&](int vbuf, const f32x16 (&s)[X], const f32x16 (&next)[X]) {
     u32x4 v[NV];
     float mx = next[0][0];
 #pragma unroll
@@ -774,15 +775,16 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (j + S::AHEAD < NV) v[j + S::AHEAD] = values(vbuf, j + S::AHEAD);
-      // the weights of the 16 keys j / MB are there: the last 8 pairs by the middle of the values, and a pair behind
+      // the weights of the 16 keys j / MB are there: the last pairs by the middle of the values, and a pair behind
       const u32x4 p = {w[4 * (j / MB)], w[4 * (j / MB) + 1], w[4 * (j / MB) + 2], w[4 * (j / MB) + 3]};
       run.o[j % MB] = Rows<32>::mfma(v[j], p, run.o[j % MB]);
-      if (j < 2 * MB) {
-        weigh(s, vbuf, EARLY + (PAIRS - EARLY) * j / (2 * MB), EARLY + (PAIRS - EARLY) * (j + 1) / (2 * MB));
-        if (j == 2 * MB - 1) finish(PAIRS - 1);
+      constexpr int H = NV / 2;
+      if (j < H) {
+        weigh(s, vbuf, EARLY + (PAIRS - EARLY) * j / H, EARLY + (PAIRS - EARLY) * (j + 1) / H);
+        if (j == H - 1) finish(PAIRS - 1);
       } else {
 #pragma unroll
-        for (int e = 32 * (j - 2 * MB) / (2 * MB); e < 32 * (j + 1 - 2 * MB) / (2 * MB); ++e) mx = fmaxf(mx, next[e >> 4][e & 15]);
+        for (int e = 16 * X * (j - H) / H; e < 16 * X * (j + 1 - H) / H; ++e) mx = fmaxf(mx, next[e >> 4][e & 15]);
         stay(mx);
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -814,15 +816,16 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
     for (int j = 0; j < KS; ++j) stay(q[j]);                   // here now: the loop must not wait for them, nor for what it asks for
     if constexpr (!S::I8) wait_loads<0>();
     __syncthreads();
-    f32x16 one[2], two[2];                                     // scores of a tile and of the next, in turn
+    f32x16 one[X], two[X];                                     // scores of a tile and of the next, in turn
     if (busy) {
-      one[0] = one[1] = f32x16(0.f);
+#pragma unroll
+      for (int x = 0; x < X; ++x) one[x] = f32x16(0.f);
 #pragma unroll
       for (int j = 0; j < NK; ++j) one[j / KS] = Rows<32>::mfma(keys(0, j), q[j % KS], one[j / KS]);
       adjust(piece.t0, 0, one);
       run.follow(one, Carry::largest(one), c);
     }
-    auto tile = [&](int i, int buf, f32x16 (&s)[2], f32x16 (&next)[2]) {       // buf: i & 1
+    auto tile = [&](int i, int buf, f32x16 (&s)[X], f32x16 (&next)[X]) {       // buf: i & 1
       const bool more = i + 1 < tiles;
       const int t = piece.t0 + i;
       if (i > 0) {
@@ -848,7 +851,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       const float mx = meet_and_largest(buf, s, next);
       if (masked(t)) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int x = 0; x < X; ++x)
           poisoned |= S::I8 ? scales_not_finite(scale_to(true, buf) + 32 * x) : tile_not_finite<D>(vplace(buf) + 32 * x * S::RB);
       }
       if (more) run.follow(next, mx, c);
@@ -1014,7 +1017,7 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
   typedef Few<D, 4, I8> F;
-  typedef Many<D, 4, 8, D == 256 ? 1 : 2, I8> M;
+  typedef Many<D, 4, D == 64 || (D == 128 && !I8) ? 64 : 32, D == 256 ? 1 : 2, I8> M;
 };
 
 // LDS beyond what a kernel has unasked: asked for once on each device, and again where that failed.
