@@ -28,11 +28,17 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) char lds_t;
 typedef const __attribute__((address_space(4))) int const_int;     // what no kernel of the call writes: scalar loads
 
+// What a call launches, from what the host knows.
 struct Plan {
-  int few, splits;         // rows up to which a sequence is the other kernel's (0: none); pieces of the keys at most
+  int few;                 // rows up to which a sequence is not taken as many
+  bool wide;               // few: up to 64, not 16
+  int few_tiles;           // row tiles of a sequence of few rows, at most
+  int few_splits, many_splits;           // pieces of its keys at most
+  int tiles;               // row tiles of the sequences of many rows, at most
+  int few_blocks, many_blocks;
   int G;
   PageDiv div;
-  float* work;
+  float *few_work, *many_work;
 };
 
 constexpr float GROWN = 8.f;
@@ -319,14 +325,16 @@ __device__ __forceinline__ void store1(const lq_attention& a, long long token, i
 // Up to 16 rows of a sequence (a token's heads): a wave takes all of them, the KW waves of a workgroup every KW-th tile of 32 keys,
 // each by itself: K and V of a tile have a place in LDS each, and the next tile's are asked for as soon as this one's are used, so
 // that 32 D .. 64 D elements a wave are on their way at any time.  Codes stay codes in LDS.
-template <int D_, int KW_, bool I8_> struct Few {
-  static constexpr int D = D_, KW = KW_, R = 16, ROWS = 16, KT = 32, LEAST = KW, THREADS = 64 * KW;
+template <int D_, int KW_, int NB_, bool I8_> struct Few {
+  static constexpr int D = D_, KW = KW_, NB = NB_, ROWS = 16 * NB, KT = 32, LEAST = KW, THREADS = 64 * KW;
   static constexpr bool I8 = I8_;
   static constexpr int ES = I8 ? 1 : 2, RB = D * ES, CPR = RB / 16, RPL = 64 / CPR;  // bytes and chunks of a row, rows of a load
   static constexpr int UNIT = KT * RB, LOADS = UNIT / 1024, SC = I8 ? 1 : 0;
   static constexpr int WAVE = 2 * UNIT + SC * 512;             // K, V, the scales of two tiles
-  static constexpr int JOIN = KW * ROWS * ((D + 4) * 4 + 8);
-  static constexpr int LDS = KW * WAVE > JOIN ? KW * WAVE : JOIN;
+  static constexpr int JOIN = KW * 16 * ((D + 4) * 4 + 8);
+  static constexpr int Q0 = KW * WAVE;                         // more than 16 rows: their queries
+  static constexpr int LDS0 = Q0 + (NB > 1 ? ROWS * D * 2 : 0), LDS = LDS0 > JOIN ? LDS0 : JOIN;
+  static __device__ __forceinline__ int place_q(int row) { return row & (D / 8 < 16 ? D / 8 - 1 : 15); }
   static constexpr int PART = ROWS * (D + 2);                  // floats of a workgroup's part of split keys
   // A chunk's place in its row, so that 256 bytes of the reads below go over all banks: 16 keys by a chunk of K; 8 keys by two chunks
   // of V, or, codes, 16 keys (of which 8 neighbours and those 16 on) by one.
@@ -340,13 +348,18 @@ template <int D_, int KW_, bool I8_> struct Few {
 template <class S>
 __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
                                          int hk, int split, int splits, int r0, const Seq& sq, float* part) {
-  constexpr int D = S::D, KW = S::KW, MB = D / 16, KS = D / 32;
+  constexpr int D = S::D, KW = S::KW, NB = S::NB, MB = D / 16, KS = D / 32;
   const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
   const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), splits, split);
   if (split >= piece.pieces) return;
-  const int rc = r0 + min(col, rows - 1), tok = rc / G, pos = sq.pos0 + tok;
-  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;              // keys from .. pos are seen
+  int rc[NB], pos[NB], from[NB];                               // rows 16 nb + col; keys from .. pos are seen
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    rc[nb] = r0 + min(16 * nb + col, rows - 1);
+    pos[nb] = sq.pos0 + rc[nb] / G;
+    from[nb] = a.window > 0 ? max(pos[nb] - a.window + 1, 0) : 0;
+  }
   const int first = sq.pos0 + r0 / G, last = sq.pos0 + (r0 + rows - 1) / G;    // all rows see full .. first
   const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;
 
@@ -387,23 +400,38 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
   };
 
   const float c = a.scale * LOG2E;
-  Run<16, D> run;
-  run.start();
+  Run<16, D> run[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) run[nb].start();
   bool poisoned = false;
   int t = piece.t0 + kw;
-  if (t < piece.t1) {
-    u32x4 q[KS];
-    {
-      const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + rc - tok * G) * a.q.hd + 8 * g;
+  u32x4 q[KS];
+  if constexpr (NB == 1) {
+    const int tok = pos[0] - sq.pos0;
+    const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + rc[0] - tok * G) * a.q.hd + 8 * g;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 32 * s);
-    }
+    for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 32 * s);
+  }
+  if (t < piece.t1) {
     places(t);
     ask_scales(0);
     ask(false);
     ask(true);
+  }
+  if constexpr (NB > 1) {
+    for (int x = threadIdx.x; x < S::ROWS * (D / 8); x += S::THREADS) {
+      const int r = x / (D / 8), ch = x % (D / 8), at = r0 + min(r, rows - 1), tok = at / G;
+      const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + at - tok * G) * a.q.hd;
+      *(u32x4*)(lds + S::Q0 + 2 * D * r + 16 * (ch ^ S::place_q(r))) = *(const u32x4*)(p + 8 * ch);
+    }
+    __syncthreads();
+  } else {
 #pragma unroll
     for (int s = 0; s < KS; ++s) stay(q[s]);                   // here now: the loop must not wait for them, nor for what it asks for
+  }
+  if (t < piece.t1) {
+    // the chunks of queries of this lane's rows, the i-th step's at ^ 64 i
+    const int qread = S::Q0 + 2 * D * col + 16 * (g ^ S::place_q(col));
     // this lane's reads: 8 channels of two keys; 4 (8) keys by 16 channels a group of 16 lanes
     const int kread = col * S::RB + (S::I8 ? ((g >> 1) ^ S::place_k(col)) * 16 + 8 * (g & 1) : (g ^ S::place_k(col)) * 16);
     const int vkey = S::I8 ? 4 * g + ((lane & 15) >> 1 & 3) + 16 * ((lane & 15) >> 3) : 4 * g + ((lane & 15) >> 2);
@@ -413,10 +441,11 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
       const float* sc = (const float*)(mine + 2 * S::UNIT + 256 * odd) + 4 * g;
       if (more) places(t + KW);
       wait_loads<S::LOADS>();                                  // K is here, V may be on its way
-      f32x4 s[2];
+      f32x4 s[NB][2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        s[x] = f32x4(0.f);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) s[nb][x] = f32x4(0.f);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           u32x4 k;
@@ -427,12 +456,14 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           } else {
             k = lds_read16(mine + 16 * x * S::RB + (kread ^ (64 * i)));
           }
-          s[x] = Rows<16>::mfma(k, q[i], s[x]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) s[nb][x] = Rows<16>::mfma(k, NB == 1 ? q[i] : lds_read16(lds + 32 * D * nb + (qread ^ (64 * i))), s[nb][x]);
+          if (NB > 1) __builtin_amdgcn_sched_barrier(0);       // operands a step at a time: registers
         }
       }
       if constexpr (S::I8) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) run.times(s[x], sc + 16 * x);
+        for (int x = 0; x < 2 * NB; ++x) Run<16, D>::times(s[x >> 1][x & 1], sc + 16 * (x & 1));
       }
       if (more) {
         wait_lds();
@@ -441,22 +472,25 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
       }
       const int k0 = 32 * t;
       const bool masked = k0 + 31 > first || k0 < full;
-      if (masked) {
+      u32x4 p[NB];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) run.mask(s[x], from - k0 - 16 * x - 4 * g, pos - k0 - 16 * x - 4 * g, -INFINITY);
-      }
-      run.follow(s, run.largest(s), c);
-      u32x4 p;
+      for (int nb = 0; nb < NB; ++nb) {
+        if (masked) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[x][e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], c, -run.ref));
-          run.l += s[x][e];
+          for (int x = 0; x < 2; ++x) Run<16, D>::mask(s[nb][x], from[nb] - k0 - 16 * x - 4 * g, pos[nb] - k0 - 16 * x - 4 * g, -INFINITY);
         }
-        if constexpr (S::I8) run.times(s[x], sc + 32 + 16 * x);
-        p[2 * x] = pk_bf16(s[x][0], s[x][1]);
-        p[2 * x + 1] = pk_bf16(s[x][2], s[x][3]);
+        run[nb].follow(s[nb], Run<16, D>::largest(s[nb]), c);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[nb][x][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][x][e], c, -run[nb].ref));
+            run[nb].l += s[nb][x][e];
+          }
+          if constexpr (S::I8) Run<16, D>::times(s[nb][x], sc + 32 + 16 * x);
+          p[nb][2 * x] = pk_bf16(s[nb][x][0], s[nb][x][1]);
+          p[nb][2 * x + 1] = pk_bf16(s[nb][x][2], s[nb][x][3]);
+        }
       }
       if (more) wait_loads<S::LOADS + S::SC>();                // V is here
       else wait_loads<0>();
@@ -472,7 +506,9 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           const u32x2 x = lds_read_tr(V + (vread ^ (32 * i))), y = lds_read_tr(V + 16 * S::RB + (vread ^ (32 * i)));
           v = u32x4{x[0], x[1], y[0], y[1]};
         }
-        run.o[i] = Rows<16>::mfma(v, p, run.o[i]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) run[nb].o[i] = Rows<16>::mfma(v, p[nb], run[nb].o[i]);
+        if (NB > 1) __builtin_amdgcn_sched_barrier(0);
       }
       if (masked) poisoned |= S::I8 ? scales_not_finite(sc - 4 * g + 32) : tile_not_finite<D>(V);
       if (more) {
@@ -480,62 +516,73 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
         ask(true);
       }
     }
-    run.l = Rows<16>::sum_over(run.l);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) run[nb].l = Rows<16>::sum_over(run[nb].l);
   }
 
-  // the waves' parts of a row, joined through LDS
-  float* jo = (float*)lds;                                     // [KW][ROWS][D + 4]
-  float* jm = jo + KW * S::ROWS * (D + 4);                     // [KW][ROWS] maxima, then sums
-  __syncthreads();
-  if (!poisoned) {
-    float* to = jo + (kw * S::ROWS + col) * (D + 4) + 4 * g;
+  // the waves' parts of a row, joined through LDS, 16 rows at a time
+  float* jo = (float*)lds;                                     // [KW][16][D + 4]
+  float* jm = jo + KW * 16 * (D + 4);                          // [KW][16] maxima, then sums
 #pragma unroll
-    for (int i = 0; i < MB; ++i) *(f32x4*)(to + 16 * i) = run.o[i];
-    if (g == 0) { jm[kw * S::ROWS + col] = run.m; jm[(KW + kw) * S::ROWS + col] = run.l; }
-  } else {
-    rows_again<D, S::I8>(a, pg, b, pl, n, hk, sq, r0, r0 + rows, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
-      constexpr int C = D / 64;
+  for (int nb = 0; nb < NB; ++nb) {
+    const int ra = r0 + 16 * nb, here = min(16, rows - 16 * nb);
+    if (here <= 0) break;
+    __syncthreads();
+    if (!poisoned) {
+      float* to = jo + (kw * 16 + col) * (D + 4) + 4 * g;
 #pragma unroll
-      for (int e = 0; e < C; ++e) jo[(kw * S::ROWS + r - r0) * (D + 4) + C * lane + e] = y[e];
-      if (lane == 0) { jm[kw * S::ROWS + r - r0] = m; jm[(KW + kw) * S::ROWS + r - r0] = l; }
-    });
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < rows * (D / 4); x += S::THREADS) {
-    const int rr = x / (D / 4), d = 4 * (x % (D / 4));
-    float M = -INFINITY, L = 0.f;
-    f32x4 y = f32x4(0.f);
+      for (int i = 0; i < MB; ++i) *(f32x4*)(to + 16 * i) = run[nb].o[i];
+      if (g == 0) { jm[kw * 16 + col] = run[nb].m; jm[(KW + kw) * 16 + col] = run[nb].l; }
+    } else {
+      rows_again<D, S::I8>(a, pg, b, pl, n, hk, sq, ra, ra + here, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
+        constexpr int C = D / 64;
 #pragma unroll
-    for (int k = 0; k < KW; ++k) M = fmaxf(M, jm[k * S::ROWS + rr]);
-#pragma unroll
-    for (int k = 0; k < KW; ++k) {
-      const float mk = jm[k * S::ROWS + rr], w = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * c);
-      L = fmaf(w, jm[(KW + k) * S::ROWS + rr], L);             // a wave without a maximum: zeros, or NaN
-      y += w * *(const f32x4*)(jo + (k * S::ROWS + rr) * (D + 4) + d);
+        for (int e = 0; e < C; ++e) jo[(kw * 16 + r - ra) * (D + 4) + C * lane + e] = y[e];
+        if (lane == 0) { jm[kw * 16 + r - ra] = m; jm[(KW + kw) * 16 + r - ra] = l; }
+      });
     }
-    if (piece.pieces > 1) {
-      *(f32x4*)(part + rr * D + d) = y;
-      if (d == 0) { part[S::ROWS * D + rr] = M; part[S::ROWS * (D + 1) + rr] = L; }
-      continue;
+    __syncthreads();
+    for (int x = threadIdx.x; x < here * (D / 4); x += S::THREADS) {
+      const int rr = x / (D / 4), d = 4 * (x % (D / 4));
+      float M = -INFINITY, L = 0.f;
+      f32x4 y = f32x4(0.f);
+#pragma unroll
+      for (int k = 0; k < KW; ++k) M = fmaxf(M, jm[k * 16 + rr]);
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const float mk = jm[k * 16 + rr], w = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * c);
+        L = fmaf(w, jm[(KW + k) * 16 + rr], L);             // a wave without a maximum: zeros, or NaN
+        y += w * *(const f32x4*)(jo + (k * 16 + rr) * (D + 4) + d);
+      }
+      if (piece.pieces > 1) {
+        *(f32x4*)(part + (16 * nb + rr) * D + d) = y;
+        if (d == 0) { part[S::ROWS * D + 16 * nb + rr] = M; part[S::ROWS * (D + 1) + 16 * nb + rr] = L; }
+        continue;
+      }
+      const int tk = (ra + rr) / G;
+      store4(a, sq.lo + tk, hk * G + (ra + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
     }
-    const int tk = (r0 + rr) / G;
-    store4(a, sq.lo + tk, hk * G + (r0 + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
   }
 }
 
-// workgroup (split, sequence, head)
+// workgroup `block` = (split, row tile, sequence, head)
 template <class S>
-__global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int item = blockIdx.x % (b.N * pg.HK), split = blockIdx.x / (b.N * pg.HK), n = item / pg.HK, hk = item % pg.HK;
+__device__ __forceinline__ void few_block(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int block) {
+  const int items = b.N * pg.HK * pl.few_tiles, item = block % items, split = block / items, hk = item % pg.HK;
+  const int tile = item / (b.N * pg.HK), n = item / pg.HK - tile * b.N;
   const Seq sq = sequence(b, pg, pl.G, n);
-  if (sq.rows <= 0 || (pl.few && sq.rows > pl.few)) return;
-  // more rows than a tile has, where no other launch takes them: one workgroup all of them, a tile after the other
-  const int splits = sq.rows > S::ROWS ? 1 : pl.splits;
-  for (int r0 = 0; r0 < sq.rows; r0 += S::ROWS) {
-    few_rows<S>(a, pg, b, pl, lds, n, hk, split, splits, r0, sq, pl.work + (long long)blockIdx.x * S::PART);
+  if (sq.rows <= 0 || (pl.many_blocks && sq.rows > S::ROWS)) return;
+  // more rows than the host said: a workgroup every few_tiles-th tile, all keys
+  const int step = S::ROWS * pl.few_tiles, splits = sq.rows > step ? 1 : pl.few_splits;
+  for (int r0 = S::ROWS * tile; r0 < sq.rows; r0 += step) {
+    few_rows<S>(a, pg, b, pl, lds, n, hk, split, splits, r0, sq, pl.few_work + (long long)block * S::PART);
     __syncthreads();
   }
+}
+template <class S>
+__global__ __launch_bounds__(S::THREADS, S::NB > 1 && S::D > 64 ? 1 : 2) void few_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  few_block<S>(a, pg, b, pl, lds, blockIdx.x);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------
@@ -668,7 +715,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   constexpr int D = S::D, KT = S::KT, X = S::X, KS = D / 16, MB = D / 32;
   const int rw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, g = lane >> 5;
   const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
-  const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), pl.splits, split);
+  const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), pl.many_splits, split);
   if (split >= piece.pieces) return;
   const int row = r0 + 32 * rw + col, rc = min(row, r0 + rows - 1), tok = rc / G, pos = sq.pos0 + tok, head = hk * G + rc - tok * G;
   const bool busy = 32 * rw < rows;                            // the wave has rows
@@ -923,9 +970,8 @@ template <int ROWS> __device__ __forceinline__ RowTile row_tile(const lq_batch& 
 // Workgroups go to the XCDs in turn: a head of the cache stays on one of them (or on 8 / HK), whose L2 then holds its tiles.
 // The last row tiles, which see the most keys, come first.
 template <class S>
-__global__ __launch_bounds__(S::THREADS) __attribute__((amdgpu_waves_per_eu(S::EU, S::EU))) void many_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl, int tiles) {
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int per = tiles * pg.HK, split = blockIdx.x / per, x = blockIdx.x % per;
+__device__ __forceinline__ void many_block(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int block) {
+  const int per = pl.tiles * pg.HK, split = block / per, x = block % per;
   int hk, number;
   if (pg.HK < 8 && 8 % pg.HK == 0 && per % 8 == 0) {
     const int share = 8 / pg.HK;
@@ -935,33 +981,53 @@ __global__ __launch_bounds__(S::THREADS) __attribute__((amdgpu_waves_per_eu(S::E
     hk = x % pg.HK;
     number = x / pg.HK;
   }
-  number = tiles - 1 - number;
+  number = pl.tiles - 1 - number;
   const RowTile rt = row_tile<S::ROWS>(b, pl.G, number);
   const Seq sq = sequence(b, pg, pl.G, rt.n);
   if (rt.r0 >= sq.rows || sq.rows <= pl.few) return;
-  many_rows<S>(a, pg, b, pl, lds, rt.n, hk, split, rt.r0, sq, pl.work + ((long long)split * per + (long long)number * pg.HK + hk) * S::PART);
+  many_rows<S>(a, pg, b, pl, lds, rt.n, hk, split, rt.r0, sq, pl.many_work + ((long long)split * per + (long long)number * pg.HK + hk) * S::PART);
+}
+template <class S>
+__global__ __launch_bounds__(S::THREADS) __attribute__((amdgpu_waves_per_eu(S::EU, S::EU)))
+void many_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  many_block<S>(a, pg, b, pl, lds, blockIdx.x);
+}
+
+// Both kinds of sequences in one launch, eight workgroups of one kind and eight of the other in turn while both last: those of few
+// rows, which wait for memory, beside those of many, which compute.
+template <class F, class M>
+__global__ __launch_bounds__(M::THREADS) __attribute__((amdgpu_waves_per_eu(M::EU, M::EU)))
+void both_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
+  static_assert(F::THREADS == M::THREADS);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int x = blockIdx.x, turns = 8 * (min(pl.few_blocks, pl.many_blocks) / 8);
+  const bool many = x < 2 * turns ? !(x & 8) : pl.many_blocks > turns && x - turns < pl.many_blocks;
+  const int block = x < 2 * turns ? (x >> 4) * 8 + (x & 7) : many ? x - turns : x - (pl.many_blocks > turns ? pl.many_blocks : turns);
+  if (many) many_block<M>(a, pg, b, pl, lds, block);
+  else few_block<F>(a, pg, b, pl, lds, block);
 }
 
 // ---- the pieces of split keys, joined -----------------------------------------------------------------------------------
 // A row's D / 4 threads take 4 channels each; P of them share out the pieces of a row.
 template <class S, bool FEW, int P>
-__global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl, int tiles) {
+__device__ __forceinline__ void join_block(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, float* lds, int block) {
   constexpr int D = S::D, ROWS = S::ROWS, C = D / 4, PER = 256 / (C * P);      // rows of a workgroup
   static_assert(PER >= 1 && ROWS % PER == 0, "rows of a workgroup");
-  __shared__ float lds[P > 1 ? 256 * 4 + 2 * P * PER : 1];
-  const int item = blockIdx.x / (ROWS / PER), rr = (blockIdx.x % (ROWS / PER)) * PER + threadIdx.x / (C * P);
+  const int item = block / (ROWS / PER), rr = (block % (ROWS / PER)) * PER + threadIdx.x / (C * P);
   const int hk = item % pg.HK, number = item / pg.HK;
-  RowTile rt = {number, 0};
+  RowTile rt = {number % b.N, number / b.N * ROWS};
   if (!FEW) rt = row_tile<ROWS>(b, pl.G, number);
   const Seq sq = sequence(b, pg, pl.G, rt.n);
-  if (FEW ? sq.rows <= 0 || sq.rows > ROWS : rt.r0 >= sq.rows || sq.rows <= pl.few) return;
+  if (rt.r0 >= sq.rows || (FEW ? sq.rows > ROWS * pl.few_tiles : sq.rows <= pl.few)) return;
   const int rows = min(ROWS, sq.rows - rt.r0);
-  if ((blockIdx.x % (ROWS / PER)) * PER >= rows) return;
-  const Piece piece = piece_of<S>(keys_of(sq, pl.G, rt.r0, rt.r0 + rows, a.window), pl.splits, 0);
+  if ((block % (ROWS / PER)) * PER >= rows) return;
+  const int splits = FEW ? pl.few_splits : pl.many_splits;
+  const Piece piece = piece_of<S>(keys_of(sq, pl.G, rt.r0, rt.r0 + rows, a.window), splits, 0);
   if (piece.pieces == 1) return;
   const int which = (threadIdx.x / C) % P, d = 4 * (threadIdx.x % C);
-  const long long step = (long long)tiles * pg.HK * S::PART;
-  const float* part = pl.work + (long long)item * S::PART;
+  const long long step = (long long)(FEW ? b.N * pl.few_tiles : pl.tiles) * pg.HK * S::PART;
+  const float* part = (FEW ? pl.few_work : pl.many_work) + (long long)item * S::PART;
   const float c = a.scale * LOG2E;
   float M = -INFINITY, L = 0.f;
   f32x4 y = f32x4(0.f);
@@ -1014,97 +1080,107 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
   store4(a, sq.lo + tk, hk * pl.G + (rt.r0 + rr - tk * pl.G), d, y * (L == 0.f ? 0.f : 1.f / L));
 }
 
+template <class F, class M, int P>
+__global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl, int few_blocks) {
+  __shared__ float lds[P > 1 ? 256 * 4 + 2 * 256 / (F::D / 4) : 1];
+  if ((int)blockIdx.x < few_blocks) join_block<F, true, P>(a, pg, b, pl, lds, blockIdx.x);
+  else join_block<M, false, P>(a, pg, b, pl, lds, blockIdx.x - few_blocks);
+}
+
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
-  typedef Few<D, 4, I8> F;
+  typedef Few<D, 4, 1, I8> F;
+  typedef Few<D, 4, D == 256 ? 2 : 4, I8> W;
   typedef Many<D, 4, D == 64 || (D == 128 && !I8) ? 64 : 32, D == 256 ? 1 : 2, I8> M;
 };
 
 // LDS beyond what a kernel has unasked: asked for once on each device, and again where that failed.
-template <class S, bool FEW> bool lds_asked() {
+template <auto* KERNEL, int LDS> bool lds_asked() {
   static std::atomic<bool> had[64];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return false;
   const bool known = dev >= 0 && dev < 64;
   if (known && had[dev].load(std::memory_order_relaxed)) return true;
-  const void* f;
-  if constexpr (FEW) f = (const void*)few_kernel<S>;
-  else f = (const void*)many_kernel<S>;
-  if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS) != hipSuccess) return false;
+  if (hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess) return false;
   if (known) had[dev].store(true, std::memory_order_relaxed);
   return true;
 }
 
-// What a call launches, from what the host knows: sizes, and the longest sequence's tokens where the caller says.
-struct Calls {
-  bool few, many;          // which kernels
-  int few_splits, many_splits, tiles;
-  long long few_work, many_work;     // floats
-};
-template <int D, bool I8> Calls calls(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest) {
+// Sizes and the longest sequence's tokens, where the caller says them, settle what a call launches and how the keys are split.
+template <int D, bool I8> Plan plan_of(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest) {
   typedef typename Shapes<D, I8>::F F;
+  typedef typename Shapes<D, I8>::W W;
   typedef typename Shapes<D, I8>::M M;
-  const long long G = a->HQ / p->HK, cus = lq_attn_cus();
-  const long long most = longest > 0 && longest < b->T ? longest : b->T;
-  Calls c = {};
-  c.few = most * G <= F::ROWS || b->N > 1;
-  c.many = most * G > F::ROWS;
-  c.tiles = (int)((long long)b->T * G / M::ROWS + b->N);
-  const long long reach = (long long)b->width * p->page;       // the longest context
-  auto pieces = [&](long long target, long long items, int least) {
-    const long long by = (target + items - 1) / items, cap = reach / least;
+  Plan c = {};
+  c.G = a->HQ / p->HK;
+  c.div = page_div(p->page);
+  const long long cus = lq_attn_cus(), most = longest > 0 && longest < b->T ? longest : b->T, rows = most * c.G;
+  const bool many = rows > 64, few = !many || b->N > 1;
+  c.wide = !many && rows > F::ROWS;
+  c.few = few ? F::ROWS : 0;
+  c.few_tiles = c.wide ? (int)((rows + W::ROWS - 1) / W::ROWS) : 1;
+  c.tiles = many ? (int)((long long)b->T * c.G / M::ROWS + b->N) : 0;
+  // keys that a row tile sees at most; under a window of its rows' tokens
+  auto reach = [&](int tile) {
+    const long long all = (long long)b->width * p->page, near = (long long)a->window + (tile - 1) / c.G + 1;
+    return a->window > 0 && near < all ? near : all;
+  };
+  auto pieces = [&](long long target, long long items, long long keys, int least) {
+    const long long by = (target + items - 1) / items, cap = keys / least;
     return (int)(by < 1 || cap < 2 ? 1 : by < cap ? (by < 256 ? by : 256) : (cap < 256 ? cap : 256));
   };
-  const long long fi = (long long)b->N * p->HK, mi = (long long)c.tiles * p->HK;
-  c.few_splits = c.few ? pieces(4 * cus, fi, F::LEAST * F::KT) : 1;
-  c.many_splits = c.many && mi < 2 * cus ? pieces(2 * cus, mi, M::LEAST * M::KT) : 1;
-  c.few_work = c.few_splits > 1 ? c.few_splits * fi * F::PART : 0;
-  c.many_work = c.many_splits > 1 ? c.many_splits * mi * M::PART : 0;
+  const long long fi = (long long)b->N * p->HK * c.few_tiles, mi = (long long)c.tiles * p->HK;
+  c.few_splits = few ? pieces((many ? 2 : 8) * cus, fi, reach(c.wide ? W::ROWS : F::ROWS), F::LEAST * F::KT) : 1;
+  c.many_splits = many && mi < 2 * cus ? pieces(2 * cus, mi, reach(M::ROWS), M::LEAST * M::KT) : 1;
+  c.few_blocks = few ? (int)(fi * c.few_splits) : 0;
+  c.many_blocks = (int)(mi * c.many_splits);
   return c;
+}
+template <int D, bool I8> long long few_floats(const Plan& c) {
+  return c.few_splits > 1 ? (long long)c.few_blocks * (c.wide ? Shapes<D, I8>::W::PART : Shapes<D, I8>::F::PART) : 0;
+}
+template <int D, bool I8> long long many_floats(const Plan& c) {
+  return c.many_splits > 1 ? (long long)c.many_blocks * Shapes<D, I8>::M::PART : 0;
 }
 
 // four groups of threads a row where there are pieces enough for them
-template <class S, bool FEW> void join(const lq_attention* a, const lq_pages* p, const lq_batch* b, const Plan& pl, int tiles, hipStream_t s) {
-  const unsigned items = (unsigned)(tiles * p->HK);
-  constexpr int per = 256 / (S::D / 4);
-  if (pl.splits > 8) join_kernel<S, FEW, 4><<<items * (S::ROWS / (per / 4)), 256, 0, s>>>(*a, *p, *b, pl, tiles);
-  else join_kernel<S, FEW, 1><<<items * (S::ROWS / per), 256, 0, s>>>(*a, *p, *b, pl, tiles);
+template <class F, class M>
+int join(const lq_attention* a, const lq_pages* p, const lq_batch* b, const Plan& pl, hipStream_t s) {
+  if (pl.few_splits == 1 && pl.many_splits == 1) return LQ_OK;
+  const int P = pl.few_splits > 8 || pl.many_splits > 8 ? 4 : 1, per = 256 / (F::D / 4 * P);
+  const int few = pl.few_splits > 1 ? b->N * p->HK * pl.few_tiles * (F::ROWS / per) : 0;
+  const int many = pl.many_splits > 1 ? pl.tiles * p->HK * (M::ROWS / per) : 0;
+  const unsigned blocks = (unsigned)few + (unsigned)many;
+  if (P == 4) join_kernel<F, M, 4><<<blocks, 256, 0, s>>>(*a, *p, *b, pl, few);
+  else join_kernel<F, M, 1><<<blocks, 256, 0, s>>>(*a, *p, *b, pl, few);
+  return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
 }
 
 template <int D, bool I8>
 int go(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest, float* work, hipStream_t s) {
   typedef typename Shapes<D, I8>::F F;
+  typedef typename Shapes<D, I8>::W W;
   typedef typename Shapes<D, I8>::M M;
-  const Calls c = calls<D, I8>(a, p, b, longest);
-  Plan pl = {};
-  pl.G = a->HQ / p->HK;
-  pl.div = page_div(p->page);
-  const int fi = b->N * p->HK, mi = c.tiles * p->HK;
-  if (c.few) {
-    if (!lds_asked<F, true>()) return LQ_ERR_HIP;
-    pl.few = c.many ? F::ROWS : 0;
-    pl.splits = c.few_splits;
-    pl.work = work;
-    few_kernel<F><<<(unsigned)(fi * c.few_splits), F::THREADS, F::LDS, s>>>(*a, *p, *b, pl);
-    if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
-    if (c.few_splits > 1) {
-      join<F, true>(a, p, b, pl, b->N, s);
-      if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
-    }
+  Plan pl = plan_of<D, I8>(a, p, b, longest);
+  pl.few_work = work;
+  pl.many_work = work + few_floats<D, I8>(pl);
+  const unsigned blocks = (unsigned)pl.few_blocks + (unsigned)pl.many_blocks;
+  if (pl.wide) {
+    if (!lds_asked<few_kernel<W>, W::LDS>()) return LQ_ERR_HIP;
+    few_kernel<W><<<blocks, W::THREADS, W::LDS, s>>>(*a, *p, *b, pl);
+  } else if (!pl.many_blocks) {
+    if (!lds_asked<few_kernel<F>, F::LDS>()) return LQ_ERR_HIP;
+    few_kernel<F><<<blocks, F::THREADS, F::LDS, s>>>(*a, *p, *b, pl);
+  } else if (!pl.few_blocks) {
+    if (!lds_asked<many_kernel<M>, M::LDS>()) return LQ_ERR_HIP;
+    many_kernel<M><<<blocks, M::THREADS, M::LDS, s>>>(*a, *p, *b, pl);
+  } else {
+    constexpr int LDS = F::LDS > M::LDS ? F::LDS : M::LDS;
+    if (!lds_asked<both_kernel<F, M>, LDS>()) return LQ_ERR_HIP;
+    both_kernel<F, M><<<blocks, M::THREADS, LDS, s>>>(*a, *p, *b, pl);
   }
-  if (c.many) {
-    if (!lds_asked<M, false>()) return LQ_ERR_HIP;
-    pl.few = c.few ? F::ROWS : 0;
-    pl.splits = c.many_splits;
-    pl.work = work + c.few_work;
-    many_kernel<M><<<(unsigned)(mi * c.many_splits), M::THREADS, M::LDS, s>>>(*a, *p, *b, pl, c.tiles);
-    if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
-    if (c.many_splits > 1) {
-      join<M, false>(a, p, b, pl, c.tiles, s);
-      if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
-    }
-  }
-  return LQ_OK;
+  if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
+  return pl.wide ? join<W, M>(a, p, b, pl, s) : join<F, M>(a, p, b, pl, s);
 }
 
 template <typename F> auto by_shape(const lq_pages* p, F f) {
@@ -1131,8 +1207,10 @@ extern "C" long long lq_attend_workspace(const lq_attention* a, const lq_pages* 
   if (int rc = check(a, p, b, longest)) return rc;
   if (b->N == 0 || b->T == 0) return 0;
   return by_shape(p, [&](auto d, auto i8) {
-    const Calls c = calls<decltype(d)::value, decltype(i8)::value>(a, p, b, longest);
-    return 4 * (c.few_work + c.many_work);
+    constexpr int D = decltype(d)::value;
+    constexpr bool I8 = decltype(i8)::value;
+    const Plan c = plan_of<D, I8>(a, p, b, longest);
+    return 4 * (few_floats<D, I8>(c) + many_floats<D, I8>(c));
   });
 }
 
