@@ -13,6 +13,7 @@
 //
 // Tiles go from the pages straight into LDS, a tile ahead, in swizzled places: both kinds of reads then spread over all banks.
 // Codes of 8 bits go through registers and into LDS as bf16, which holds them exactly; their scales enter S and P in fp32.
+#include <algorithm>
 #include <atomic>
 
 #include "lq_attn.h"
@@ -31,8 +32,6 @@ typedef const __attribute__((address_space(4))) int const_int;     // what no ke
 // What a call launches, from what the host knows.
 struct Plan {
   int few;                 // rows up to which a sequence is not taken as many
-  bool wide;               // few: up to 64, not 16
-  int few_tiles;           // row tiles of a sequence of few rows, at most
   int few_splits, many_splits;           // pieces of its keys at most
   int tiles;               // row tiles of the sequences of many rows, at most
   int few_blocks, many_blocks;
@@ -325,16 +324,14 @@ __device__ __forceinline__ void store1(const lq_attention& a, long long token, i
 // Up to 16 rows of a sequence (a token's heads): a wave takes all of them, the KW waves of a workgroup every KW-th tile of 32 keys,
 // each by itself: K and V of a tile have a place in LDS each, and the next tile's are asked for as soon as this one's are used, so
 // that 32 D .. 64 D elements a wave are on their way at any time.  Codes stay codes in LDS.
-template <int D_, int KW_, int NB_, bool I8_> struct Few {
-  static constexpr int D = D_, KW = KW_, NB = NB_, ROWS = 16 * NB, KT = 32, LEAST = KW, THREADS = 64 * KW;
+template <int D_, int KW_, bool I8_> struct Few {
+  static constexpr int D = D_, KW = KW_, R = 16, ROWS = 16, KT = 32, LEAST = KW, THREADS = 64 * KW;
   static constexpr bool I8 = I8_;
   static constexpr int ES = I8 ? 1 : 2, RB = D * ES, CPR = RB / 16, RPL = 64 / CPR;  // bytes and chunks of a row, rows of a load
   static constexpr int UNIT = KT * RB, LOADS = UNIT / 1024, SC = I8 ? 1 : 0;
   static constexpr int WAVE = 2 * UNIT + SC * 512;             // K, V, the scales of two tiles
-  static constexpr int JOIN = KW * 16 * ((D + 4) * 4 + 8);
-  static constexpr int Q0 = KW * WAVE;                         // more than 16 rows: their queries
-  static constexpr int LDS0 = Q0 + (NB > 1 ? ROWS * D * 2 : 0), LDS = LDS0 > JOIN ? LDS0 : JOIN;
-  static __device__ __forceinline__ int place_q(int row) { return row & (D / 8 < 16 ? D / 8 - 1 : 15); }
+  static constexpr int JOIN = KW * ROWS * ((D + 4) * 4 + 8);
+  static constexpr int LDS = KW * WAVE > JOIN ? KW * WAVE : JOIN;
   static constexpr int PART = ROWS * (D + 2);                  // floats of a workgroup's part of split keys
   // A chunk's place in its row, so that 256 bytes of the reads below go over all banks: 16 keys by a chunk of K; 8 keys by two chunks
   // of V, or, codes, 16 keys (of which 8 neighbours and those 16 on) by one.
@@ -348,18 +345,13 @@ template <int D_, int KW_, int NB_, bool I8_> struct Few {
 template <class S>
 __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int n,
                                          int hk, int split, int splits, int r0, const Seq& sq, float* part) {
-  constexpr int D = S::D, KW = S::KW, NB = S::NB, MB = D / 16, KS = D / 32;
+  constexpr int D = S::D, KW = S::KW, MB = D / 16, KS = D / 32;
   const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int G = pl.G, rows = min(S::ROWS, sq.rows - r0);
   const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), splits, split);
   if (split >= piece.pieces) return;
-  int rc[NB], pos[NB], from[NB];                               // rows 16 nb + col; keys from .. pos are seen
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    rc[nb] = r0 + min(16 * nb + col, rows - 1);
-    pos[nb] = sq.pos0 + rc[nb] / G;
-    from[nb] = a.window > 0 ? max(pos[nb] - a.window + 1, 0) : 0;
-  }
+  const int rc = r0 + min(col, rows - 1), tok = rc / G, pos = sq.pos0 + tok;
+  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;              // keys from .. pos are seen
   const int first = sq.pos0 + r0 / G, last = sq.pos0 + (r0 + rows - 1) / G;    // all rows see full .. first
   const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;
 
@@ -400,38 +392,23 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
   };
 
   const float c = a.scale * LOG2E;
-  Run<16, D> run[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb) run[nb].start();
+  Run<16, D> run;
+  run.start();
   bool poisoned = false;
   int t = piece.t0 + kw;
-  u32x4 q[KS];
-  if constexpr (NB == 1) {
-    const int tok = pos[0] - sq.pos0;
-    const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + rc[0] - tok * G) * a.q.hd + 8 * g;
-#pragma unroll
-    for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 32 * s);
-  }
   if (t < piece.t1) {
+    u32x4 q[KS];
+    {
+      const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + rc - tok * G) * a.q.hd + 8 * g;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) q[s] = *(const u32x4*)(p + 32 * s);
+    }
     places(t);
     ask_scales(0);
     ask(false);
     ask(true);
-  }
-  if constexpr (NB > 1) {
-    for (int x = threadIdx.x; x < S::ROWS * (D / 8); x += S::THREADS) {
-      const int r = x / (D / 8), ch = x % (D / 8), at = r0 + min(r, rows - 1), tok = at / G;
-      const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * G + at - tok * G) * a.q.hd;
-      *(u32x4*)(lds + S::Q0 + 2 * D * r + 16 * (ch ^ S::place_q(r))) = *(const u32x4*)(p + 8 * ch);
-    }
-    __syncthreads();
-  } else {
 #pragma unroll
     for (int s = 0; s < KS; ++s) stay(q[s]);                   // here now: the loop must not wait for them, nor for what it asks for
-  }
-  if (t < piece.t1) {
-    // the chunks of queries of this lane's rows, the i-th step's at ^ 64 i
-    const int qread = S::Q0 + 2 * D * col + 16 * (g ^ S::place_q(col));
     // this lane's reads: 8 channels of two keys; 4 (8) keys by 16 channels a group of 16 lanes
     const int kread = col * S::RB + (S::I8 ? ((g >> 1) ^ S::place_k(col)) * 16 + 8 * (g & 1) : (g ^ S::place_k(col)) * 16);
     const int vkey = S::I8 ? 4 * g + ((lane & 15) >> 1 & 3) + 16 * ((lane & 15) >> 3) : 4 * g + ((lane & 15) >> 2);
@@ -441,11 +418,10 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
       const float* sc = (const float*)(mine + 2 * S::UNIT + 256 * odd) + 4 * g;
       if (more) places(t + KW);
       wait_loads<S::LOADS>();                                  // K is here, V may be on its way
-      f32x4 s[NB][2];
+      f32x4 s[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[nb][x] = f32x4(0.f);
+        s[x] = f32x4(0.f);
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
           u32x4 k;
@@ -456,14 +432,12 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           } else {
             k = lds_read16(mine + 16 * x * S::RB + (kread ^ (64 * i)));
           }
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) s[nb][x] = Rows<16>::mfma(k, NB == 1 ? q[i] : lds_read16(lds + 32 * D * nb + (qread ^ (64 * i))), s[nb][x]);
-          if (NB > 1) __builtin_amdgcn_sched_barrier(0);       // operands a step at a time: registers
+          s[x] = Rows<16>::mfma(k, q[i], s[x]);
         }
       }
       if constexpr (S::I8) {
 #pragma unroll
-        for (int x = 0; x < 2 * NB; ++x) Run<16, D>::times(s[x >> 1][x & 1], sc + 16 * (x & 1));
+        for (int x = 0; x < 2; ++x) run.times(s[x], sc + 16 * x);
       }
       if (more) {
         wait_lds();
@@ -472,25 +446,22 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
       }
       const int k0 = 32 * t;
       const bool masked = k0 + 31 > first || k0 < full;
-      u32x4 p[NB];
+      if (masked) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        if (masked) {
+        for (int x = 0; x < 2; ++x) run.mask(s[x], from - k0 - 16 * x - 4 * g, pos - k0 - 16 * x - 4 * g, -INFINITY);
+      }
+      run.follow(s, run.largest(s), c);
+      u32x4 p;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) Run<16, D>::mask(s[nb][x], from[nb] - k0 - 16 * x - 4 * g, pos[nb] - k0 - 16 * x - 4 * g, -INFINITY);
+      for (int x = 0; x < 2; ++x) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[x][e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], c, -run.ref));
+          run.l += s[x][e];
         }
-        run[nb].follow(s[nb], Run<16, D>::largest(s[nb]), c);
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[nb][x][e] = __builtin_amdgcn_exp2f(fmaf(s[nb][x][e], c, -run[nb].ref));
-            run[nb].l += s[nb][x][e];
-          }
-          if constexpr (S::I8) Run<16, D>::times(s[nb][x], sc + 32 + 16 * x);
-          p[nb][2 * x] = pk_bf16(s[nb][x][0], s[nb][x][1]);
-          p[nb][2 * x + 1] = pk_bf16(s[nb][x][2], s[nb][x][3]);
-        }
+        if constexpr (S::I8) run.times(s[x], sc + 32 + 16 * x);
+        p[2 * x] = pk_bf16(s[x][0], s[x][1]);
+        p[2 * x + 1] = pk_bf16(s[x][2], s[x][3]);
       }
       if (more) wait_loads<S::LOADS + S::SC>();                // V is here
       else wait_loads<0>();
@@ -506,9 +477,7 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
           const u32x2 x = lds_read_tr(V + (vread ^ (32 * i))), y = lds_read_tr(V + 16 * S::RB + (vread ^ (32 * i)));
           v = u32x4{x[0], x[1], y[0], y[1]};
         }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) run[nb].o[i] = Rows<16>::mfma(v, p[nb], run[nb].o[i]);
-        if (NB > 1) __builtin_amdgcn_sched_barrier(0);
+        run.o[i] = Rows<16>::mfma(v, p, run.o[i]);
       }
       if (masked) poisoned |= S::I8 ? scales_not_finite(sc - 4 * g + 32) : tile_not_finite<D>(V);
       if (more) {
@@ -516,71 +485,64 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
         ask(true);
       }
     }
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) run[nb].l = Rows<16>::sum_over(run[nb].l);
+    run.l = Rows<16>::sum_over(run.l);
   }
 
-  // the waves' parts of a row, joined through LDS, 16 rows at a time
-  float* jo = (float*)lds;                                     // [KW][16][D + 4]
-  float* jm = jo + KW * 16 * (D + 4);                          // [KW][16] maxima, then sums
+  // the waves' parts of a row, joined through LDS
+  float* jo = (float*)lds;                                     // [KW][ROWS][D + 4]
+  float* jm = jo + KW * S::ROWS * (D + 4);                     // [KW][ROWS] maxima, then sums
+  __syncthreads();
+  if (!poisoned) {
+    float* to = jo + (kw * S::ROWS + col) * (D + 4) + 4 * g;
 #pragma unroll
-  for (int nb = 0; nb < NB; ++nb) {
-    const int ra = r0 + 16 * nb, here = min(16, rows - 16 * nb);
-    if (here <= 0) break;
-    __syncthreads();
-    if (!poisoned) {
-      float* to = jo + (kw * 16 + col) * (D + 4) + 4 * g;
+    for (int i = 0; i < MB; ++i) *(f32x4*)(to + 16 * i) = run.o[i];
+    if (g == 0) { jm[kw * S::ROWS + col] = run.m; jm[(KW + kw) * S::ROWS + col] = run.l; }
+  } else {
+    rows_again<D, S::I8>(a, pg, b, pl, n, hk, sq, r0, r0 + rows, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
+      constexpr int C = D / 64;
 #pragma unroll
-      for (int i = 0; i < MB; ++i) *(f32x4*)(to + 16 * i) = run[nb].o[i];
-      if (g == 0) { jm[kw * 16 + col] = run[nb].m; jm[(KW + kw) * 16 + col] = run[nb].l; }
-    } else {
-      rows_again<D, S::I8>(a, pg, b, pl, n, hk, sq, ra, ra + here, piece.t0 + kw, piece.t1, KW, [&](int r, float m, float l, const float* y) {
-        constexpr int C = D / 64;
+      for (int e = 0; e < C; ++e) jo[(kw * S::ROWS + r - r0) * (D + 4) + C * lane + e] = y[e];
+      if (lane == 0) { jm[kw * S::ROWS + r - r0] = m; jm[(KW + kw) * S::ROWS + r - r0] = l; }
+    });
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < rows * (D / 4); x += S::THREADS) {
+    const int rr = x / (D / 4), d = 4 * (x % (D / 4));
+    float M = -INFINITY, L = 0.f;
+    f32x4 y = f32x4(0.f);
 #pragma unroll
-        for (int e = 0; e < C; ++e) jo[(kw * 16 + r - ra) * (D + 4) + C * lane + e] = y[e];
-        if (lane == 0) { jm[kw * 16 + r - ra] = m; jm[(KW + kw) * 16 + r - ra] = l; }
-      });
+    for (int k = 0; k < KW; ++k) M = fmaxf(M, jm[k * S::ROWS + rr]);
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const float mk = jm[k * S::ROWS + rr], w = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * c);
+      L = fmaf(w, jm[(KW + k) * S::ROWS + rr], L);             // a wave without a maximum: zeros, or NaN
+      y += w * *(const f32x4*)(jo + (k * S::ROWS + rr) * (D + 4) + d);
     }
-    __syncthreads();
-    for (int x = threadIdx.x; x < here * (D / 4); x += S::THREADS) {
-      const int rr = x / (D / 4), d = 4 * (x % (D / 4));
-      float M = -INFINITY, L = 0.f;
-      f32x4 y = f32x4(0.f);
-#pragma unroll
-      for (int k = 0; k < KW; ++k) M = fmaxf(M, jm[k * 16 + rr]);
-#pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const float mk = jm[k * 16 + rr], w = mk == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((mk - M) * c);
-        L = fmaf(w, jm[(KW + k) * 16 + rr], L);             // a wave without a maximum: zeros, or NaN
-        y += w * *(const f32x4*)(jo + (k * 16 + rr) * (D + 4) + d);
-      }
-      if (piece.pieces > 1) {
-        *(f32x4*)(part + (16 * nb + rr) * D + d) = y;
-        if (d == 0) { part[S::ROWS * D + 16 * nb + rr] = M; part[S::ROWS * (D + 1) + 16 * nb + rr] = L; }
-        continue;
-      }
-      const int tk = (ra + rr) / G;
-      store4(a, sq.lo + tk, hk * G + (ra + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
+    if (piece.pieces > 1) {
+      *(f32x4*)(part + rr * D + d) = y;
+      if (d == 0) { part[S::ROWS * D + rr] = M; part[S::ROWS * (D + 1) + rr] = L; }
+      continue;
     }
+    const int tk = (r0 + rr) / G;
+    store4(a, sq.lo + tk, hk * G + (r0 + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
   }
 }
 
-// workgroup `block` = (split, row tile, sequence, head)
+// workgroup `block` = (split, sequence, head)
 template <class S>
 __device__ __forceinline__ void few_block(const lq_attention& a, const lq_pages& pg, const lq_batch& b, const Plan& pl, char* lds, int block) {
-  const int items = b.N * pg.HK * pl.few_tiles, item = block % items, split = block / items, hk = item % pg.HK;
-  const int tile = item / (b.N * pg.HK), n = item / pg.HK - tile * b.N;
+  const int items = b.N * pg.HK, item = block % items, split = block / items, n = item / pg.HK, hk = item % pg.HK;
   const Seq sq = sequence(b, pg, pl.G, n);
   if (sq.rows <= 0 || (pl.many_blocks && sq.rows > S::ROWS)) return;
-  // more rows than the host said: a workgroup every few_tiles-th tile, all keys
-  const int step = S::ROWS * pl.few_tiles, splits = sq.rows > step ? 1 : pl.few_splits;
-  for (int r0 = S::ROWS * tile; r0 < sq.rows; r0 += step) {
+  // more rows than a tile has, where nobody else takes them: one workgroup all of them, a tile after the other
+  const int splits = sq.rows > S::ROWS ? 1 : pl.few_splits;
+  for (int r0 = 0; r0 < sq.rows; r0 += S::ROWS) {
     few_rows<S>(a, pg, b, pl, lds, n, hk, split, splits, r0, sq, pl.few_work + (long long)block * S::PART);
     __syncthreads();
   }
 }
 template <class S>
-__global__ __launch_bounds__(S::THREADS, S::NB > 1 && S::D > 64 ? 1 : 2) void few_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
+__global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_pages pg, lq_batch b, Plan pl) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   few_block<S>(a, pg, b, pl, lds, blockIdx.x);
 }
@@ -1016,17 +978,17 @@ __device__ __forceinline__ void join_block(const lq_attention& a, const lq_pages
   static_assert(PER >= 1 && ROWS % PER == 0, "rows of a workgroup");
   const int item = block / (ROWS / PER), rr = (block % (ROWS / PER)) * PER + threadIdx.x / (C * P);
   const int hk = item % pg.HK, number = item / pg.HK;
-  RowTile rt = {number % b.N, number / b.N * ROWS};
+  RowTile rt = {number, 0};
   if (!FEW) rt = row_tile<ROWS>(b, pl.G, number);
   const Seq sq = sequence(b, pg, pl.G, rt.n);
-  if (rt.r0 >= sq.rows || (FEW ? sq.rows > ROWS * pl.few_tiles : sq.rows <= pl.few)) return;
+  if (FEW ? sq.rows <= 0 || sq.rows > ROWS : rt.r0 >= sq.rows || sq.rows <= pl.few) return;
   const int rows = min(ROWS, sq.rows - rt.r0);
   if ((block % (ROWS / PER)) * PER >= rows) return;
   const int splits = FEW ? pl.few_splits : pl.many_splits;
   const Piece piece = piece_of<S>(keys_of(sq, pl.G, rt.r0, rt.r0 + rows, a.window), splits, 0);
   if (piece.pieces == 1) return;
   const int which = (threadIdx.x / C) % P, d = 4 * (threadIdx.x % C);
-  const long long step = (long long)(FEW ? b.N * pl.few_tiles : pl.tiles) * pg.HK * S::PART;
+  const long long step = (long long)(FEW ? b.N : pl.tiles) * pg.HK * S::PART;
   const float* part = (FEW ? pl.few_work : pl.many_work) + (long long)item * S::PART;
   const float c = a.scale * LOG2E;
   float M = -INFINITY, L = 0.f;
@@ -1089,8 +1051,7 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
-  typedef Few<D, 4, 1, I8> F;
-  typedef Few<D, 4, D == 256 ? 2 : 4, I8> W;
+  typedef Few<D, 4, I8> F;
   typedef Many<D, 4, D == 64 || (D == 128 && !I8) ? 64 : 32, D == 256 ? 1 : 2, I8> M;
 };
 
@@ -1109,66 +1070,58 @@ template <auto* KERNEL, int LDS> bool lds_asked() {
 // Sizes and the longest sequence's tokens, where the caller says them, settle what a call launches and how the keys are split.
 template <int D, bool I8> Plan plan_of(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest) {
   typedef typename Shapes<D, I8>::F F;
-  typedef typename Shapes<D, I8>::W W;
   typedef typename Shapes<D, I8>::M M;
   Plan c = {};
   c.G = a->HQ / p->HK;
   c.div = page_div(p->page);
   const long long cus = lq_attn_cus(), most = longest > 0 && longest < b->T ? longest : b->T, rows = most * c.G;
-  const bool many = rows > 64, few = !many || b->N > 1;
-  c.wide = !many && rows > F::ROWS;
+  // Which kernels, by rows: a sequence of up to 16 (a token's heads) reads its keys by waves of its own, which 64 of them at contexts up
+  // to 8192 do at 4.9 TB/s.  Beside longer ones that is worth a second kind of workgroup only if the others are short by the mean (us,
+  // with it / without): 32 sequences of up to 8 tokens, 8 heads a key head of 256 95 / 65, 5 of up to 777 under a window 19.5 / 19.4.
+  // A piece of 449 tokens beside 15 of one token, 4 heads a key head: 86 with it; without, a tile of 128 rows for 4.
+  const bool hint = longest > 0 && longest < b->T, many = rows > F::ROWS;
+  const bool few = !many || (b->N > 1 && (!hint || (b->T - most) * c.G <= (long long)F::ROWS * (b->N - 1)));
   c.few = few ? F::ROWS : 0;
-  c.few_tiles = c.wide ? (int)((rows + W::ROWS - 1) / W::ROWS) : 1;
   c.tiles = many ? (int)((long long)b->T * c.G / M::ROWS + b->N) : 0;
   // keys that a row tile sees at most; under a window of its rows' tokens
   auto reach = [&](int tile) {
     const long long all = (long long)b->width * p->page, near = (long long)a->window + (tile - 1) / c.G + 1;
     return a->window > 0 && near < all ? near : all;
   };
+  // Pieces of the keys, so that workgroups are as many as the chip holds at once.  A workgroup costs as much before its first and after
+  // its last key as some 500 keys, and a part is written and read again; four times as many where pieces still have 1024 keys (us, as
+  // many as held / twice / four times): 64 sequences up to 8192 of 8 heads of 128 267 / 266 / 255, 64 up to 4099 of 2 of 256 78 / 78 / 85 and from
+  // codes 61 / 68 / 89, 8 up to 4099 of 8 of 128 24 / 26 / 31, 2 up to 1024 9.5 / 12; tiles of many rows: 32 sequences up to 4099 of
+  // 2 of 256 58 / 65 / 65, a piece of 449 over 4096 of 8 of 128 beside 15 of one token 86 / 86 / 85.
+  constexpr int HELD = F::LDS > 81920 ? 1 : D == 64 ? 4 : 2;   // workgroups of few rows on a CU
   auto pieces = [&](long long target, long long items, long long keys, int least) {
     const long long by = (target + items - 1) / items, cap = keys / least;
     return (int)(by < 1 || cap < 2 ? 1 : by < cap ? (by < 256 ? by : 256) : (cap < 256 ? cap : 256));
   };
-  const long long fi = (long long)b->N * p->HK * c.few_tiles, mi = (long long)c.tiles * p->HK;
-  c.few_splits = few ? pieces((many ? 2 : 8) * cus, fi, reach(c.wide ? W::ROWS : F::ROWS), F::LEAST * F::KT) : 1;
-  c.many_splits = many && mi < 2 * cus ? pieces(2 * cus, mi, reach(M::ROWS), M::LEAST * M::KT) : 1;
+  const long long fi = (long long)b->N * p->HK, mi = (long long)c.tiles * p->HK;
+  c.few_splits = few ? std::max(pieces(HELD * cus, fi, reach(F::ROWS), F::LEAST * F::KT),
+                                many ? 1 : pieces(4 * HELD * cus, fi, reach(F::ROWS), 1024)) : 1;
+  c.many_splits = many && mi < M::EU * cus ? pieces(M::EU * cus, mi, reach(M::ROWS), M::LEAST * M::KT) : 1;
   c.few_blocks = few ? (int)(fi * c.few_splits) : 0;
   c.many_blocks = (int)(mi * c.many_splits);
   return c;
 }
 template <int D, bool I8> long long few_floats(const Plan& c) {
-  return c.few_splits > 1 ? (long long)c.few_blocks * (c.wide ? Shapes<D, I8>::W::PART : Shapes<D, I8>::F::PART) : 0;
+  return c.few_splits > 1 ? (long long)c.few_blocks * Shapes<D, I8>::F::PART : 0;
 }
 template <int D, bool I8> long long many_floats(const Plan& c) {
   return c.many_splits > 1 ? (long long)c.many_blocks * Shapes<D, I8>::M::PART : 0;
 }
 
-// four groups of threads a row where there are pieces enough for them
-template <class F, class M>
-int join(const lq_attention* a, const lq_pages* p, const lq_batch* b, const Plan& pl, hipStream_t s) {
-  if (pl.few_splits == 1 && pl.many_splits == 1) return LQ_OK;
-  const int P = pl.few_splits > 8 || pl.many_splits > 8 ? 4 : 1, per = 256 / (F::D / 4 * P);
-  const int few = pl.few_splits > 1 ? b->N * p->HK * pl.few_tiles * (F::ROWS / per) : 0;
-  const int many = pl.many_splits > 1 ? pl.tiles * p->HK * (M::ROWS / per) : 0;
-  const unsigned blocks = (unsigned)few + (unsigned)many;
-  if (P == 4) join_kernel<F, M, 4><<<blocks, 256, 0, s>>>(*a, *p, *b, pl, few);
-  else join_kernel<F, M, 1><<<blocks, 256, 0, s>>>(*a, *p, *b, pl, few);
-  return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
-}
-
 template <int D, bool I8>
 int go(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest, float* work, hipStream_t s) {
   typedef typename Shapes<D, I8>::F F;
-  typedef typename Shapes<D, I8>::W W;
   typedef typename Shapes<D, I8>::M M;
   Plan pl = plan_of<D, I8>(a, p, b, longest);
   pl.few_work = work;
   pl.many_work = work + few_floats<D, I8>(pl);
   const unsigned blocks = (unsigned)pl.few_blocks + (unsigned)pl.many_blocks;
-  if (pl.wide) {
-    if (!lds_asked<few_kernel<W>, W::LDS>()) return LQ_ERR_HIP;
-    few_kernel<W><<<blocks, W::THREADS, W::LDS, s>>>(*a, *p, *b, pl);
-  } else if (!pl.many_blocks) {
+  if (!pl.many_blocks) {
     if (!lds_asked<few_kernel<F>, F::LDS>()) return LQ_ERR_HIP;
     few_kernel<F><<<blocks, F::THREADS, F::LDS, s>>>(*a, *p, *b, pl);
   } else if (!pl.few_blocks) {
@@ -1180,7 +1133,15 @@ int go(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest,
     both_kernel<F, M><<<blocks, M::THREADS, LDS, s>>>(*a, *p, *b, pl);
   }
   if (hipGetLastError() != hipSuccess) return LQ_ERR_HIP;
-  return pl.wide ? join<W, M>(a, p, b, pl, s) : join<F, M>(a, p, b, pl, s);
+  if (pl.few_splits == 1 && pl.many_splits == 1) return LQ_OK;
+  // four groups of threads a row where there are pieces enough for them
+  const int P = pl.few_splits > 8 || pl.many_splits > 8 ? 4 : 1, per = 256 / (D / 4 * P);
+  const int few_join = pl.few_splits > 1 ? b->N * p->HK * (F::ROWS / per) : 0;
+  const int many_join = pl.many_splits > 1 ? pl.tiles * p->HK * (M::ROWS / per) : 0;
+  const unsigned joins = (unsigned)few_join + (unsigned)many_join;
+  if (P == 4) join_kernel<F, M, 4><<<joins, 256, 0, s>>>(*a, *p, *b, pl, few_join);
+  else join_kernel<F, M, 1><<<joins, 256, 0, s>>>(*a, *p, *b, pl, few_join);
+  return hipGetLastError() == hipSuccess ? LQ_OK : LQ_ERR_HIP;
 }
 
 template <typename F> auto by_shape(const lq_pages* p, F f) {
