@@ -214,6 +214,26 @@ template <int R, int D> struct Run {
   }
 };
 
+// Two weights as bf16 for the second product, codes' with the scales vs of their values.  Their sum l is of what was rounded: a key that
+// outweighs the others then has no error left, two alike half of it (against 64 bits, 64 sequences up to 8192 from codes: 0.0024 -> 0.0017,
+// which is the outputs' own rounding).  With scales, a rounded product is taken back through 1 / vs, `by`; where the scale is zero, not
+// finite or far from one, so that a product or 1 / vs could leave the range of fp32, the weight itself counts (`by` 0).  Products below
+// the smallest number are weights below 1e-19 then, of sums of 2^-8 or more.
+__device__ __forceinline__ float inverse(float vs) { return fabsf(vs) > 1e-18f && fabsf(vs) < 1e18f ? __builtin_amdgcn_rcpf(vs) : 0.f; }
+template <bool I8> __device__ __forceinline__ uint32_t weigh2(float a, float b, float va, float vb, float bya, float byb, float& l) {
+  if constexpr (I8) {
+    const uint32_t w = pk_bf16(a * va, b * vb);
+    const float wa = bf_lo(w), wb = bf_hi(w);
+    l += bya != 0.f ? wa * bya : a;
+    l += byb != 0.f ? wb * byb : b;
+    return w;
+  } else {
+    const uint32_t w = pk_bf16(a, b);
+    l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, w), s16x2{0x3f80, 0x3f80}, l, false);
+    return w;
+  }
+}
+
 // whether 32 rows of D bf16 in LDS hold an infinity or NaN
 template <int D> __device__ __forceinline__ bool tile_not_finite(const char* tile) {
   const int lane = threadIdx.x & 63;
@@ -457,11 +477,15 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[x][e] = __builtin_amdgcn_exp2f(fmaf(s[x][e], c, -run.ref));
-          run.l += s[x][e];
         }
-        if constexpr (S::I8) run.times(s[x], sc + 32 + 16 * x);
-        p[2 * x] = pk_bf16(s[x][0], s[x][1]);
-        p[2 * x + 1] = pk_bf16(s[x][2], s[x][3]);
+        f32x4 vs = f32x4(1.f), by = f32x4(1.f);
+        if constexpr (S::I8) {
+          vs = *(const f32x4*)(sc + 32 + 16 * x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) by[e] = inverse(vs[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) p[2 * x + e / 2] = weigh2<S::I8>(s[x][e], s[x][e + 1], vs[e], vs[e + 1], by[e], by[e + 1], run.l);
       }
       if (more) wait_loads<S::LOADS + S::SC>();                // V is here
       else wait_loads<0>();
@@ -556,7 +580,7 @@ template <int D_, int RW_, int KT_, int EU_, bool I8_> struct Many {
   static constexpr int D = D_, RW = RW_, EU = EU_, KT = KT_, X = KT / 32, LEAST = 512 / KT, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
   static constexpr bool I8 = I8_;
   static constexpr int RB = 2 * D, TILE = KT * RB;             // bytes in LDS
-  static constexpr int K0 = 0, V0 = 2 * TILE, SCALES = 4 * TILE, LDS = SCALES + (I8 ? 4 * KT * 4 : 0);
+  static constexpr int K0 = 0, V0 = 2 * TILE, SCALES = 4 * TILE, LDS = SCALES + (I8 ? 6 * KT * 4 : 0);          // scales of K and of V twice, the inverses of V's
   static constexpr int PART = ROWS * (D + 2);
   static constexpr int AHEAD = D == 256 ? 6 : 4;               // operands on their way: registers
   static constexpr int OWN = KT / RW;                          // keys of a tile that a wave loads, all of one page
@@ -667,6 +691,7 @@ template <class S> struct Tiles {
         }
       }
       if (lane < OWN) scale[rw * OWN + lane] = values ? vsc : ksc;
+      if (values && lane < OWN) scale[2 * KT + rw * OWN + lane] = inverse(vsc);
     }
   }
 };
@@ -726,20 +751,15 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   // instructions, and the operand of the one AHEAD of it.  Weights go in pairs: the product in the exponent of one beside
   // the exponentials of the one before, and the rounding and the sum (of what was rounded) of the one before that.
   constexpr int PAIRS = 8 * X, EARLY = X == 1 ? 5 : 4 * X;      // of a tile; those beside the next scores, with all four of the first operand
-  float ex[2], old[2], vs[2];
+  float ex[2], old[2], vs[2], by[2];
   uint32_t w[PAIRS];
   auto exponent = [&](const f32x16 (&s)[X], int i) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) { ex[e] = fmaf(s[i >> 3][2 * (i & 7) + e], c, -run.ref); stay(ex[e]); }
   };
   auto finish = [&](int i) {
-    if constexpr (S::I8) {
-      w[i] = pk_bf16(old[0] * vs[0], old[1] * vs[1]);
-      run.l += old[0] + old[1];
-    } else {
-      w[i] = pk_bf16(old[0], old[1]);
-      run.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(s16x2, w[i]), s16x2{0x3f80, 0x3f80}, run.l, false);
-    }
+    if constexpr (S::I8) w[i] = weigh2<true>(old[0], old[1], vs[0], vs[1], by[0], by[1], run.l);
+    else w[i] = weigh2<false>(old[0], old[1], 1.f, 1.f, 1.f, 1.f, run.l);
     stay(w[i]);
   };
   auto weigh = [&](const f32x16 (&s)[X], int buf, int lo, int hi) {            // pairs lo .. hi - 1; exponents of lo are there
@@ -754,8 +774,9 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       for (int e = 0; e < 2; ++e) old[e] = f[e];
       if constexpr (S::I8) {
         const f32x2 x = *(const f32x2*)(scale_at(true, buf) + 32 * (i >> 3) + 8 * ((i & 7) >> 1) + 2 * (i & 1));
-        vs[0] = x[0];
-        vs[1] = x[1];
+        const f32x2 y = *(const f32x2*)(scale_at(true, buf) + 2 * KT + 32 * (i >> 3) + 8 * ((i & 7) >> 1) + 2 * (i & 1));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { vs[e] = x[e]; by[e] = y[e]; }
       }
     }
   };
@@ -1052,7 +1073,7 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
   typedef Few<D, 4, I8> F;
-  typedef Many<D, 4, D == 64 || (D == 128 && !I8) ? 64 : 32, D == 256 ? 1 : 2, I8> M;
+  typedef Many<D, 4, !I8 && D <= 128 ? 64 : 32, D == 256 ? 1 : 2, I8> M;
 };
 
 // LDS beyond what a kernel has unasked: asked for once on each device, and again where that failed.

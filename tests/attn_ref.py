@@ -3,11 +3,13 @@
 Bars.  An output of rope_norm is rounded once, 2^-8 of it at most; before that the hardware's sine and cosine are off by less than
 2^-19 (test_sine_and_cosine), of the pair's magnitude, and fp32 products by a few 2^-24.
 
-An output of attend is sum_j w_j v_j, sum_j w_j = 1.  Each weight is rounded to bf16, off by 2^-8 of it at most: 2^-8 A with A =
-sum_j w_j |v_j|; the rounding of the output adds 2^-8 of it; scores in fp32 are off by D 2^-24 of |q| |k| scale at most (5e-5 at
-|q| |k| scale of 3 and D = 256, where the bars are used), which moves the weights by as much: 2^-12 A is above both.  Roundings of weights have random signs, so that
-the error's norm is 2^-8 of that of sqrt(sum_j w_j^2 v_j^2) at most in the mean (a rounding's rms is 2^-8 / 3^1/2 or less), and the
-same for the last one."""
+An output of attend is sum_j w_j v_j / sum_j w_j.  Each weight is rounded to bf16, w_j (1 + d_j) with |d_j| <= 2^-8, above and below
+alike, so that with sum_j w_j = 1 the quotient is off by sum_j w_j d_j (v_j - out), to first order: by 2^-8 (A + |out|) at most with
+A = sum_j w_j |v_j|.  The rounding of the output adds 2^-8 |out|; scores in fp32 are off by D 2^-24 of |q| |k| scale at most (5e-5 at
+|q| |k| scale of 3 and D = 256, where the bars are used), which moves the weights by as much: 2^-12 A is above both that and the second
+order.  Roundings of weights have random signs and an rms of 2^-8 / 3^1/2 at most, so that the error's norm is in the mean at most
+that of 2^-8 / 3^1/2 sqrt(sum_j w_j^2 (v_j - out)^2 + out^2), S^2 = sum_j w_j^2 v_j^2: below 2^-8 / 3^1/2 sqrt(2 S^2 + 3 out^2), as (a - b)^2 <=
+2 a^2 + 2 b^2 and sum_j w_j^2 <= 1, and so below 2^-8 sqrt(S^2 + out^2)."""
 import torch
 
 BF16, F64 = torch.bfloat16, torch.float64
@@ -102,7 +104,7 @@ def near(got, want, A, S):
     held = ~torch.isnan(want)
     assert torch.isfinite(got[held]).all(), "not finite"
     err = (got - want)[held].abs()
-    bar = 2.0 ** -8 * (want.abs() + A) + 2.0 ** -12 * A + 1e-30
+    bar = 2.0 ** -8 * (2 * want.abs() + A) + 2.0 ** -12 * A + 1e-30
     off = err > bar[held]
     assert not off.any(), (int(off.sum()), float((err / bar[held]).max()))
     norm, most = float(err.norm()), float((want * want + S * S)[held].sum().sqrt())

@@ -94,6 +94,15 @@ def test_rope_norm_one_token_and_many():
     check_rope(R.inputs(8, [1500, 20], [1501, 20], 12, 2, 128))                               # two
 
 
+@pytest.mark.parametrize("kw", [dict(HQ=16, HK=2, D=256, rot=64), dict(HQ=5, HK=1, D=64, rot=16), dict(HQ=6, HK=3, D=128), dict(HQ=1, HK=1, D=256, rot=0)])
+@pytest.mark.parametrize("interleaved,int8", [(False, False), (True, False), (False, True), (True, True)])
+def test_rope_norm_more_tokens_than_workgroups_are_held(kw, interleaved, int8):
+    """Several tokens a workgroup: sequences that begin and end inside one, no place, bad pages, rows of no sequence at the end."""
+    d = R.inputs(13, [1500, 1, 2, 999, 5], [1500, 7, 0, 1203, 3], page=32, int8=int8, extra=3, **kw)
+    d["table"][0, 3], d["table"][3, 20], d["table"][3, 21] = -1, d["kp"].shape[0], 2 ** 31 - 1
+    check_rope(d, interleaved=interleaved, offset=0.5)
+
+
 def test_rope_norm_padding_and_bad_pages():
     d = R.inputs(9, [4, 3, 6], [0, 2, 40], 4, 2, 128, extra=2)          # no place at all; two of three tokens; all
     check_rope(d)
@@ -381,6 +390,37 @@ def test_same_call_same_bits():
     d = R.inputs(51, [1, 90, 3], [3000, 190, 64], 8, 2, 128)
     a, b = attend(R.cuda(d)).clone(), attend(R.cuda(d))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("HQ,HK,D", [(16, 2, 256), (6, 2, 128), (4, 4, 64)])
+@pytest.mark.parametrize("new,ctx", [([50], [6000]), ([200], [300]), ([3, 1, 77], [2000, 900, 77]), ([1, 1], [4099, 40])])
+def test_calls_again_are_the_same_bits(new, ctx, HQ, HK, D, int8):
+    """Row tiles that are not full, pieces of the keys and both kinds of sequences: four calls of the same inputs."""
+    g = R.cuda(R.inputs(54, new, ctx, HQ, HK, D, int8=int8))
+    outs = [attend(g).clone() for _ in range(4)]
+    assert all(torch.equal(outs[0], x) for x in outs[1:])
+
+
+@pytest.mark.parametrize("longest", [None, 90])
+@pytest.mark.parametrize("new", [[90] + 20 * [1], [90, 40, 30, 1, 60], [1, 90, 16, 17, 3, 1]])
+@pytest.mark.parametrize("HQ,HK,D,int8", [(16, 2, 256, False), (8, 2, 128, True), (8, 8, 64, False)])
+def test_sequences_of_one_token_beside_longer_ones(new, longest, HQ, HK, D, int8):
+    """With the longest's tokens said, the others' mean settles whether those of few rows have workgroups of their own."""
+    ctx = [max(m, (37 * i * i) % 700) for i, m in enumerate(new)]
+    check_attend(R.inputs(55, new, ctx, HQ, HK, D, int8=int8), longest=longest)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("factor", [1e-25, 1e-17, 1e17, 1e20])
+def test_scales_of_any_size(factor, new, D):
+    """Scales next to and beyond those whose inverse is taken, some of them zero, beside ordinary ones.  A weight's product
+    with its scale and codes stays within fp32 throughout (1e20 127 2^8)."""
+    d = R.inputs(56, [new], [200], 4, 2, D, int8=True)
+    d["vs"][::2] *= factor
+    d["vs"][1::4, 3] = 0
+    check_attend(d)
 
 
 def test_empty_calls():
