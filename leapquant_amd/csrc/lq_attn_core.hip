@@ -5,14 +5,15 @@
 // A row r is a new token and one of the G = HQ / HK heads that read the same head of the cache, numbered token by token, so that
 // a key or value is read once for all of them.  One pass over the keys in tiles, with the running maximum m and sum of a row.
 //
-// A wave owns 32 rows.  It forms S^T = K Q^T with 32 x 32 matrix instructions: a lane then holds 16 of 32 keys of one row, its
-// maximum takes one exchange with lane ^ 32, and the probabilities are already laid out as the right operand of O^T = V^T P^T,
-// keys in an order that the transposing reads of V from LDS follow.  m moves only when a row's maximum has grown by 2^8 or more:
-// sums and outputs stay in fp32, so that only their common factor changes.  Probabilities are rounded to bf16 for the second
-// product (2^-9 each, of random sign), their sum is not.
+// A wave forms S^T = K Q^T, keys by rows: a lane then holds scores of one row, its maximum takes one or two lane exchanges, and the weights
+// are already laid out as the right operand of O^T = V^T P^T, keys in an order that the transposing reads of V from LDS follow.  m
+// moves only when a row's maximum has grown by 2^8 or more: sums and outputs stay in fp32, so that only their common factor
+// changes.  Weights are rounded to bf16 for the second product, and their sum is of what was rounded (weigh2).
 //
-// Tiles go from the pages straight into LDS, a tile ahead, in swizzled places: both kinds of reads then spread over all banks.
-// Codes of 8 bits go through registers and into LDS as bf16, which holds them exactly; their scales enter S and P in fp32.
+// Two kinds of workgroups: "few" for sequences of up to 16 rows, bound by memory, "many" for tiles of 128 rows, bound by the matrix
+// cores and the clock; where a call has both kinds, in one launch.  Keys are split into pieces where the rows do not fill the chip,
+// and a second launch joins them.  Tiles go from the pages straight into LDS in places that spread every read over all 64 banks (bank conflicts
+// of a prompt of 8192: 7.1e7 -> 3.9e6 cycles).
 #include <algorithm>
 #include <atomic>
 
@@ -344,6 +345,11 @@ __device__ __forceinline__ void store1(const lq_attention& a, long long token, i
 // Up to 16 rows of a sequence (a token's heads): a wave takes all of them, the KW waves of a workgroup every KW-th tile of 32 keys,
 // each by itself: K and V of a tile have a place in LDS each, and the next tile's are asked for as soon as this one's are used, so
 // that 32 D .. 64 D elements a wave are on their way at any time.  Codes stay codes in LDS.
+//
+// Measured (MI355X): 64 sequences up to 8192 of 8 heads of 128 255 us, 5.2 TB/s, a large copy's rate; from codes 170 us, 4.0 TB/s,
+// beside the conversion of the codes.  One sequence of 8192, 2 heads of 256: 10 us and 5 for the join, chains of
+// loads.  Workgroups of 32 or 64 rows of this kind lose to tiles of many rows (32 sequences of up to 64 rows, 2 heads of 256,
+// 75 us against 58; one of 48 rows over 16384, 8 heads of 128, 44 against 23): their queries no longer fit beside the outputs, and one wave a SIMD shows every wait.
 template <int D_, int KW_, bool I8_> struct Few {
   static constexpr int D = D_, KW = KW_, R = 16, ROWS = 16, KT = 32, LEAST = KW, THREADS = 64 * KW;
   static constexpr bool I8 = I8_;
@@ -575,7 +581,11 @@ __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_page
 // RW waves of 32 rows each share tiles of KT keys, K and V twice in LDS, K a tile ahead of V.  A wave forms the scores of a tile while it
 // takes the exponentials of the one before, and looks for their maximum while that one meets its values, so that its vector
 // instructions go in the shadow of its matrix instructions.  What bounds it then is the number of a wave's instructions.
-// Codes go through registers and into LDS as bf16.
+// Codes go through registers and into LDS as bf16, which holds them exactly; scales enter S and P in fp32.
+//
+// Measured (MI355X): a prompt of 8192, 32 / 8 heads of 128, 535 us, 1.03 PFLOP/s (a large product by the library 1.31): its clock falls to
+// 1.5 .. 1.95 GHz; a piece of 2048 over 32768, 16 / 2 heads of 256, 1100 us, 0.98 PFLOP/s, one wave a SIMD; 4096 from codes of 32 / 8 of 128
+// 289 us.  Without the order of instructions below 584 and 2184; without queries waited for before the loop 573 and 1344.
 template <int D_, int RW_, int KT_, int EU_, bool I8_> struct Many {
   static constexpr int D = D_, RW = RW_, EU = EU_, KT = KT_, X = KT / 32, LEAST = 512 / KT, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
   static constexpr bool I8 = I8_;
@@ -1073,6 +1083,9 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 // ---- launches ---------------------------------------------------------------------------------------------------------------
 template <int D, bool I8> struct Shapes {
   typedef Few<D, 4, I8> F;
+  // Tiles of 64 keys, or 32 where 64 do not fit the registers: heads of 256 and codes (prompt of
+  // 8192 of heads of 128 573 -> 563 us by 64; 4096 from codes 666, spilled, -> 258 by 32).  Heads of 256 hold 32 rows of outputs in half the registers of
+  // a SIMD: one wave there.
   typedef Many<D, 4, !I8 && D <= 128 ? 64 : 32, D == 256 ? 1 : 2, I8> M;
 };
 
