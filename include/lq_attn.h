@@ -44,7 +44,7 @@ typedef struct lq_batch {
   const int* lens;        /* [N] */
   const int* table;       /* [N] rows of `width` entries, table_ld apart */
   long long table_ld;
-  int width;              /* width * page < 2^31, width * page * page < 2^40 */
+  int width;              /* width * page < 2^31 (lq_attend: 2^31 - 4096), width * page * page < 2^40 */
   int N, T;
 } lq_batch;
 

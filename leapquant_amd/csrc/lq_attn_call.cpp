@@ -165,8 +165,8 @@ lq_pages pages(PyObject* o, const Device& dev) {
   dev.on(v, "pages.v");
   return p;
 }
-void limits(const lq_batch& b, const lq_pages& p) {
-  if ((long long)b.width * p.page >= 0x7fffffffll || (unsigned long long)b.width * p.page * (unsigned long long)p.page >= 1ull << 40)
+void limits(const lq_batch& b, const lq_pages& p, long long most) {
+  if ((long long)b.width * p.page > most || (unsigned long long)b.width * p.page * (unsigned long long)p.page >= 1ull << 40)
     raise(PyExc_ValueError, "table: %d pages of %d tokens are more than the kernels' places hold", b.width, p.page);
 }
 // a weight of D elements in fp32 or bf16 (true)
@@ -241,7 +241,7 @@ PyObject* rope_norm(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     r.offset = (float)number(arg[12], "offset");
     r.interleaved = truth(arg[13]);
     const Batch b = batch(arg[7], arg[8], arg[9], dev, T);
-    limits(b.b, p);
+    limits(b.b, p, 0x7ffffffell);
     dev.gpu();
     const Current current(dev.dev);
     return lq_rope_norm(&r, &p, &b.b, stream(dev.dev));
@@ -272,7 +272,7 @@ PyObject* attend(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     if (longest < 0) raise(PyExc_ValueError, "longest: a number of tokens expected, got %lld", longest);
     a.window = (int)window;
     const Batch b = batch(arg[2], arg[3], arg[4], dev, T);
-    limits(b.b, p);
+    limits(b.b, p, 0x7fffffffll - 4096);
     dev.gpu();
     const Current current(dev.dev);
     const int most = (int)(longest < T ? longest : T);

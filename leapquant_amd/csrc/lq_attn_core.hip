@@ -105,13 +105,15 @@ __device__ __forceinline__ Seq sequence(const lq_batch& b, const lq_pages& p, in
   return s;
 }
 
+// the first key that position pos sees; pos may lie before 0, and a window be as long as an int
+__device__ __forceinline__ int first_key(int pos, int window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 // keys [lo, hi) that rows [r0, r1) see
 struct Keys { int lo, hi; };
 __device__ __forceinline__ Keys keys_of(const Seq& s, int G, int r0, int r1, int window) {
   Keys k;
   const int first = s.pos0 + r0 / G, last = s.pos0 + (r1 - 1) / G;
   k.hi = max(last + 1, 0);
-  k.lo = window > 0 ? max(first - window + 1, 0) : 0;
+  k.lo = first_key(first, window);
   if (k.lo > k.hi) k.lo = k.hi;
   return k;
 }
@@ -266,7 +268,7 @@ __device__ __forceinline__ void rows_again(const lq_attention& a, const lq_pages
   const int lane = threadIdx.x & 63, tend = max(sq.len - 1, 0);
   const float c = a.scale * LOG2E;
   for (int r = ra; r < rb; ++r) {
-    const int tok = r / pl.G, pos = sq.pos0 + tok, from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+    const int tok = r / pl.G, pos = sq.pos0 + tok, from = first_key(pos, a.window);
     const bf16_t* q = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)(hk * pl.G + r - tok * pl.G) * a.q.hd;
     float m = -INFINITY, l = 0.f, y[C] = {};
 #pragma unroll 1
@@ -377,9 +379,9 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
   const Piece piece = piece_of<S>(keys_of(sq, G, r0, r0 + rows, a.window), splits, split);
   if (split >= piece.pieces) return;
   const int rc = r0 + min(col, rows - 1), tok = rc / G, pos = sq.pos0 + tok;
-  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;              // keys from .. pos are seen
+  const int from = first_key(pos, a.window);              // keys from .. pos are seen
   const int first = sq.pos0 + r0 / G, last = sq.pos0 + (r0 + rows - 1) / G;    // all rows see full .. first
-  const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;
+  const int full = first_key(last, a.window);
 
   char* const mine = lds + kw * S::WAVE;
   const int* tab = b.table + (long long)n * b.table_ld;
@@ -717,8 +719,8 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   const int row = r0 + 32 * rw + col, rc = min(row, r0 + rows - 1), tok = rc / G, pos = sq.pos0 + tok, head = hk * G + rc - tok * G;
   const bool busy = 32 * rw < rows;                            // the wave has rows
   const int first = sq.pos0 + min(r0 + 32 * rw, r0 + rows - 1) / G, last = sq.pos0 + (min(r0 + 32 * rw + 32, r0 + rows) - 1) / G;
-  const int from = a.window > 0 ? max(pos - a.window + 1, 0) : 0;               // keys from .. pos are seen
-  const int full = a.window > 0 ? max(last - a.window + 1, 0) : 0;              // all rows of the wave see full .. first
+  const int from = first_key(pos, a.window);               // keys from .. pos are seen
+  const int full = first_key(last, a.window);              // all rows of the wave see full .. first
   u32x4 q[KS];
   {
     const bf16_t* p = (const bf16_t*)a.q.p + (long long)(sq.lo + tok) * a.q.ld + (long long)head * a.q.hd + 8 * g;
@@ -1110,7 +1112,7 @@ template <int D, bool I8> Plan plan_of(const lq_attention* a, const lq_pages* p,
   c.div = page_div(p->page);
   const long long cus = lq_attn_cus(), most = longest > 0 && longest < b->T ? longest : b->T, rows = most * c.G;
   // Which kernels, by rows: a sequence of up to 16 (a token's heads) reads its keys by waves of its own, which 64 of them at contexts up
-  // to 8192 do at 4.9 TB/s.  Beside longer ones that is worth a second kind of workgroup only if the others are short by the mean (us,
+  // to 8192 do at 5.2 TB/s.  Beside longer ones that is worth a second kind of workgroup only if the others are short by the mean (us,
   // with it / without): 32 sequences of up to 8 tokens, 8 heads a key head of 256 95 / 65, 5 of up to 777 under a window 19.5 / 19.4.
   // A piece of 449 tokens beside 15 of one token, 4 heads a key head: 86 with it; without, a tile of 128 rows for 4.
   const bool hint = longest > 0 && longest < b->T, many = rows > F::ROWS;
@@ -1191,7 +1193,8 @@ int check(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longe
   if (!rows_ok(a->q) || !rows_ok(a->gate) || !rows_ok(a->out) || !a->q.p || !a->out.p) return LQ_ERR_ARG;
   if (!rows_apart(a->out, b->T, a->HQ, p->D)) return LQ_ERR_ARG;
   const long long G = a->HQ / p->HK;
-  // rows, row tiles and workgroups in 32 bits
+  // places of a tile past the last key, rows, row tiles and workgroups in 32 bits
+  if ((long long)b->width * p->page > 0x7fffffffll - 4096) return LQ_ERR_ARG;
   if (((long long)b->T + 64) * G > 0x3fffffffll || ((long long)b->T * G / 64 + b->N + 8) * p->HK > 0x7fffffffll / 256) return LQ_ERR_ARG;
   return LQ_OK;
 }

@@ -161,6 +161,8 @@ def test_attend_refuses_work_and_sizes(lib):
     assert need > 0                                             # one token over 16000: pieces
     for work, n in ((None, need), (16, need - 1), (8, need)):
         assert lib.lq_attend(*ref, 1, work, n, None) == -1
+    far = _batch(N=1, T=1, width=(1 << 27) - 1)                 # 2^31 - 16 places: a tile past the last would leave 32 bits
+    assert _call(lib, a=a, b=far) == -1 and lib.lq_attend_workspace(ref[0], ref[1], ctypes.byref(far), 1) == -1
     big = _batch(N=1, T=1 << 30, width=4)
     assert _call(lib, a=a, b=big) == -1                         # rows in 32 bits
 

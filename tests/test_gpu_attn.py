@@ -243,6 +243,12 @@ def test_values_that_are_not_finite_reach_who_sees_them(D):
     R.near(got, *want)
 
 
+@pytest.mark.parametrize("new,ctx", [([6, 2], [3, 90]), ([70], [40]), ([90, 1], [60, 0])])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40])
+def test_the_longest_windows_and_rows_before_the_first_position(new, ctx, window):
+    check_attend(R.inputs(34, new, ctx, 4, 2, 128), window=window)
+
+
 def test_attend_padding_and_rows_before_the_first_position():
     d = R.inputs(35, [2, 5, 3, 60], [0, 3, 0, 20], 8, 2, 128, extra=1)
     out = check_attend(d).cpu()
