@@ -75,8 +75,8 @@ template <int N> __device__ __forceinline__ void load16s(const char* base, const
     load16s<4>(base, {off[4], off[5], off[6], off[7]}, lds + 4096);
   } else
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
-                 "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:3072"
-                 :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]) : "memory", "m0");
+                 "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:%6"
+                 :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "n"(3 * 1024) : "memory", "m0");
 }
 __device__ __forceinline__ void load4(const float* from, const char* lds) {
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
