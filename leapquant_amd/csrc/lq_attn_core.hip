@@ -867,6 +867,10 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       adjust(piece.t0, 0, one);
       run.follow(one, Carry::largest(one), c);
     }
+    // Every wave has used up the first keys and their scales before any asks for, or settles, the third tile's over them: the loop's first
+    // barrier comes only after that, and a wave without rows is there at once.  In the loop a barrier lies between: what is asked for goes where
+    // the turn before read, after this turn's barrier; codes settle before it, where two turns before read.
+    __syncthreads();
     auto tile = [&](int i, int buf, f32x16 (&s)[X], f32x16 (&next)[X]) {       // buf: i & 1
       const bool more = i + 1 < tiles;
       const int t = piece.t0 + i;

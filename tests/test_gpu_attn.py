@@ -489,3 +489,19 @@ def test_a_layer_in_pieces_is_the_layer(window, int8):
     now = {n: v.cpu() if isinstance(v, torch.Tensor) else v for n, v in g.items()}
     now["q"] = R.rope(full)[0].to(BF16)
     R.near(got[-40:], *(x[-40:] for x in R.attend(now, window=window)))
+
+
+# ---- the start of a walk over tiles of keys ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("HQ,HK,D", [(16, 2, 256), (8, 2, 128), (4, 4, 64)])
+def test_warm_calls_of_part_full_tiles(HQ, HK, D, int8):
+    """Waves without rows beside waves with rows, walks of three tiles of keys and more: the first call is right, and calls whose
+    keys lie in the L2 are the same bits.  (Which write comes before which read in LDS: tests/test_attn_order.py.)"""
+    G = HQ // HK
+    for new, ctx in (([20 // G + 17], [400]), ([33 + 128 // G, 40], [500, 130]), ([100], [100 + 64 * 3])):
+        d = R.inputs(57, new, ctx, HQ, HK, D, int8=int8, page=32)
+        g = R.cuda(d)
+        first = attend(g, longest=max(new)).clone()
+        R.near(first, *R.attend(d))
+        same = torch.stack([(attend(g, longest=max(new)) == first).all() for _ in range(30)])
+        assert same.all()
