@@ -227,11 +227,16 @@ __global__ __launch_bounds__(TH) void rope_norm_kernel(lq_rope r, lq_pages p, lq
         if (write) *(u32x4*)((bf16_t*)to + (long long)at.page * p.page_ld + at.in * p.row_ld + h * p.head_ld + d0) = pack8(y);
       } else if (__any(write)) {
         float big = 0.f;
+        bool nan = false;                                      // a maximum drops it
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(y[e]));
+        for (int e = 0; e < 8; ++e) {
+          big = fmaxf(big, fabsf(y[e]));
+          nan |= y[e] != y[e];
+        }
         big = lanes_max<LANES>(big);
-        const float scale = big > 1e-30f ? big * (1.f / 127.f) : 0.f;
-        const float inv = big > 1e-30f && big < INFINITY ? 127.f / big : 0.f;
+        nan = (__ballot(nan) >> ((threadIdx.x & 63) - lane)) & ((1ull << LANES) - 1);
+        const float scale = nan ? NAN : big > 1e-30f ? big * (1.f / 127.f) : 0.f;
+        const float inv = !nan && big > 1e-30f && big < INFINITY ? 127.f / big : 0.f;
         uint32_t o[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {

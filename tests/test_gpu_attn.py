@@ -103,6 +103,15 @@ def test_rope_norm_more_tokens_than_workgroups_are_held(kw, interleaved, int8):
     check_rope(d, interleaved=interleaved, offset=0.5)
 
 
+@pytest.mark.parametrize("kw", [dict(HQ=16, HK=2, D=256, rot=64), dict(HQ=5, HK=1, D=64, rot=16), dict(HQ=6, HK=3, D=128), dict(HQ=1, HK=1, D=256, rot=0)])
+@pytest.mark.parametrize("interleaved,int8", [(False, False), (True, False), (False, True), (True, True)])
+def test_rope_norm_more_tokens_than_workgroups_are_held(kw, interleaved, int8):
+    """Several tokens a workgroup: sequences that begin and end inside one, no place, bad pages, rows of no sequence at the end."""
+    d = R.inputs(13, [1500, 1, 2, 999, 5], [1500, 7, 0, 1203, 3], page=32, int8=int8, extra=3, **kw)
+    d["table"][0, 3], d["table"][3, 20], d["table"][3, 21] = -1, d["kp"].shape[0], 2 ** 31 - 1
+    check_rope(d, interleaved=interleaved, offset=0.5)
+
+
 def test_rope_norm_padding_and_bad_pages():
     d = R.inputs(9, [4, 3, 6], [0, 2, 40], 4, 2, 128, extra=2)          # no place at all; two of three tokens; all
     check_rope(d)
@@ -429,6 +438,37 @@ def test_scales_of_any_size(factor, new, D):
     check_attend(d)
 
 
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("HQ,HK,D", [(16, 2, 256), (6, 2, 128), (4, 4, 64)])
+@pytest.mark.parametrize("new,ctx", [([50], [6000]), ([200], [300]), ([3, 1, 77], [2000, 900, 77]), ([1, 1], [4099, 40])])
+def test_calls_again_are_the_same_bits(new, ctx, HQ, HK, D, int8):
+    """Row tiles that are not full, pieces of the keys and both kinds of sequences: four calls of the same inputs."""
+    g = R.cuda(R.inputs(54, new, ctx, HQ, HK, D, int8=int8))
+    outs = [attend(g).clone() for _ in range(4)]
+    assert all(torch.equal(outs[0], x) for x in outs[1:])
+
+
+@pytest.mark.parametrize("longest", [None, 90])
+@pytest.mark.parametrize("new", [[90] + 20 * [1], [90, 40, 30, 1, 60], [1, 90, 16, 17, 3, 1]])
+@pytest.mark.parametrize("HQ,HK,D,int8", [(16, 2, 256, False), (8, 2, 128, True), (8, 8, 64, False)])
+def test_sequences_of_one_token_beside_longer_ones(new, longest, HQ, HK, D, int8):
+    """With the longest's tokens said, the others' mean settles whether those of few rows have workgroups of their own."""
+    ctx = [max(m, (37 * i * i) % 700) for i, m in enumerate(new)]
+    check_attend(R.inputs(55, new, ctx, HQ, HK, D, int8=int8), longest=longest)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("factor", [1e-25, 1e-17, 1e17, 1e20])
+def test_scales_of_any_size(factor, new, D):
+    """Scales next to and beyond those whose inverse is taken, some of them zero, beside ordinary ones.  A weight's product
+    with its scale and codes stays within fp32 throughout (1e20 127 2^8)."""
+    d = R.inputs(56, [new], [200], 4, 2, D, int8=True)
+    d["vs"][::2] *= factor
+    d["vs"][1::4, 3] = 0
+    check_attend(d)
+
+
 def test_empty_calls():
     d = R.inputs(52, [1], [5], 4, 2, 128)
     g = R.cuda(d)
@@ -505,3 +545,36 @@ def test_warm_calls_of_part_full_tiles(HQ, HK, D, int8):
         R.near(first, *R.attend(d))
         same = torch.stack([(attend(g, longest=max(new)) == first).all() for _ in range(30)])
         assert same.all()
+
+
+# ---- 8-bit pages hide nothing ----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [[6, 40], [2030, 90]], ids=["few", "many"])          # a token a workgroup, and several
+def test_nan_goes_through_8_bit_pages(new, D, interleaved):
+    """A NaN in a head of a key or value makes that head's scale NaN and its codes 0, an infinity beside it or not; the tokens
+    that see it have NaN in the query heads that read it, all others what they had."""
+    d = R.inputs(58, new, new, 4, 2, D, page=32, int8=True)
+    T, last = sum(new), new[0] - 2
+    d["k"][last, 1, D - 3] = NAN                     # a key's head is NaN as a whole after its norm
+    d["v"][T - 5, 0, D // 2 + 1], d["v"][T - 5, 0, 7] = NAN, INF
+    g = R.cuda(d)
+    rope(g, interleaved=interleaved)
+    clean = dict(d, k=torch.nan_to_num(d["k"], 0.0, 0.0), v=torch.nan_to_num(d["v"], 0.0, 0.0))
+    _, k, where = R.rope(clean, interleaved=interleaved)
+    got = {x: g[x].cpu() for x in ("kp", "vp", "ks", "vs")}
+    for t, page, place in where:
+        for x, vals, bad in (("k", k, (last, 1)), ("v", d["v"].to(F64), (T - 5, 0))):
+            for h in range(2):
+                s, c = got[x + "s"][page, place, h], got[x + "p"][page, place, h]
+                if (t, h) == bad:
+                    assert torch.isnan(s) and (c == 0).all(), (x, t, h)
+                else:
+                    big = float(vals[t, h].abs().amax())
+                    # the head's largest by test_rope_norm's bar, 2^-16 of it, and the scale's own rounding
+                    assert abs(float(s) - big / 127) <= 2.0 ** -15 * big / 127, (x, t, h)
+    out = attend(g).cpu()
+    hit = torch.zeros(T, 4, D, dtype=torch.bool)
+    hit[last:new[0], 2:] = True
+    hit[T - 5:, :2] = True
+    assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
