@@ -56,7 +56,7 @@ typedef struct lq_rows {
 
 /* x rsqrt(mean(x^2) + eps) (offset + weight) over each head of q and k, then its first `rot` elements turned in pairs by position *
  * inv_freq: (i, i + rot / 2), or interleaved (2i, 2i + 1).  q goes to out, which may be q, k and v to the new tokens' places in the
- * pages (8 bits: code = rint(x / scale), scale = max|x| / 127 of a token's head, NaN where the head holds one; a
+ * pages (8 bits: code = rint(x / scale), scale = max|x| / 127 of a token's head, NaN where the head holds one, 0 where max|x| <= 1e-30; a
  * scale of 0, or not finite, has codes of 0).
  * A token whose table entry is outside 0 .. NP - 1 is not written.  Places that two new tokens of a call share hold either's. */
 typedef struct lq_rope {

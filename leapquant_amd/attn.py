@@ -37,8 +37,8 @@ def rope_norm(q, k, v, q_weight, k_weight, inv_freq, pages, table, loc, lens, ou
 
     q, out: bf16 [T, HQ, D]; k, v: bf16 [T, HK, D]; any token and head strides divisible by 16 bytes.  Weights fp32 or bf16 [D]; offset
     1 for weights stored around zero.  inv_freq: fp32 or fp64, a multiple of 8 elements (none: no rotation); angles are formed in
-    64 bits.  Pages in 8 bits take code = rint(x / scale) with scale = max|x| / 127 of a token's head: NaN where the head holds one,
-    with codes of 0 for these and for infinite ones.  Two new tokens of a call do not share a place in the pages."""
+    64 bits.  Pages in 8 bits take code = rint(x / scale) with scale = max|x| / 127 of a token's head: NaN where the head holds one, 0
+    where max|x| <= 1e-30, with codes of 0 for these and for infinite ones.  Two new tokens of a call do not share a place in the pages."""
     _lib.attn_call().rope_norm(q, k, v, q_weight, k_weight, inv_freq, pages, table, loc, lens, out, eps, offset, interleaved)
 
 

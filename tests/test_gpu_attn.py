@@ -578,3 +578,21 @@ def test_nan_goes_through_8_bit_pages(new, D, interleaved):
     hit[last:new[0], 2:] = True
     hit[T - 5:, :2] = True
     assert torch.isnan(out[hit]).all() and torch.isfinite(out[~hit]).all()
+
+
+def test_heads_of_next_to_nothing_in_8_bits():
+    """Heads whose largest is at most 1e-30 have scales and codes of 0, the next larger ones have neither."""
+    d = R.inputs(59, [6], [6], 2, 2, 64, int8=True)
+    d["v"] *= 0
+    tiny = torch.tensor([1e-30, 1e-38, 1.01e-30, 1e-29, -1e-30, -1.01e-30]).to(BF16)
+    d["v"][:, :, 5] = tiny[:, None]
+    g = R.cuda(d)
+    rope(g)
+    for t, page, place in R.rope(d)[2]:
+        s, c = g["vs"][page, place].cpu(), g["vp"][page, place].cpu()
+        big = abs(float(tiny[t]))
+        if big <= 1e-30:
+            assert (s == 0).all() and (c == 0).all(), t
+        else:
+            # one rounding of 1 / 127 and one of the product
+            assert ((s.to(F64) - big / 127).abs() <= 2.0 ** -23 * big / 127).all() and (c[:, 5].abs() == 127).all(), t
