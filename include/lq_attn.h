@@ -37,8 +37,8 @@ typedef struct lq_pages {
 /* A ragged batch: sequence n holds the packed new tokens loc[n] .. loc[n + 1] - 1 of T, the last ones of its lens[n] cached tokens.
  * Token t of a sequence (its position, from 0) is at t % page in page table[n * table_ld + t / page].  The kernels hold
  * every offset to 0 <= loc[n] <= loc[n + 1] <= T and lens[n] to 0 .. width * page; a new token before position 0 (as all of a
- * padding sequence with lens[n] <= 0) sees and writes nothing, its outputs are zero.  Rows of outputs that no sequence
- * holds are not written. */
+ * padding sequence with lens[n] <= 0) sees and writes nothing, its outputs are zero whatever its inputs hold.  Rows of outputs
+ * that no sequence holds are not written. */
 typedef struct lq_batch {
   const int* loc;         /* [N + 1] */
   const int* lens;        /* [N] */

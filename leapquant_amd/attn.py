@@ -11,9 +11,9 @@ scale, with fp32 scales [pages, page, heads], one a token and head.
 A ragged batch is given by `loc` [N + 1] (sequence n holds the packed new tokens loc[n] .. loc[n + 1] - 1), `lens` [N], the cached
 tokens of each sequence with the new ones, which are the last of them, and `table` [N, width]: token t of sequence n is at t %
 page in page table[n, t // page].  New tokens before a sequence's position 0 (all of them where lens is 0: padding) have outputs of
-zero and write nothing; rows that no sequence holds are left as they are.  A table entry outside the cache is not written; it
-reads page 0.  Calls launch on the current stream of their tensors' device, never synchronise and can be captured in a graph;
-they work forward only (no autograd).
+zero, whatever their inputs hold, and write nothing; rows that no sequence holds are left as they are.  A table entry outside
+the cache is not written; it reads page 0.  Calls launch on the current stream of their tensors' device, never synchronise and can
+be captured in a graph; they work forward only (no autograd).
 """
 import typing
 

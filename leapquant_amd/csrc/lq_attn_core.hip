@@ -333,13 +333,14 @@ __device__ __forceinline__ f32x4 gate4(const lq_rows& gate, long long token, int
   for (int e = 0; e < 4; ++e) y[e] = __builtin_amdgcn_rcpf(1.0f + __expf(-z[e]));
   return y;
 }
-__device__ __forceinline__ void store4(const lq_attention& a, long long token, int head, int d, f32x4 y) {
-  if (a.gate.p) y *= gate4(a.gate, token, head, d);
+// An output at position pos.  Before 0 the row sees nothing: y is zero, and stays so whatever the gate of such a row holds.
+__device__ __forceinline__ void store4(const lq_attention& a, long long token, int pos, int head, int d, f32x4 y) {
+  if (a.gate.p && pos >= 0) y *= gate4(a.gate, token, head, d);
   *(u32x2*)((bf16_t*)a.out.p + token * a.out.ld + (long long)head * a.out.hd + d) = u32x2{pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
 }
 
-__device__ __forceinline__ void store1(const lq_attention& a, long long token, int head, int d, float y) {
-  if (a.gate.p) y *= __builtin_amdgcn_rcpf(1.0f + __expf(-bf2f(((const bf16_t*)a.gate.p)[token * a.gate.ld + (long long)head * a.gate.hd + d])));
+__device__ __forceinline__ void store1(const lq_attention& a, long long token, int pos, int head, int d, float y) {
+  if (a.gate.p && pos >= 0) y *= __builtin_amdgcn_rcpf(1.0f + __expf(-bf2f(((const bf16_t*)a.gate.p)[token * a.gate.ld + (long long)head * a.gate.hd + d])));
   ((bf16_t*)a.out.p)[token * a.out.ld + (long long)head * a.out.hd + d] = f2bf(y);
 }
 
@@ -556,7 +557,7 @@ __device__ __forceinline__ void few_rows(const lq_attention& a, const lq_pages& 
       continue;
     }
     const int tk = (r0 + rr) / G;
-    store4(a, sq.lo + tk, hk * G + (r0 + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
+    store4(a, sq.lo + tk, sq.pos0 + tk, hk * G + (r0 + rr - tk * G), d, y * (L == 0.f ? 0.f : 1.f / L));
   }
 }
 
@@ -919,7 +920,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
       for (int e = 0; e < C; ++e) {
         const int d = C * lane + e;
         if (piece.pieces > 1) part[(r - r0) * D + d] = y[e];
-        else store1(a, sq.lo + tk, hk * G + r - tk * G, d, y[e] * inv);
+        else store1(a, sq.lo + tk, sq.pos0 + tk, hk * G + r - tk * G, d, y[e] * inv);
       }
       if (piece.pieces > 1 && lane == 0) { part[S::ROWS * D + r - r0] = m; part[S::ROWS * (D + 1) + r - r0] = l; }
     });
@@ -941,7 +942,7 @@ __device__ __forceinline__ void many_rows(const lq_attention& a, const lq_pages&
   for (int i = 0; i < MB; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      store4(a, sq.lo + tok, head, 32 * i + 8 * e + 4 * g, f32x4{run.o[i][4 * e], run.o[i][4 * e + 1], run.o[i][4 * e + 2], run.o[i][4 * e + 3]} * inv);
+      store4(a, sq.lo + tok, pos, head, 32 * i + 8 * e + 4 * g, f32x4{run.o[i][4 * e], run.o[i][4 * e + 1], run.o[i][4 * e + 2], run.o[i][4 * e + 3]} * inv);
       __builtin_amdgcn_sched_barrier(0);                       // not all gates at once: their registers
     }
 }
@@ -1076,7 +1077,7 @@ __device__ __forceinline__ void join_block(const lq_attention& a, const lq_pages
   }
   if (rr >= rows) return;
   const int tk = (rt.r0 + rr) / pl.G;
-  store4(a, sq.lo + tk, hk * pl.G + (rt.r0 + rr - tk * pl.G), d, y * (L == 0.f ? 0.f : 1.f / L));
+  store4(a, sq.lo + tk, sq.pos0 + tk, hk * pl.G + (rt.r0 + rr - tk * pl.G), d, y * (L == 0.f ? 0.f : 1.f / L));
 }
 
 template <class F, class M, int P>

@@ -596,3 +596,24 @@ def test_heads_of_next_to_nothing_in_8_bits():
         else:
             # one rounding of 1 / 127 and one of the product
             assert ((s.to(F64) - big / 127).abs() <= 2.0 ** -23 * big / 127).all() and (c[:, 5].abs() == 127).all(), t
+
+
+# ---- outputs of rows before the first position ------------------------------------------------------------------------------
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new,ctx", [([2, 5, 1], [0, 3, 40]), ([70, 60], [0, 20]), ([1, 90, 2], [3000, 60, 0]), ([3, 2], [1, 5000])])
+def test_padding_is_zero_whatever_its_gate_holds(new, ctx, D, int8):
+    """Sequences without cached tokens, and partly before position 0, whose queries and gates hold NaN and infinities: alone, beside others, and
+    where keys are split and joined."""
+    d = R.inputs(61, new, ctx, 8, 2, D, int8=int8, gate=True)
+    none = torch.zeros(sum(new), dtype=torch.bool)
+    for lo, m, all_ in R.batch(d):
+        none[lo:lo + max(m - all_, 0)] = True
+    want = R.attend(d)
+    assert none.any() and (want[0][none] == 0).all()
+    for bad in (NAN, INF, -INF):
+        d["gate"][none] = d["q"][none] = bad
+        for longest in (None, max(new)):
+            out = attend(R.cuda(d), longest=longest)
+            assert (out.cpu()[none] == 0).all(), bad
+            R.near(out, *want)
