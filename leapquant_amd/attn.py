@@ -12,8 +12,9 @@ A ragged batch is given by `loc` [N + 1] (sequence n holds the packed new tokens
 tokens of each sequence with the new ones, which are the last of them, and `table` [N, width]: token t of sequence n is at t %
 page in page table[n, t // page].  New tokens before a sequence's position 0 (all of them where lens is 0: padding) have outputs of
 zero, whatever their inputs hold, and write nothing; rows that no sequence holds are left as they are.  A table entry outside
-the cache is not written; it reads page 0.  Calls launch on the current stream of their tensors' device, never synchronise and can
-be captured in a graph; they work forward only (no autograd).
+the cache is not written; it reads page 0.  The three are int32; other integer types are converted in each call, far values held to
+int32's range.  Calls launch on the current stream of their tensors' device, never synchronise and can be captured in a graph;
+they work forward only (no autograd).
 """
 import typing
 

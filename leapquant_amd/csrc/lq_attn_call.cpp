@@ -95,13 +95,22 @@ void apart(const lq_rows& r, long long T, long long H, long long D) {
   if (!ok) raise(PyExc_ValueError, "out: heads that overlap each other (strides %lld, %lld)", r.ld, r.hd);
 }
 
+// Integers of another type as int32.  Wider ones are held to its range, where the kernels take them for what they are: outside the
+// cache, or past the last token.  (As they are, 2^32 would become page 0.)
+at::Tensor narrowed(const at::Tensor& t) {
+  const auto type = t.scalar_type();
+  if (type != at::kLong && type != at::ScalarType::UInt32 && type != at::ScalarType::UInt64) return t.to(at::kInt).contiguous();
+  at::Tensor wide = t.to(at::kLong);
+  if (type == at::ScalarType::UInt64) wide = wide.masked_fill(wide.lt(0), 0x7fffffff);          // 2^63 and more
+  return wide.clamp(-0x80000000ll, 0x7fffffffll).to(at::kInt).contiguous();
+}
 // an int32 index tensor; other integer types are converted
 at::Tensor index(const at::Tensor& t, const Device& dev, long long n, const char* name) {
   dev.on(t, name);
   if (t.dim() != 1 || t.size(0) != n) raise(PyExc_ValueError, "%s: 1-D with %lld elements expected, got shape %s", name, n, shape_of(t).c_str());
   if (t.scalar_type() == at::kInt && t.is_contiguous()) return t;
   if (!at::isIntegralType(t.scalar_type(), false)) raise(PyExc_TypeError, "%s: integers expected, got %s", name, type_of(t).c_str());
-  return t.to(at::kInt).contiguous();
+  return narrowed(t);
 }
 
 struct Batch {
@@ -116,7 +125,7 @@ Batch batch(PyObject* table, PyObject* loc, PyObject* lens, const Device& dev, l
   if (!at::isIntegralType(t.scalar_type(), false)) raise(PyExc_TypeError, "table: integers expected, got %s", type_of(t).c_str());
   const long long N = t.size(0), width = t.size(1);
   if (N >= 0x7fffffff || T >= 0x7fffffff || width >= 0x7fffffff) raise(PyExc_ValueError, "at most 2^31 - 2 sequences, tokens and pages a sequence");
-  r.table = t.scalar_type() == at::kInt && (width < 2 || t.stride(1) == 1) ? t : t.to(at::kInt).contiguous();
+  r.table = t.scalar_type() == at::kInt && (width < 2 || t.stride(1) == 1) ? t : narrowed(t);
   r.loc = index(tensor(loc, "loc"), dev, N + 1, "loc");
   r.lens = index(tensor(lens, "lens"), dev, N, "lens");
   r.b = {(const int*)r.loc.data_ptr(), (const int*)r.lens.data_ptr(), (const int*)r.table.data_ptr(), N < 2 ? width : r.table.stride(0),

@@ -617,3 +617,47 @@ def test_padding_is_zero_whatever_its_gate_holds(new, ctx, D, int8):
             out = attend(R.cuda(d), longest=longest)
             assert (out.cpu()[none] == 0).all(), bad
             R.near(out, *want)
+
+
+# ---- indexes of other integer types ------------------------------------------------------------------------------------------
+def test_wide_indexes_do_not_wrap():
+    """int64 tables, offsets and lengths past 32 bits are held to what there is, as those within."""
+    far = 2 ** 32
+    d = R.inputs(62, [5, 40, 3], [30, 60, 20], 4, 2, 128)
+    d["table"] = d["table"].long()
+    d["table"][0, 1], d["table"][1, 3], d["table"][1, 0], d["table"][2, 1] = far + 1, -far + 1, -2 ** 63, 2 ** 63 - 1
+    d["loc"] = torch.tensor([-far, 5, 45, far + 46])          # the last one to T
+    d["lens"] = torch.tensor([30, far + 7, -far + 20])        # all that the table has; none
+    check_attend(d)
+    check_rope(d)
+    small = R.inputs(63, [5, 3], [30, 20], 4, 2, 128)
+    for t in (torch.uint8, torch.int16, torch.uint16, torch.uint32, torch.uint64):
+        check_attend(dict(small, table=small["table"].to(t), loc=small["loc"].to(t), lens=small["lens"].to(t)))
+    for t, n in ((torch.uint32, 2 ** 32 - 1), (torch.uint64, 2 ** 64 - 5)):
+        d = R.inputs(63, [5, 3], [30, 20], 4, 2, 128)
+        g = R.cuda(d)
+        d["table"][0, 1], d["lens"][1], d["loc"][2] = -1, 10 ** 9, 10 ** 9
+        for x, at in (("table", (0, 1)), ("lens", 1), ("loc", 2)):
+            g[x] = g[x].to(t)
+            g[x][at] = torch.tensor(n, dtype=t)
+        R.near(attend(g), *R.attend(d))
+
+
+def test_wide_indexes_in_a_graph():
+    """A captured call converts the indexes at every replay."""
+    d = R.inputs(64, [1, 40], [300, 60], 4, 2, 128)
+    g = R.cuda(d)
+    for x in ("table", "loc", "lens"):
+        g[x] = g[x].long()
+    attend(g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(g)
+    for n in (300, 170, 2 ** 33):
+        g["lens"][0] = n
+        g["out"].fill_(5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        d["lens"][0] = min(n, 10 ** 9)
+        R.near(g["out"], *R.attend(d))
