@@ -79,7 +79,7 @@ typedef struct lq_attention {
   lq_rows q, gate, out;
   int HQ;
   int window;
-  float scale;            /* positive */
+  float scale;            /* positive, below 2^127 */
 } lq_attention;
 int lq_attend(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest, void* work, long long work_bytes,
               void* stream);

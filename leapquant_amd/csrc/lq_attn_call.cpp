@@ -275,7 +275,7 @@ PyObject* attend(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     a.HQ = (int)HQ;
     const double scale = arg[6] == Py_None ? 1.0 / std::sqrt((double)D) : number(arg[6], "scale");
     a.scale = (float)scale;
-    if (!(a.scale > 0.f) || std::isinf(a.scale)) raise(PyExc_ValueError, "scale: positive and finite expected");
+    if (!(a.scale > 0.f) || a.scale >= 0x1p127f) raise(PyExc_ValueError, "scale: positive and below 2^127 expected");
     const long long window = integer(arg[7], "window"), longest = arg[9] == Py_None ? 0 : integer(arg[9], "longest");
     if (window < 0 || window > 0x7fffffff) raise(PyExc_ValueError, "window: 0 (none) or a number of tokens expected, got %lld", window);
     if (longest < 0) raise(PyExc_ValueError, "longest: a number of tokens expected, got %lld", longest);

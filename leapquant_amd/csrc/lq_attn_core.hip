@@ -1193,7 +1193,7 @@ template <typename F> auto by_shape(const lq_pages* p, F f) {
 
 int check(const lq_attention* a, const lq_pages* p, const lq_batch* b, int longest) {
   if (!a || !pages_ok(p) || !batch_ok(b, p) || longest < 0) return LQ_ERR_ARG;
-  if (a->HQ <= 0 || a->HQ % p->HK || a->window < 0 || !(a->scale > 0.f) || a->scale > 3.4e38f) return LQ_ERR_ARG;
+  if (a->HQ <= 0 || a->HQ % p->HK || a->window < 0 || !(a->scale > 0.f) || a->scale >= 0x1p127f) return LQ_ERR_ARG;      // times log2(e) in fp32
   if (b->N == 0 || b->T == 0) return LQ_OK;
   if (!rows_ok(a->q) || !rows_ok(a->gate) || !rows_ok(a->out) || !a->q.p || !a->out.p) return LQ_ERR_ARG;
   if (!rows_apart(a->out, b->T, a->HQ, p->D)) return LQ_ERR_ARG;

@@ -270,3 +270,17 @@ def test_a_call_with_other_arguments_does_not_reach_the_tensors():
         for args in ((), (1,), (None,) * 14, (None,) * 10):
             with pytest.raises(TypeError):
                 f(*args)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, 3e38])
+def test_attend_refuses_scales_that_leave_32_bits(lib, scale):
+    """The kernels take scale times log2(e) in fp32; just below the border it is finite."""
+    assert _call(lib, a=_attention(scale=scale), b=_batch(**FULL)) == -1
+    assert lib.lq_attend_workspace(*(ctypes.byref(x) for x in (_attention(scale=1.7e38), _pages(), _batch(**FULL))), 0) >= 0
+    d = _args()
+    d["attend"] = dict(scale=scale)
+    with pytest.raises(ValueError, match="2\\^127"):
+        _both(d)[1]()
+    d["attend"] = dict(scale=1.7e38)
+    with pytest.raises(ValueError, match="GPU tensors only"):
+        _both(d)[1]()
