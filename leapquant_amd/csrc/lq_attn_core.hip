@@ -63,17 +63,12 @@ __device__ __forceinline__ void load16(const char* base, uint32_t off, const cha
 }
 // N of them, the j-th with an immediate of 1024 j bytes on both its address and its place
 template <int N> __device__ __forceinline__ void load16s(const char* base, const uint32_t (&off)[N], const char* lds) {
-  static_assert(N == 1 || N == 2 || N == 4 || N == 8, "loads of a wave");
+  static_assert(N == 2 || N == 4, "loads of a wave");          // an immediate has 12 bits
   const unsigned to = (unsigned)(size_t)(const lds_t*)lds;
-  if constexpr (N == 1)
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0" :: "s"(base), "s"(to), "v"(off[0]) : "memory", "m0");
-  else if constexpr (N == 2)
+  if constexpr (N == 2)
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024"
                  :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]) : "memory", "m0");
-  else if constexpr (N == 8) {                                 // an immediate has 12 bits: the j-th of 1024 (j & 3)
-    load16s<4>(base, {off[0], off[1], off[2], off[3]}, lds);
-    load16s<4>(base, {off[4], off[5], off[6], off[7]}, lds + 4096);
-  } else
+  else
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %2, %0\n\tglobal_load_lds_dwordx4 %3, %0 offset:1024\n\t"
                  "global_load_lds_dwordx4 %4, %0 offset:2048\n\tglobal_load_lds_dwordx4 %5, %0 offset:%6"
                  :: "s"(base), "s"(to), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "n"(3 * 1024) : "memory", "m0");
@@ -609,8 +604,8 @@ template <class S> struct Tiles {
   static constexpr int D = S::D, KT = S::KT, OWN = S::OWN, ES = S::I8 ? 1 : 2, CPR = D * ES / 16, RPL = 64 / CPR;
   static constexpr int LOADS = OWN / RPL > 0 ? OWN / RPL : 1;
   static_assert(S::I8 || OWN % RPL == 0, "a load of a whole wave");
-  // The j-th load's immediate, 1024 (j & 3), moves its place in LDS and its address: the offsets are that much less, and the bases
-  // 4096 less.
+  // The j-th load's immediate, 1024 j, moves its place in LDS and its address: the offsets are that much less, and, so that none is
+  // below 0, the bases 4096 less.
   static constexpr int LESS = S::I8 ? 0 : 4096;
   const_int* tab;
   const char* kbase;
@@ -644,7 +639,7 @@ template <class S> struct Tiles {
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int k = min(RPL * j + lane / CPR, OWN - 1), tk = rw * OWN + k;
-      const uint32_t off = (uint32_t)k * row_bytes + LESS - (S::I8 ? 0 : 1024 * (j & 3));
+      const uint32_t off = (uint32_t)k * row_bytes + LESS - (S::I8 ? 0 : 1024 * j);
       koff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_k(tk));
       voff[j] = off + 16 * (S::I8 ? lane % CPR : (lane % CPR) ^ S::place_v(tk));
     }
