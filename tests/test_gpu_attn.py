@@ -661,3 +661,49 @@ def test_wide_indexes_in_a_graph():
         torch.cuda.synchronize()
         d["lens"][0] = min(n, 10 ** 9)
         R.near(g["out"], *R.attend(d))
+
+
+# ---- layouts ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("new,ctx", [([1, 3], [400, 90]), ([70, 1], [200, 90])])
+def test_layouts_of_pages_and_tables(new, ctx):
+    """Codes and scales by head, scales beside each other in one tensor, a table that is a column range of a wider one."""
+    d = R.inputs(65, new, ctx, 8, 2, 128, page=32, int8=True)
+    NP, page, HK, D = d["kp"].shape
+    g = R.cuda(d)
+    codes = torch.stack([g["kp"], g["vp"]], 1).transpose(2, 3).contiguous()              # [pages, 2, heads, page, D]
+    scales = torch.zeros(HK, NP, 2, page, 3, device="cuda")
+    for i, x in enumerate(("k", "v")):
+        g[x + "p"] = codes[:, i].transpose(1, 2)
+        s = scales[:, :, i, :, 1].permute(1, 2, 0)                                        # head-major, three floats apart
+        s.copy_(g[x + "s"])
+        g[x + "s"] = s
+    wide = torch.full((len(new), d["table"].shape[1] + 5), 2 ** 30, dtype=torch.int32, device="cuda")
+    wide[:, 2:-3] = g["table"]
+    g["table"] = wide[:, 2:-3]
+    assert g["table"].stride(0) > g["table"].shape[1]
+    for longest in (None, max(new)):
+        R.near(attend(g, longest=longest), *R.attend(d))
+    check_rope(d, g)
+    assert (scales[..., 0] == 0).all() and (scales[..., 2] == 0).all()
+
+
+def test_8_bit_pages_past_32_bit_offsets():
+    """Codes of more than 2^32 bytes and scales beside them: the last pages."""
+    NP, page, HK, D = 140000, 16, 8, 256
+    d = R.inputs(66, [1, 40, 3], [90, 80, 3], 16, 8, 256, int8=True)
+    g = R.cuda(d)
+    few = d["kp"].shape[0]
+    for x in ("kp", "vp", "ks", "vs"):
+        big = torch.zeros((NP,) + tuple(d[x].shape[1:]), device="cuda", dtype=d[x].dtype)
+        big[NP - few:] = g[x]
+        g[x] = big
+    assert g["kp"].numel() > 2 ** 32
+    g["table"] = g["table"] + NP - few
+    R.near(attend(g), *R.attend(d))
+    rope(g)
+    last = {x: g[x][NP - few:].cpu() for x in ("kp", "vp", "ks", "vs")}
+    assert not any(g[x][:NP - few].any() for x in ("kp", "vp"))
+    for t, p, o in R.rope(d)[2]:
+        w = d["v"][t].to(F64)
+        s = last["vs"][p, o].to(F64)[:, None]
+        assert not ((last["vp"][p, o].to(F64) * s - w).abs() > 0.5 * s * (1 + 2.0 ** -10) + 2.0 ** -17 * w.abs().amax(-1, keepdim=True)).any()
