@@ -707,3 +707,18 @@ def test_8_bit_pages_past_32_bit_offsets():
         w = d["v"][t].to(F64)
         s = last["vs"][p, o].to(F64)[:, None]
         assert not ((last["vp"][p, o].to(F64) * s - w).abs() > 0.5 * s * (1 + 2.0 ** -10) + 2.0 ** -17 * w.abs().amax(-1, keepdim=True)).any()
+
+
+# ---- more sequences than a wave has lanes -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("N", [65, 150, 4200])
+def test_many_sequences(N):
+    """The search for a token's and a row tile's sequence takes two and three steps; empty sequences, padding, a few longer ones."""
+    gen = torch.Generator().manual_seed(N)
+    new = torch.randint(0, 3, (N,), generator=gen).tolist()
+    ctx = [m + int(x) for m, x in zip(new, torch.randint(0, 20, (N,), generator=gen))]
+    for n in (0, N // 2, N - 1):
+        new[n], ctx[n] = 70, 90
+    ctx[3] = ctx[N - 2] = 0
+    for longest in (None, 70):
+        check_attend(R.inputs(67, new, ctx, 2, 1, 64, extra=2), longest=longest)
+    check_rope(R.inputs(68, new, ctx, 2, 1, 64, extra=2))
