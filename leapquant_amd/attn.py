@@ -49,6 +49,7 @@ def attend(q, pages, table, loc, lens, out, scale=None, window=0, gate=None, lon
 
     q, out, gate: bf16 [T, HQ, D], any token and head strides divisible by 16 bytes; out may be q.  HQ is a multiple of the pages'
     heads; head h reads head h // (HQ / HK).  scale: positive (below 2^127), D^-1/2 by default.  longest: new tokens of the longest
-    sequence where the host knows them (a host integer, which decides on speed only).  What a token does not see, infinities and NaN
+    sequence where the host knows them (a host integer, which decides on speed only; decode batches without it take up to 1.6 times as
+    long).  A table no wider than the batch needs saves short contexts a launch.  What a token does not see, infinities and NaN
     among it, does not reach its output."""
     _lib.attn_call().attend(q, pages, table, loc, lens, out, scale, window, gate, longest)

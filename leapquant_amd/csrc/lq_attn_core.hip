@@ -344,9 +344,9 @@ __device__ __forceinline__ void store1(const lq_attention& a, long long token, i
 // each by itself: K and V of a tile have a place in LDS each, and the next tile's are asked for as soon as this one's are used, so
 // that 32 D .. 64 D elements a wave are on their way at any time.  Codes stay codes in LDS.
 //
-// Measured (MI355X): 64 sequences up to 8192 of 8 heads of 128 255 us, 5.2 TB/s, a large copy's rate; from codes 170 us, 4.0 TB/s,
-// beside the conversion of the codes.  One sequence of 8192, 2 heads of 256: 10 us and 5 for the join, chains of
-// loads.  Workgroups of 32 or 64 rows of this kind lose to tiles of many rows (32 sequences of up to 64 rows, 2 heads of 256,
+// Measured (MI355X): 64 sequences up to 8192 of 8 heads of 128 256 us, 5.2 TB/s, a large copy's rate (reads alone reach 6.3 by plain
+// loads, 7.2 by nontemporal ones); from codes 168 us, 4.1 TB/s, beside the conversion of the codes.  One sequence of 8192, 2 heads of
+// 256: 10 us and 5 for the join, chains of loads.  Workgroups of 32 or 64 rows of this kind lose to tiles of many rows (32 sequences of up to 64 rows, 2 heads of 256,
 // 75 us against 58; one of 48 rows over 16384, 8 heads of 128, 44 against 23): their queries no longer fit beside the outputs, and one wave a SIMD shows every wait.
 template <int D_, int KW_, bool I8_> struct Few {
   static constexpr int D = D_, KW = KW_, R = 16, ROWS = 16, KT = 32, LEAST = KW, THREADS = 64 * KW;
@@ -581,9 +581,9 @@ __global__ __launch_bounds__(S::THREADS) void few_kernel(lq_attention a, lq_page
 // instructions go in the shadow of its matrix instructions.  What bounds it then is the number of a wave's instructions.
 // Codes go through registers and into LDS as bf16, which holds them exactly; scales enter S and P in fp32.
 //
-// Measured (MI355X): a prompt of 8192, 32 / 8 heads of 128, 535 us, 1.03 PFLOP/s (a large product by the library 1.31): its clock falls to
-// 1.5 .. 1.95 GHz; a piece of 2048 over 32768, 16 / 2 heads of 256, 1100 us, 0.98 PFLOP/s, one wave a SIMD; 4096 from codes of 32 / 8 of 128
-// 289 us.  Without the order of instructions below 584 and 2184; without queries waited for before the loop 573 and 1344.
+// Measured (MI355X): a prompt of 8192, 32 / 8 heads of 128, 520 .. 535 us, 1.03 .. 1.06 PFLOP/s (a large product by the library 1.31): its clock falls to
+// 1.5 .. 1.95 GHz; a piece of 2048 over 32768, 16 / 2 heads of 256, 1095 .. 1120 us, 0.95 .. 0.97 PFLOP/s, one wave a SIMD; 4096 tokens of 32 / 8
+// of 128 145 us, from codes 257.  Without the order of instructions below 584 and 2184; without queries waited for before the loop 573 and 1344.
 template <int D_, int RW_, int KT_, int EU_, bool I8_> struct Many {
   static constexpr int D = D_, RW = RW_, EU = EU_, KT = KT_, X = KT / 32, LEAST = 512 / KT, R = 32, ROWS = 32 * RW, THREADS = 64 * RW;
   static constexpr bool I8 = I8_;
@@ -1086,7 +1086,7 @@ __global__ __launch_bounds__(256) void join_kernel(lq_attention a, lq_pages pg, 
 template <int D, bool I8> struct Shapes {
   typedef Few<D, 4, I8> F;
   // Tiles of 64 keys, or 32 where 64 do not fit the registers: heads of 256 and codes (prompt of
-  // 8192 of heads of 128 573 -> 563 us by 64; 4096 from codes 666, spilled, -> 258 by 32).  Heads of 256 hold 32 rows of outputs in half the registers of
+  // 8192 of heads of 128 573 -> 563 us by 64; 4096 from codes 666, spilled, -> 257 by 32).  Heads of 256 hold 32 rows of outputs in half the registers of
   // a SIMD: one wave there.
   typedef Many<D, 4, !I8 && D <= 128 ? 64 : 32, D == 256 ? 1 : 2, I8> M;
 };
@@ -1115,11 +1115,15 @@ template <int D, bool I8> Plan plan_of(const lq_attention* a, const lq_pages* p,
   // to 8192 do at 5.2 TB/s.  Beside longer ones that is worth a second kind of workgroup only if the others are short by the mean (us,
   // with it / without): 32 sequences of up to 8 tokens, 8 heads a key head of 256 95 / 65, 5 of up to 777 under a window 19.5 / 19.4.
   // A piece of 449 tokens beside 15 of one token, 4 heads a key head: 86 with it; without, a tile of 128 rows for 4.
+  // Without the hint any sequence may be the long one: both kinds are launched, the few one with the other's registers and fewer pieces (us,
+  // said / not said: 64 single tokens up to 8192 of 8 heads of 128 257 / 345, from codes 169 / 273, 32 of up to 8 tokens up to 4099 of 2
+  // of 256 58 / 87).
   const bool hint = longest > 0 && longest < b->T, many = rows > F::ROWS;
   const bool few = !many || (b->N > 1 && (!hint || (b->T - most) * c.G <= (long long)F::ROWS * (b->N - 1)));
   c.few = few ? F::ROWS : 0;
   c.tiles = many ? (int)((long long)b->T * c.G / M::ROWS + b->N) : 0;
-  // keys that a row tile sees at most; under a window of its rows' tokens
+  // keys that a row tile sees at most, by the table's width; under a window of its rows' tokens.  Short contexts under a wide table get a
+  // join with nothing to join (us, as wide as needed / 4096 pages: 64 single tokens at 200 of 8 heads of 128 10.6 / 15.8, at 1000 39 / 47).
   auto reach = [&](int tile) {
     const long long all = (long long)b->width * p->page, near = (long long)a->window + (tile - 1) / c.G + 1;
     return a->window > 0 && near < all ? near : all;

@@ -13,7 +13,8 @@
 // then a wave takes GROUP heads of all of them at a time, their loads on their way together, the weights loaded once.
 // Few: a workgroup takes one token, a wave GROUP heads of it, and each lane forms its own angles: no barrier in the chain.
 //
-// Measured (MI355X): 41530 tokens of 16 + 2 + 2 heads of 256 175 us (4.9 TB/s; a large copy 5.2), 8192 of 16 + 8 + 8 of 128 32 us
+// Measured (MI355X): 41530 tokens of 16 + 2 + 2 heads of 256 175 us (4.9 TB/s; a large copy 5.2), into
+// 8-bit pages 177, 8192 of 16 + 8 + 8 of 128 32 us
 // (4.2 TB/s); a wave's 159 vector instructions for 64 x 8 elements are the next bound.  A decode batch of 64 tokens 5 us: its chain of
 // three loads and the launch.  Per wave 4 tokens at a time 192 us, 16 at a time in two halves 191, 128 threads 196, 512 209.
 #include "lq_attn.h"

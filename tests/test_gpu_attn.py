@@ -707,6 +707,8 @@ def test_8_bit_pages_past_32_bit_offsets():
         w = d["v"][t].to(F64)
         s = last["vs"][p, o].to(F64)[:, None]
         assert not ((last["vp"][p, o].to(F64) * s - w).abs() > 0.5 * s * (1 + 2.0 ** -10) + 2.0 ** -17 * w.abs().amax(-1, keepdim=True)).any()
+    del g, big                                # what lasts of later tests would lie in these segments and keep them
+    torch.cuda.empty_cache()
 
 
 # ---- more sequences than a wave has lanes -------------------------------------------------------------------------------------
